@@ -17,7 +17,7 @@ from pathlib import Path
 import torch  # noqa: F401  -- must be loaded before the HIP library, see module docstring
 
 LIB_PATH = Path(__file__).resolve().parent / "liboudjat_hip.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 OK = 0
 STATUS_NAMES = {
@@ -47,6 +47,11 @@ FUSION_GEO_MEAN = 4
 IMPORTANCE_L2 = 0
 IMPORTANCE_ENERGY = 1
 IMPORTANCE_RMS = 2
+DTYPE_BF16 = 0
+DTYPE_FP16 = 1
+POS_I32 = 0
+POS_I64 = 1
+POS_F32 = 2
 
 
 class OudjatUnavailable(RuntimeError):
@@ -156,12 +161,21 @@ SIGNATURES: dict[str, list] = {
     "oudjat_scale_bias_rows": [_p, _i64, _i64, _i64, _f32, _p, _p, _p, _i64, _p],
     "oudjat_swiglu_scaled": [_p, _f32, _p, _p, _f32, _p, _i64, _i64, _p, _p],
     "oudjat_amax_update": [_p, _i64, _i64, _i64, _p, _p],
+    "oudjat_packed_plan": [_p, _i32, _p, _i32, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _p, _p],
+    "oudjat_rope_axes": [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _p, _i32, _i64, _i64, _i64, _p,
+                         _p, _p, _i64, _i64, _p, _i64, _i64, _p],
+    "oudjat_qk_norm_rope_kv": [_p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p, _p, _p, _p, _f32, _p, _i32, _i64, _i64,
+                               _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p],
+    "oudjat_packed_attention": [_p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64,
+                                _i64, _i32, _p, _i32, _p, _i32, _i64, _f32, _i32, _i32, _p, _i64, _p, _i64, _p],
+    "oudjat_packed_attention_workspace_elems": [_i64, _i64, _i64, _i64, _i64],
     "oudjat_query_attention_prob_noalloc": [_p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _p,
                                             _i64, _i32, _p],
 }
 _RESTYPES = {"oudjat_status_string": ctypes.c_char_p, "oudjat_last_error": ctypes.c_char_p,
              "oudjat_linear_workspace_elems": ctypes.c_int64, "oudjat_linear_warm_slots": ctypes.c_int64,
              "oudjat_sparse_query_attention_workspace_elems": ctypes.c_int64,
+             "oudjat_packed_attention_workspace_elems": ctypes.c_int64,
              "oudjat_patch_attention_prob_workspace_elems": ctypes.c_int64}
 
 _lock = threading.Lock()

@@ -737,6 +737,75 @@ int oudjat_swiglu_scaled(const uint16_t* x1, float s1, const uint16_t* b1, const
 int oudjat_amax_update(const uint16_t* x, int64_t M, int64_t K, int64_t stride_m, float* amax,
                        oudjat_stream_t stream);
 
+/* ---- Packed sequences: rows of sequences of different lengths, one after another ------------------------
+ * None of these has a counterpart in the reference, whose token rows are rectangular (images of a batch share one
+ * length; threshold plans are padded to the longest, block.py:492-621). Element types: OUDJAT_BF16 or OUDJAT_FP16
+ * bit patterns as uint16_t, one type per call. */
+enum oudjat_dtype { OUDJAT_BF16 = 0, OUDJAT_FP16 = 1 };
+/* Type of a position tensor. */
+enum oudjat_pos { OUDJAT_POS_I32 = 0, OUDJAT_POS_I64 = 1, OUDJAT_POS_F32 = 2 };
+
+/* Row offsets, key lengths and cache slots of S sequences from their lengths (device arrays; *_wide: int64, else
+ * int32). q_lens[s] new rows, k_lens[s] keys with these among them. Negative lengths count as 0.
+ *   cu_q [S + 1] int32: cu_q[s + 1] = min(q_lens[0] + .. + q_lens[s], rows);
+ *   k_out [S] int32: the key lengths, each cut to key_cap (a cache of key_cap tokens per sequence), or, with
+ *     packed_keys, their running sum cut to key_cap (key rows packed like the queries); cu_k [S + 1] int64 the
+ *     running sum;
+ *   batch_idx, token_idx [rows] int64: row r of sequence s is token k_out[s] - cu_q[s + 1] + r of it (a sequence's
+ *     new rows are its last tokens); -1, -1 for rows past the last sequence and where that token is negative.
+ * At most 4096 sequences; row maps 16-byte aligned. */
+int oudjat_packed_plan(const void* q_lens, int q_wide, const void* k_lens, int k_wide, int64_t S, int64_t rows,
+                       int64_t key_cap, int packed_keys, int32_t* cu_q, int32_t* k_out, int64_t* cu_k,
+                       int64_t* batch_idx, int64_t* token_idx, oudjat_stream_t stream);
+
+/* Rotate-half rotation of q [rows, Hq, Dh] and k [rows, Hk, Dh] (row and head strides) by positions with several
+ * axes: with R / 2 the sum of `sections` (host array, one entry per axis: how many consecutive frequencies it
+ * has), dims (i, i + R/2), i < R/2, of row m turn by pos[m, axis of i] * inv_freq[i] radians (formed in 64 bits);
+ * dims from R on are copied. fp32 arithmetic, one rounding. pos [rows, axes] with strides pos_rs, pos_as of type
+ * oudjat_pos, 1 to 4 axes. The outputs may be the inputs (in place) but not overlap them otherwise. Hq or Hk may
+ * be 0. Dh % 16 == 0, Dh <= 512; R / 2 a multiple of 8; 16-byte aligned rows and heads. */
+int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, const uint16_t* k, int64_t k_rs, int64_t k_hs,
+                     int64_t rows, int64_t Hq, int64_t Hk, int64_t Dh, int dtype, const void* pos, int pos_kind,
+                     int64_t pos_rs, int64_t pos_as, int64_t axes, const float* inv_freq, const int64_t* sections,
+                     uint16_t* q_out, int64_t qo_rs, int64_t qo_hs, uint16_t* k_out, int64_t ko_rs, int64_t ko_hs,
+                     oudjat_stream_t stream);
+
+/* qkv rows [rows, Hq + 2 Hk, Dh] (row stride x_rs: query, key, value heads) in one pass: every query and key head
+ * normed over its Dh values (x / sqrt(mean(x^2) + eps) * w; layer_norm: x - mean(x) for x, and + b; w and b of
+ * Dh values or NULL), rotated as in oudjat_rope_axes, rounded once; queries to q_out [rows, Hq, Dh] (row stride
+ * qo_rs), keys and (unchanged) values to kv + batch * kv_bs + token * kv_ns (+ kv_cs for values), Hk x Dh packed.
+ * Rows whose (batch, token) lies outside B x N are skipped: neither q_out nor the cache is written for them. The
+ * slots of the other rows must be unique. Dh 64 or 128; 16-byte aligned rows. */
+int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t rows, int64_t Hq, int64_t Hk, int64_t Dh,
+                           int dtype, int layer_norm, const uint16_t* q_weight, const uint16_t* q_bias,
+                           const uint16_t* k_weight, const uint16_t* k_bias, float eps, const void* pos, int pos_kind,
+                           int64_t pos_rs, int64_t pos_as, int64_t axes, const float* inv_freq,
+                           const int64_t* sections, const int64_t* batch_idx, const int64_t* token_idx, uint16_t* kv,
+                           int64_t kv_bs, int64_t kv_ns, int64_t kv_cs, int64_t B, int64_t N, uint16_t* q_out,
+                           int64_t qo_rs, oudjat_stream_t stream);
+
+/* Grouped-head attention of packed query rows over the keys of their own sequences. Query head h reads key head
+ * h / (Hq / Hk). Sequence s has query rows cu_q[s] .. cu_q[s + 1] - 1 (int32, or int64 if cu_wide; cut to 0 .. rows)
+ * of q [rows, Hq, Dh] and n_s keys:
+ *   batched: keys (s, 0 .. n_s - 1) of k, v [>= S, key_cap, Hk, Dh] (strides k_bs, k_rs, k_hs and the same for v),
+ *            n_s = keys[s] cut to 0 .. key_cap;
+ *   packed:  rows keys[s] .. keys[s + 1] - 1 of k, v [key_cap, Hk, Dh] (k_bs, v_bs unused), cut to 0 .. key_cap.
+ *   (keys: int32, or int64 if keys_wide.)
+ * out[r, h*Dh..] = softmax(q . K^T * scale) . V in fp32 with the probabilities rounded to the type; causal: row i of
+ * a sequence's m sees keys 0 .. n_s - m + i (the last row sees all). A row that sees no key is 0; hidden keys and
+ * values have no influence whatever they hold; rows past the last sequence are not written.
+ * Where one workgroup per tile of query rows would leave CUs idle, the keys are split over several and merged by a
+ * second launch (in part order): workspace of oudjat_packed_attention_workspace_elems fp32 elements, 16-byte
+ * aligned, else OUDJAT_ERR_INVALID_ARGUMENT. Deterministic. Dh 64 or 128; scale > 0 and finite; 16-byte aligned
+ * rows and heads of q, k, v, 8-byte aligned of out; strides not negative. */
+int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64_t rows, int64_t Hq, int64_t Dh,
+                            const uint16_t* k, int64_t k_bs, int64_t k_rs, int64_t k_hs, const uint16_t* v,
+                            int64_t v_bs, int64_t v_rs, int64_t v_hs, int64_t Hk, int64_t key_cap, int batched,
+                            const void* cu_q, int cu_wide, const void* keys, int keys_wide, int64_t S, float scale,
+                            int causal, int dtype, uint16_t* out, int64_t out_rs, float* workspace,
+                            int64_t workspace_elems, oudjat_stream_t stream);
+int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh);
+
 #ifdef __cplusplus
 }
 #endif
