@@ -1,18 +1,38 @@
 // Grouped-head attention of packed query rows over the keys of their own sequences, causal or not.
 //
-// Row r of sequence s (m rows, n keys) sees the keys j < n (causal: j <= n - m + i for its i-th row):
-//   out = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * (q . k_j) - max_j ...)
-// with the running maximum and sum of an online softmax in fp32. Hidden keys are not read, so whatever they hold
-// has no influence; a row that sees none is 0.
+// A sequence of m rows and n keys: its row i sees the keys j < n (causal: j <= n - m + i),
+//   out = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c (q . k_j) - c mu),  c = scale log2 e,
+// with an online softmax: mu is a reference that follows the running maximum, and sum and output are rescaled when it
+// moves. Scores, statistics and outputs are fp32; the p_j are rounded to the element type for the second product, and
+// the sum is of the rounded values, so that numerator and normaliser use the same weights.
 //
-// One wave per (row, query head): 64 keys at a time, a key per lane for the scores, then Dh / 64 dims per lane for
-// the values.
+// The G query heads of a key head are packed into the query rows: packed row r of a sequence is token r / G, head
+// r % G of the group, so that one pass over a key head's K and V serves the whole group, a single token fills G rows
+// of a tile, and a causal tile spans few tokens.
+//
+// Work is dealt by the sequences' lengths, which only the device knows: a workgroup is one (item, key head), item = (tile of
+// R packed rows, part of its keys); the items of all sequences are numbered one after another, a sequence's last tile
+// (the one with the most keys) first, and every wave finds its item by a scan over the lengths, 64 sequences at a
+// time (about a microsecond up to some hundreds of sequences, against a plan launch of 3 us per layer). The grid
+// is an upper bound from the numbers of rows and sequences; workgroups past the last item leave.
+//
+// Few items are split by keys (`split`): every part is left with about units / target key tiles, parts write their running
+// reference, sum and unnormalised rows to the workspace, and a second launch merges them in part order.
+//
+// Two kernels. packed_attn_rows: R = 32 W rows, a wave owns 32, all waves of the workgroup share K/V tiles of 64 keys.
+// packed_attn_keys, for few rows: R = 16, the four waves share the rows and take 32 keys each in turn.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
+#include "attn.hpp"
 #include "common.hpp"
 
 namespace oudjat {
+
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef short i16x8_t __attribute__((ext_vector_type(8)));
 
 struct PackedAttn {
   const uint16_t* q;
@@ -22,85 +42,873 @@ struct PackedAttn {
   const void *cu_q, *keys;
   uint16_t* out;
   int64_t o_rs;
-  int rows, S, Hq, G;
+  int rows, S, Hk, G;
   int key_cap;
-  bool cu_wide, keys_wide, batched, causal, fp16;
+  bool cu_wide, keys_wide, batched, causal;
   float scale_log2;
+  // Key parts: 0 = never split; else the number of parts that a key head's items are cut into at the most, beside
+  // their own number, and the fewest key tiles of a part.
+  int target, min_tiles;
+  int items;      // items a key head has at the most (the grid)
+  float* ws;      // parts, then the directory
+  int2* dir;      // [rows][Hq]: first item of the row's tile, its parts | row in the tile << 16
 };
 
-__device__ __forceinline__ int64_t load_idx(const void* p, int i, bool wide) {
-  return wide ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
+// Element types on the matrix cores.
+struct AttnBf16 {
+  typedef bf16x8_t v8;
+  static constexpr int kOne = 0x3f80, kExp = 0x7f80;
+  static __device__ __forceinline__ f32x16_t mfma32(v8 a, v8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4_t mfma16(v8 a, v8 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float sum8(v8 p, float acc) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    const v2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 0, 1), ones, acc, false);
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 2, 3), ones, acc, false);
+    acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 4, 5), ones, acc, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(p, p, 6, 7), ones, acc, false);
+  }
+  typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+};
+struct AttnFp16 {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  static constexpr int kOne = 0x3c00, kExp = 0x7c00;
+  static __device__ __forceinline__ f32x16_t mfma32(v8 a, v8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4_t mfma16(v8 a, v8 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float sum8(v8 p, float acc) {
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    const v2 ones = {(_Float16)1.0f, (_Float16)1.0f};
+    acc = __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 0, 1), ones, acc, false);
+    acc = __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 2, 3), ones, acc, false);
+    acc = __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 4, 5), ones, acc, false);
+    return __builtin_amdgcn_fdot2(__builtin_shufflevector(p, p, 6, 7), ones, acc, false);
+  }
+  typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+};
+
+template <class E>
+__device__ __forceinline__ typename E::v8 as8(const uint4& v) {
+  return __builtin_bit_cast(typename E::v8, v);
 }
-__device__ __forceinline__ int clamp_idx(int64_t v, int lo, int hi) {
-  return v < lo ? lo : (v > hi ? hi : (int)v);
-}
-__device__ __forceinline__ float elem(uint16_t x, bool fp16) {
-  return fp16 ? (float)__builtin_bit_cast(_Float16, x) : bf16_to_f32(x);
+template <class E>
+__device__ __forceinline__ typename E::v8 round8(const float* f) {
+  const f32x8_t v = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
+  return __builtin_convertvector(v, typename E::v8);
 }
 
-template <int DH>
-__global__ __launch_bounds__(256) void packed_attn_kernel(PackedAttn a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= (int64_t)a.rows * a.Hq) return;
-  const int row = (int)(unit / a.Hq), h = (int)(unit - (int64_t)row * a.Hq), hk = h / a.G;
-  int lo = 0, hi = a.S;
-  while (lo < hi) {  // first sequence that ends past the row
-    const int mid = (lo + hi) >> 1;
-    if (clamp_idx(load_idx(a.cu_q, mid + 1, a.cu_wide), 0, a.rows) > row) hi = mid;
-    else lo = mid + 1;
-  }
-  const int s = lo;
-  if (s >= a.S) return;
-  const int q0 = clamp_idx(load_idx(a.cu_q, s, a.cu_wide), 0, a.rows);
-  if (row < q0) return;
-  const int m = clamp_idx(load_idx(a.cu_q, s + 1, a.cu_wide), q0, a.rows) - q0;
-  int n, k0 = 0;
+__device__ __forceinline__ int load_idx(const void* p, int i, bool wide, int lo, int hi) {
+  const int64_t v = wide ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
+  return v < lo ? lo : (v > hi ? hi : (int)v);
+}
+
+// A sequence's rows and keys, and the item that a workgroup takes of it. Uniform over the wave.
+struct Item {
+  int seq, q0, m, n, k0;  // first row, rows, keys, first key row (packed keys)
+  int tile, part, parts;
+};
+
+// Sequence s: rows and keys, cut to the buffers.
+__device__ __forceinline__ void load_seq(const PackedAttn& a, int s, Item& t) {
+  t.q0 = load_idx(a.cu_q, s, a.cu_wide, 0, a.rows);
+  t.m = load_idx(a.cu_q, s + 1, a.cu_wide, t.q0, a.rows) - t.q0;
+  t.k0 = 0;
   if (a.batched) {
-    n = clamp_idx(load_idx(a.keys, s, a.keys_wide), 0, a.key_cap);
+    t.n = load_idx(a.keys, s, a.keys_wide, 0, a.key_cap);
   } else {
-    k0 = clamp_idx(load_idx(a.keys, s, a.keys_wide), 0, a.key_cap);
-    n = clamp_idx(load_idx(a.keys, s + 1, a.keys_wide), k0, a.key_cap) - k0;
+    t.k0 = load_idx(a.keys, s, a.keys_wide, 0, a.key_cap);
+    t.n = load_idx(a.keys, s + 1, a.keys_wide, t.k0, a.key_cap) - t.k0;
   }
-  const int lim = a.causal ? min(n, max(0, n - m + (row - q0) + 1)) : n;
-  const uint16_t* qp = a.q + (int64_t)row * a.q_rs + (int64_t)h * a.q_hs;
-  const uint16_t* kp = a.k + (a.batched ? (int64_t)s * a.k_bs : (int64_t)k0 * a.k_rs) + (int64_t)hk * a.k_hs;
-  const uint16_t* vp = a.v + (a.batched ? (int64_t)s * a.v_bs : (int64_t)k0 * a.v_rs) + (int64_t)hk * a.v_hs;
-  float o[DH / 64] = {}, mx = -INFINITY, l = 0.0f;
-  for (int j0 = 0; j0 < lim; j0 += 64) {
-    const int j = j0 + lane;
-    float sc = -INFINITY;
-    if (j < lim) {
-      sc = 0.0f;
-      const uint16_t* kr = kp + (int64_t)j * a.k_rs;
-      for (int d = 0; d < DH; ++d) sc = fmaf(elem(qp[d], a.fp16), elem(kr[d], a.fp16), sc);
-      sc *= a.scale_log2;
+}
+
+// Item number `item` of a key head, tiles of R packed rows and KT keys; false past the last. Parts of a sequence's
+// tiles: ceil(its key tiles / C), with C = max(min_tiles, units / target) and units the key tiles of all tiles, so
+// that a key head has at most its own tiles + target items.
+template <int R, int KT>
+__device__ __forceinline__ bool find_item(const PackedAttn& a, int item, Item& w) {
+  const int lane = threadIdx.x & 63;
+  Item t;
+  int chunk = 1 << 30;
+  auto tiles = [&](const Item& x) { return (int)(((int64_t)x.m * a.G + R - 1) / R); };
+  auto key_tiles = [&](const Item& x) { return (x.n + KT - 1) / KT; };
+  auto load = [&](int s0) {
+    t.q0 = t.m = t.n = t.k0 = 0;
+    if (s0 + lane < a.S) load_seq(a, s0 + lane, t);
+  };
+  load(0);
+  if (a.target) {
+    float units = (float)tiles(t) * (float)key_tiles(t);
+    for (int s0 = 64; s0 < a.S; s0 += 64) {
+      load(s0);
+      units += (float)tiles(t) * (float)key_tiles(t);
     }
-    const float m_new = fmaxf(mx, wave_max(sc)), ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = exp2f(mx - ref), p = exp2f(sc - ref);
-    l = l * alpha + wave_sum(p);
-    mx = m_new;
-    for (int e = 0; e < DH / 64; ++e) o[e] *= alpha;
-    const int here = min(64, lim - j0);
-    for (int i = 0; i < here; ++i) {
-      const float pi = __shfl(p, i, 64);
-      for (int e = 0; e < DH / 64; ++e)
-        o[e] = fmaf(pi, elem(vp[(int64_t)(j0 + i) * a.v_rs + e * 64 + lane], a.fp16), o[e]);
+    units = wave_sum(units);
+    chunk = max(a.min_tiles, (int)ceilf(units / (float)a.target));
+    if (a.S > 64) load(0);
+  }
+  int base = 0;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    if (s0) load(s0);
+    const int nt = tiles(t), kt = key_tiles(t);
+    const int parts = max(1, (kt + chunk - 1) / chunk);
+    const int mine = nt * parts;
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += up;
+    }
+    const int total = __builtin_amdgcn_readlane(incl, 63);
+    if (item < base + total) {
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + incl > item));
+      const int within = item - base - __builtin_amdgcn_readlane(incl - mine, l);
+      w.seq = s0 + l;
+      w.q0 = __builtin_amdgcn_readlane(t.q0, l);
+      w.m = __builtin_amdgcn_readlane(t.m, l);
+      w.n = __builtin_amdgcn_readlane(t.n, l);
+      w.k0 = __builtin_amdgcn_readlane(t.k0, l);
+      w.parts = __builtin_amdgcn_readlane(parts, l);
+      const int from_last = within / w.parts;
+      w.part = within - from_last * w.parts;
+      w.tile = __builtin_amdgcn_readlane(nt, l) - 1 - from_last;
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+// Keys that token i of the sequence sees.
+__device__ __forceinline__ int seen_keys(const PackedAttn& a, const Item& w, int i) {
+  return a.causal ? min(w.n, max(0, w.n - w.m + i + 1)) : w.n;
+}
+
+// Floats of one part: reference and sum of R rows, then R rows of DH.
+__host__ __device__ constexpr int64_t part_floats(int R, int DH) { return (int64_t)R * (DH + 2); }
+
+// V^T fragment with its infinities and NaNs taken out (0) and told apart: plus / minus hold 1 where the element is
+// +inf / -inf, both where it is NaN.
+template <class E>
+__device__ __forceinline__ void split_nonfinite(i16x8_t& v, i16x8_t& plus, i16x8_t& minus) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int b = (int)(uint16_t)v[e], mag = b & 0x7fff;
+    const bool bad = mag >= E::kExp, nan = mag > E::kExp;
+    v[e] = bad ? 0 : v[e];
+    plus[e] = bad && (nan || !(b & 0x8000)) ? (short)E::kOne : 0;
+    minus[e] = bad && (nan || (b & 0x8000)) ? (short)E::kOne : 0;
+  }
+}
+template <class V>
+__device__ __forceinline__ V add_nonfinite(V o, V plus, V minus, int n) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (e < n) {
+      if (plus[e] > 0.0f) o[e] += INFINITY;
+      if (minus[e] > 0.0f) o[e] -= INFINITY;
+    }
+  return o;
+}
+
+__device__ __forceinline__ i16x8_t join8(i16x4_t lo, i16x4_t hi) {
+  return i16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+__device__ __forceinline__ i16x4_t read_tr(const unsigned char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)p);
+}
+
+// exp2 arguments are finite or -inf: a reference of -inf (no key seen yet) is replaced by 0.
+__device__ __forceinline__ float ref_shift(float m, float scale_log2) { return m == -INFINITY ? 0.0f : m * scale_log2; }
+
+// ------------------------------------------------------------------------------------------------
+// Rows kernel. Each wave computes S^T = K . Q^T (two blocks of 32 keys x 32 rows on v_mfma_f32_32x32x16) and
+// O^T += V^T . P^T: a row is one lane pair (l, l ^ 32), whose registers hold its scores, so that the softmax is a
+// register reduction and one lane exchange, and P^T feeds the second product from registers. K and V tiles go from
+// HBM to LDS by buffer loads, four stages deep, each through a descriptor of exactly the keys that its tile has
+// left (built per tile from 64-bit addresses, so that a sequence may span more than 4 GiB): keys past the
+// sequence's last load as zeros, whatever lies there. The scores of the next tile are issued before the softmax of
+// this one.
+// Hidden keys inside a sequence (causal) have score -inf, weight 0; a non-finite value among them would still give
+// 0 * inf = NaN in the second product. Only where a row came out non-finite is the item done again on a slow path
+// that takes such values out of the product and adds them to the rows that see them.
+// ------------------------------------------------------------------------------------------------
+template <class E, int DH, int W>
+__global__ __launch_bounds__(W * 64) void packed_attn_rows_kernel(PackedAttn a) {
+  constexpr int R = 32 * W, QK_STEPS = DH / 16, OB = DH / 32, NST = 4;
+  constexpr int ROWB = 2 * DH, CPR = DH / 8, TILEB = kKeyTile * ROWB, RPI = 1024 / ROWB, STAGE = 2 * TILEB;
+  constexpr int LPW = kKeyTile / (RPI * W);
+  static_assert(RPI * W % 16 == 0 && LPW >= 1, "the swizzle repeats every 16 rows");
+  typedef typename E::v8 v8;
+  extern __shared__ __align__(16) unsigned char smem[];
+
+  const int item = blockIdx.x / a.Hk, h = blockIdx.x - item * a.Hk;
+  Item w;
+  if (!find_item<R, kKeyTile>(a, item, w)) return;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int total = w.m * a.G;                       // packed rows of the sequence
+  const int r0 = w.tile * R, rw = r0 + wave * 32;    // first row of the tile and of this wave
+  const int row = rw + l32;
+  const bool active = rw < total, mine = row < total;
+  const int tok = row / a.G, head = row - tok * a.G;
+  const int lim = mine ? seen_keys(a, w, tok) : w.n;
+  // Keys: the tile's last row sees kend, its first lim_tile (all full tiles below need no mask); the same per wave.
+  const int kend = seen_keys(a, w, (min(r0 + R, total) - 1) / a.G);
+  const int lim_tile = seen_keys(a, w, r0 / a.G);
+  const int kend_wave = active ? seen_keys(a, w, (min(rw + 32, total) - 1) / a.G) : 0;
+  const int lim_wave = active ? seen_keys(a, w, rw / a.G) : w.n;
+  const int all_tiles = (kend + kKeyTile - 1) / kKeyTile;
+  const int per = (all_tiles + w.parts - 1) / w.parts;
+  const int tb = w.part * per;                       // first key tile of this part; tiles are numbered from it below
+  const int ntiles = max(0, min(per, all_tiles - tb));
+  const int nfull = lim_tile / kKeyTile - tb;
+
+  const uint16_t* kbase = a.k + (a.batched ? (int64_t)w.seq * a.k_bs : (int64_t)w.k0 * a.k_rs) + (int64_t)h * a.k_hs;
+  const uint16_t* vbase = a.v + (a.batched ? (int64_t)w.seq * a.v_bs : (int64_t)w.k0 * a.v_rs) + (int64_t)h * a.v_hs;
+
+  v8 qf[QK_STEPS];  // lane: row l32, dims 16 ks + 8 g ..
+  {
+    const uint16_t* qp = a.q + (int64_t)(w.q0 + tok) * a.q_rs + (int64_t)(h * a.G + head) * a.q_hs + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < QK_STEPS; ++ks) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (mine) x = *reinterpret_cast<const uint4*>(qp + 16 * ks);
+      qf[ks] = as8<E>(x);
     }
   }
-  uint16_t* op = a.out + (int64_t)row * a.o_rs + (int64_t)h * DH;
-  for (int e = 0; e < DH / 64; ++e) {
-    const float y = lim ? o[e] / l : 0.0f;
-    op[e * 64 + lane] = a.fp16 ? __builtin_bit_cast(uint16_t, (_Float16)y) : (uint16_t)f32_to_bf16(y);
+
+  const int lrow = RPI * wave + lane / CPR;  // tile row that this lane loads, and rows RPI W further on
+  const uint32_t chunk = (uint32_t)(((lane % CPR) ^ tile_swz<DH>(lrow)) << 4);
+  const uint32_t koff0 = (uint32_t)lrow * (uint32_t)a.k_rs * 2u + chunk, voff0 = (uint32_t)lrow * (uint32_t)a.v_rs * 2u + chunk;
+  auto issue = [&](int stage, int t) __attribute__((always_inline)) {
+    const int key0 = (tb + t) * kKeyTile, last = min(kKeyTile, w.n - key0) - 1;
+    const i32x4_t rk = make_buffer_rsrc(kbase + (int64_t)key0 * a.k_rs, (uint32_t)last * (uint32_t)a.k_rs * 2u + ROWB);
+    const i32x4_t rv = make_buffer_rsrc(vbase + (int64_t)key0 * a.v_rs, (uint32_t)last * (uint32_t)a.v_rs * 2u + ROWB);
+    unsigned char* base = smem + stage * STAGE + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      buffer_load_lds16(rk, base + i * W * 1024, koff0 + (uint32_t)(i * RPI * W) * (uint32_t)a.k_rs * 2u);
+      buffer_load_lds16(rv, base + i * W * 1024 + TILEB, voff0 + (uint32_t)(i * RPI * W) * (uint32_t)a.v_rs * 2u);
+    }
+  };
+  auto wait_tiles = [&](int n) __attribute__((always_inline)) {  // tiles that may stay in flight
+    if (n <= 0) wait_vmcnt<0>();
+    else if (n == 1) wait_vmcnt<2 * LPW>();
+    else wait_vmcnt<4 * LPW>();
+  };
+
+  f32x16_t o[OB];
+  float m_i = -INFINITY, l_i = 0.0f;
+#pragma unroll
+  for (int d = 0; d < OB; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+
+  int koff[QK_STEPS], voff[OB][2];
+#pragma unroll
+  for (int ks = 0; ks < QK_STEPS; ++ks) koff[ks] = tile_slot<DH>(l32, ks * 2 + g);
+  {
+    const int sl = lane & 15, hh = (lane >> 4) & 1, key = 4 * g + (sl >> 2);
+#pragma unroll
+    for (int db = 0; db < OB; ++db) {
+      const int dcol = 32 * db + 16 * hh + 4 * (sl & 3);  // first of the 4 dims this lane addresses
+      voff[db][0] = TILEB + tile_slot<DH>(key, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+      voff[db][1] = TILEB + tile_slot<DH>(key + 8, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+    }
   }
+
+  struct Scores {
+    f32x16_t s[2];  // s[kb][v]: key 32 kb + 8 (v / 4) + 4 g + v % 4, row l32
+  };
+  auto scores = [&](Scores& sc, const unsigned char* st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      v8 kf[QK_STEPS];
+#pragma unroll
+      for (int ks = 0; ks < QK_STEPS; ++ks)
+        kf[ks] = as8<E>(*reinterpret_cast<const uint4*>(st + koff[ks] + kb * 32 * ROWB));
+      const f32x16_t zero = {};
+      sc.s[kb] = E::mfma32(kf[0], qf[0], zero);
+#pragma unroll
+      for (int ks = 1; ks < QK_STEPS; ++ks) sc.s[kb] = E::mfma32(kf[ks], qf[ks], sc.s[kb]);
+    }
+  };
+  // MODE 0: no key of the tile is hidden from any row; 1: some may be; 2: and values may be non-finite.
+  auto finish = [&](Scores& sc, const unsigned char* st, int t, auto mode) __attribute__((always_inline)) {
+    constexpr int MODE = decltype(mode)::value;
+    f32x16_t (&s)[2] = sc.s;
+    const int key0 = (tb + t) * kKeyTile;
+    if (MODE && key0 + kKeyTile > lim_wave) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (key0 + kb * 32 + 8 * (v >> 2) + 4 * g + (v & 3) >= lim) s[kb][v] = -INFINITY;
+    }
+    float mq[4];
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      mq[q4] = s[q4 >> 1][8 * (q4 & 1)];
+#pragma unroll
+      for (int v = 1; v < 8; ++v) mq[q4] = fmaxf(mq[q4], s[q4 >> 1][8 * (q4 & 1) + v]);
+    }
+    const float mx = xor32_max(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
+    const float m_new = softmax_ref_max(m_i, mx, a.scale_log2);
+    const float mc = ref_shift(m_new, a.scale_log2);
+    const float alpha = __builtin_amdgcn_exp2f(fmaf(m_i, a.scale_log2, -mc));
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], a.scale_log2, -mc));
+    v8 pf[4];
+    float rs[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float tmp[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tmp[e] = s[j >> 1][8 * (j & 1) + e];
+      pf[j] = round8<E>(tmp);
+      rs[j] = E::sum8(pf[j], 0.0f);
+    }
+    l_i = l_i * alpha + xor32_sum((rs[0] + rs[1]) + (rs[2] + rs[3]));
+    m_i = m_new;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < OB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+    }
+#pragma unroll
+    for (int db = 0; db < OB; ++db) {
+      [[maybe_unused]] f32x16_t plus = {}, minus = {};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        i16x8_t vt = join8(read_tr(st + voff[db][0] + j * 16 * ROWB), read_tr(st + voff[db][1] + j * 16 * ROWB));
+        if constexpr (MODE == 2) {
+          i16x8_t vp, vm;
+          split_nonfinite<E>(vt, vp, vm);
+          plus = E::mfma32(__builtin_bit_cast(v8, vp), pf[j], plus);
+          minus = E::mfma32(__builtin_bit_cast(v8, vm), pf[j], minus);
+        }
+        o[db] = E::mfma32(__builtin_bit_cast(v8, vt), pf[j], o[db]);
+      }
+      if constexpr (MODE == 2) o[db] = add_nonfinite(o[db], plus, minus, 16);
+    }
+  };
+
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  // Iteration t: wait for tile t + 1, barrier (every wave is done with tile t - 1's stage), refill that stage with
+  // tile t + 3, issue the scores of tile t + 1, then softmax and second product of tile t. All waves of the
+  // workgroup pass the same barriers; waves without rows only load.
+  auto pipeline = [&](auto work_c) __attribute__((always_inline)) {
+    constexpr bool WORK = decltype(work_c)::value;
+    Scores sa, sb;
+    auto sees = [&](int t) { return WORK && (tb + t) * kKeyTile < kend_wave; };
+    if (sees(0)) scores(sa, smem);
+    auto step = [&](auto stage_c, int t, Scores& cur, Scores& nxt, auto mode) __attribute__((always_inline)) {
+      constexpr int SG = decltype(stage_c)::value, MODE = decltype(mode)::value;
+      if (!MODE || t + 1 < ntiles) {
+        wait_tiles(min(NST - 3, ntiles - 2 - t));
+        block_barrier();
+        if (t + NST - 1 < ntiles) issue((SG + NST - 1) % NST, t + NST - 1);
+        if (MODE ? sees(t + 1) : WORK) scores(nxt, smem + ((SG + 1) % NST) * STAGE);
+      }
+      if (MODE ? sees(t) : WORK) finish(cur, smem + SG * STAGE, t, mode);
+    };
+    int t = 0;
+    for (; t + NST < ntiles && t + NST < nfull; t += NST) {  // nothing hidden in tiles t .. t + 4
+      step(I0{}, t, sa, sb, I0{});
+      step(I1{}, t + 1, sb, sa, I0{});
+      step(I2{}, t + 2, sa, sb, I0{});
+      step(I3{}, t + 3, sb, sa, I0{});
+    }
+    for (; t < ntiles; t += NST) {
+      step(I0{}, t, sa, sb, I1{});
+      if (t + 1 < ntiles) step(I1{}, t + 1, sb, sa, I1{});
+      if (t + 2 < ntiles) step(I2{}, t + 2, sa, sb, I1{});
+      if (t + 3 < ntiles) step(I3{}, t + 3, sb, sa, I1{});
+    }
+  };
+  if (ntiles > 0) {
+#pragma unroll
+    for (int st = 0; st < NST - 1; ++st)
+      if (st < ntiles) issue(st, st);
+    wait_tiles(min(NST - 2, ntiles - 1));
+    block_barrier();
+    if (active) pipeline(std::true_type{});
+    else pipeline(std::false_type{});
+    if (a.causal && (tb + ntiles) * kKeyTile > lim_tile) {  // keys were hidden by causality
+      float z = 0.0f;
+#pragma unroll
+      for (int d = 0; d < OB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) z = fmaf(o[d][v], 0.0f, z);
+      if (__syncthreads_or(mine && z != 0.0f)) {
+        m_i = -INFINITY;
+        l_i = 0.0f;
+#pragma unroll
+        for (int d = 0; d < OB; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+#pragma unroll 1
+        for (int t = 0; t < ntiles; ++t) {
+          __syncthreads();
+          issue(0, t);
+          wait_vmcnt<0>();
+          __syncthreads();
+          if ((tb + t) * kKeyTile < kend_wave) {
+            Scores sc;
+            scores(sc, smem);
+            finish(sc, smem, t, I2{});
+          }
+        }
+      }
+    }
+  }
+
+  // O^T: lane l, register v of block db -> dim 32 db + 8 (v / 4) + 4 g + v % 4 of row l32.
+  if (!mine) return;
+  const int orow = w.q0 + tok, ohead = h * a.G + head;
+  if (a.target && w.part == 0 && g == 0)
+    a.dir[(int64_t)orow * a.Hk * a.G + ohead] = make_int2(item, w.parts | (row - r0) << 16);
+  if (w.parts > 1) {
+    float* ws = a.ws + ((int64_t)item * a.Hk + h) * part_floats(R, DH);
+    const int r = row - r0;
+    if (g == 0) {
+      ws[r] = m_i;
+      ws[R + r] = l_i;
+    }
+    float* wo = ws + 2 * R + (int64_t)r * DH + 4 * g;
+#pragma unroll
+    for (int d = 0; d < OB; ++d)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4)
+        *reinterpret_cast<f32x4_t*>(wo + 32 * d + 8 * r4) =
+            f32x4_t{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+    return;
+  }
+  const float inv = l_i == 0.0f ? 0.0f : 1.0f / l_i;
+  uint16_t* op = a.out + (int64_t)orow * a.o_rs + (int64_t)ohead * DH + 4 * g;
+#pragma unroll
+  for (int d = 0; d < OB; ++d)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const f32x4_t x = {o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv};
+      *reinterpret_cast<typename E::v4*>(op + 32 * d + 8 * r4) = __builtin_convertvector(x, typename E::v4);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Keys kernel, for sequences of few packed rows (single tokens): 16 rows per workgroup, whose four waves take 32 keys
+// each in turn through rings of their own in LDS, so that no barrier holds a wave and the loads of a CU (up to 96 KB)
+// are never drained; the waves' results meet in LDS at the end. Bound by reading K and V once.
+// S^T per 16-key block on v_mfma_f32_16x16x32 (lane l, G = l / 16: keys 4 G + v of row l % 16), O^T per 16 dims
+// (keys 4 G + {0..3} and 16 + 4 G + {0..3} per lane, V^T by the transposing LDS read).
+// ------------------------------------------------------------------------------------------------
+template <class E, int DH, int NS>
+__global__ __launch_bounds__(256) void packed_attn_keys_kernel(PackedAttn a) {
+  constexpr int R = 16, WAVES = 4, KEYS = 32, QK_STEPS = DH / 32, DB = DH / 16;
+  constexpr int ROWB = 2 * DH, CPR = DH / 8, TILEB = KEYS * ROWB, RPI = 1024 / ROWB, L = KEYS / RPI;
+  typedef typename E::v8 v8;
+  extern __shared__ __align__(16) unsigned char smem[];
+
+  const int item = blockIdx.x / a.Hk, h = blockIdx.x - item * a.Hk;
+  Item w;
+  if (!find_item<R, WAVES * KEYS>(a, item, w)) return;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, G = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int total = w.m * a.G, r0 = w.tile * R, row = r0 + l16;
+  const bool mine = row < total;
+  const int tok = row / a.G, head = row - tok * a.G;
+  const int lim = mine ? seen_keys(a, w, tok) : w.n;
+  const int kend = seen_keys(a, w, (min(r0 + R, total) - 1) / a.G);
+  const int lim_tile = seen_keys(a, w, r0 / a.G);
+  constexpr int KT = WAVES * KEYS;
+  const int all_tiles = (kend + KT - 1) / KT, per = (all_tiles + w.parts - 1) / w.parts;
+  const int kfirst = w.part * per * KT, klast = min(kend, kfirst + per * KT);  // this part's keys
+  const int n32 = max(0, (klast - kfirst + KEYS - 1) / KEYS);
+  const int cnt = (n32 - wave + WAVES - 1) / WAVES;  // tiles of this wave: wave, wave + 4, ...
+
+  const uint16_t* kbase = a.k + (a.batched ? (int64_t)w.seq * a.k_bs : (int64_t)w.k0 * a.k_rs) + (int64_t)h * a.k_hs;
+  const uint16_t* vbase = a.v + (a.batched ? (int64_t)w.seq * a.v_bs : (int64_t)w.k0 * a.v_rs) + (int64_t)h * a.v_hs;
+  unsigned char* kring = smem + wave * (2 * NS * TILEB);
+  unsigned char* vring = kring + NS * TILEB;
+
+  v8 qf[QK_STEPS];  // lane: row l16, dims 32 ks + 8 G ..
+  {
+    const uint16_t* qp = a.q + (int64_t)(w.q0 + tok) * a.q_rs + (int64_t)(h * a.G + head) * a.q_hs + 8 * G;
+#pragma unroll
+    for (int ks = 0; ks < QK_STEPS; ++ks) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (mine) x = *reinterpret_cast<const uint4*>(qp + 32 * ks);
+      qf[ks] = as8<E>(x);
+    }
+  }
+  auto key_of = [&](int t) { return kfirst + (WAVES * t + wave) * KEYS; };
+  auto issue = [&](unsigned char* ring, const uint16_t* base, int64_t rs, int t) __attribute__((always_inline)) {
+    const int key0 = key_of(t), last = min(KEYS, w.n - key0) - 1;
+    const i32x4_t rsrc = make_buffer_rsrc(base + (int64_t)key0 * rs, (uint32_t)last * (uint32_t)rs * 2u + ROWB);
+    unsigned char* dst = ring + (t % NS) * TILEB;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int r = RPI * i + lane / CPR;
+      buffer_load_lds16(rsrc, dst + i * 1024,
+                        (uint32_t)r * (uint32_t)rs * 2u + (uint32_t)(((lane % CPR) ^ tile_swz<DH>(r)) << 4));
+    }
+  };
+  // At most n of this wave's K or V tiles may stay in flight.
+  auto wait_loads = [&](int n) __attribute__((always_inline)) {
+    static_assert((2 * NS - 1) * L < 64, "vmcnt range");
+    if (n >= 2 * NS - 1) wait_vmcnt<(2 * NS - 1) * L>();
+    else if (NS > 3 && n == 6) wait_vmcnt<6 * L>();
+    else if (NS > 3 && n == 5) wait_vmcnt<5 * L>();
+    else if (NS > 2 && n == 4) wait_vmcnt<4 * L>();
+    else if (NS > 2 && n == 3) wait_vmcnt<3 * L>();
+    else if (n == 2) wait_vmcnt<2 * L>();
+    else if (n == 1) wait_vmcnt<L>();
+    else wait_vmcnt<0>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto reads_done = [&]() __attribute__((always_inline)) {  // this wave's LDS reads, before their stage is refilled
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  int koff[QK_STEPS], voff[DB][2];
+#pragma unroll
+  for (int ks = 0; ks < QK_STEPS; ++ks) koff[ks] = tile_slot<DH>(l16, 4 * ks + G);
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    const int dcol = 16 * db + 4 * (l16 & 3), key = 4 * G + (l16 >> 2);
+    voff[db][0] = tile_slot<DH>(key, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+    voff[db][1] = tile_slot<DH>(key + 16, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+  }
+
+  f32x4_t o[DB];
+  float m_i, l_i;
+  auto reset = [&]() {
+    m_i = -INFINITY;
+    l_i = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  };
+  reset();
+  f32x4_t s[2];
+  auto scores = [&](const unsigned char* st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      s[kb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < QK_STEPS; ++ks)
+        s[kb] = E::mfma16(as8<E>(*reinterpret_cast<const uint4*>(st + koff[ks] + kb * 16 * ROWB)), qf[ks], s[kb]);
+    }
+  };
+  v8 pf;
+  auto softmax = [&](int key0) __attribute__((always_inline)) {
+    if (key0 + KEYS > lim_tile) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (key0 + 16 * kb + 4 * G + v >= lim) s[kb][v] = -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+    mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = xor32_max(xor16_max(mx));
+    const float m_new = softmax_ref_max(m_i, mx, a.scale_log2);
+    const float mc = ref_shift(m_new, a.scale_log2);
+    const float alpha = __builtin_amdgcn_exp2f(fmaf(m_i, a.scale_log2, -mc));
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], a.scale_log2, -mc));
+    pf = round8<E>(p);
+    l_i = l_i * alpha + xor32_sum(xor16_sum(E::sum8(pf, 0.0f)));
+    m_i = m_new;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= alpha;
+    }
+  };
+  auto values = [&](const unsigned char* st, auto safe) __attribute__((always_inline)) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      i16x8_t vt = join8(read_tr(st + voff[db][0]), read_tr(st + voff[db][1]));
+      if constexpr (decltype(safe)::value) {
+        i16x8_t vp, vm;
+        split_nonfinite<E>(vt, vp, vm);
+        const f32x4_t zero = {};
+        const f32x4_t plus = E::mfma16(__builtin_bit_cast(v8, vp), pf, zero);
+        const f32x4_t minus = E::mfma16(__builtin_bit_cast(v8, vm), pf, zero);
+        o[db] = E::mfma16(__builtin_bit_cast(v8, vt), pf, o[db]);
+        o[db] = add_nonfinite(o[db], plus, minus, 4);
+      } else {
+        o[db] = E::mfma16(__builtin_bit_cast(v8, vt), pf, o[db]);
+      }
+    }
+  };
+
+#pragma unroll
+  for (int t = 0; t < NS; ++t)
+    if (t < cnt) {
+      issue(kring, kbase, a.k_rs, t);
+      issue(vring, vbase, a.v_rs, t);
+    }
+#pragma unroll 1
+  for (int t = 0; t < cnt; ++t) {
+    const int ahead = 2 * min(NS - 1, cnt - 1 - t);  // loads of the tiles after this one
+    wait_loads(ahead + 1);
+    scores(kring + (t % NS) * TILEB);
+    if (t + NS < cnt) {
+      reads_done();
+      issue(kring, kbase, a.k_rs, t + NS);
+    }
+    softmax(key_of(t));
+    wait_loads(ahead + (t + NS < cnt ? 1 : 0));
+    values(vring + (t % NS) * TILEB, std::false_type{});
+    if (t + NS < cnt) {
+      reads_done();
+      issue(vring, vbase, a.v_rs, t + NS);
+    }
+  }
+  if (a.causal && klast > lim_tile) {  // keys were hidden by causality: see the rows kernel
+    float z = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) z = fmaf(o[d][v], 0.0f, z);
+    if (__builtin_amdgcn_ballot_w64(mine && z != 0.0f)) {
+      reset();
+#pragma unroll 1
+      for (int t = 0; t < cnt; ++t) {
+        reads_done();
+        issue(kring, kbase, a.k_rs, t);
+        issue(vring, vbase, a.v_rs, t);
+        wait_loads(0);
+        scores(kring + (t % NS) * TILEB);
+        softmax(key_of(t));
+        values(vring + (t % NS) * TILEB, std::true_type{});
+      }
+    }
+  }
+
+  // The four waves' results: references and sums, then rows of DH + 4 floats (conflict-free writes of 16 rows).
+  constexpr int OROW = DH + 4, WROWS = 2 * R + R * OROW;
+  float* park = reinterpret_cast<float*>(smem);
+  __syncthreads();
+  {
+    float* p = park + wave * WROWS;
+    if (G == 0) {
+      p[l16] = m_i;
+      p[R + l16] = l_i;
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4_t*>(p + 2 * R + l16 * OROW + 16 * d + 4 * G) = o[d];
+  }
+  __syncthreads();
+  const int r = threadIdx.x / CPR, c = threadIdx.x % CPR;  // row, 8 dims
+  if (r >= R || r0 + r >= total) return;
+  float mp[WAVES], m = -INFINITY, l = 0.0f, x[8] = {};
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    mp[i] = park[i * WROWS + r];
+    m = fmaxf(m, mp[i]);
+  }
+  const float mc = ref_shift(m, a.scale_log2);
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    const float f = __builtin_amdgcn_exp2f(fmaf(mp[i], a.scale_log2, -mc));
+    l = fmaf(park[i * WROWS + R + r], f, l);
+    const float* src = park + i * WROWS + 2 * R + r * OROW + 8 * c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(src[e], f, x[e]);
+  }
+  const int otok = (r0 + r) / a.G, orow = w.q0 + otok, ohead = h * a.G + (r0 + r - otok * a.G);
+  if (a.target && w.part == 0 && c == 0)
+    a.dir[(int64_t)orow * a.Hk * a.G + ohead] = make_int2(item, w.parts | r << 16);
+  if (w.parts > 1) {
+    float* ws = a.ws + ((int64_t)item * a.Hk + h) * part_floats(R, DH);
+    if (c == 0) {
+      ws[r] = m;
+      ws[R + r] = l;
+    }
+    f32x4_t* wo = reinterpret_cast<f32x4_t*>(ws + 2 * R + (int64_t)r * DH + 8 * c);
+    wo[0] = f32x4_t{x[0], x[1], x[2], x[3]};
+    wo[1] = f32x4_t{x[4], x[5], x[6], x[7]};
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= inv;
+  const v8 y = round8<E>(x);
+  *reinterpret_cast<v8*>(a.out + (int64_t)orow * a.o_rs + (int64_t)ohead * DH + 8 * c) = y;
+}
+
+// Merge of the key parts: a wave per (row, query head), DH / 8 lanes of 8 dims by 64 / (DH / 8) parts at a time.
+// With m = max_p m_p and f_p = 2^(c (m_p - m)): out = sum_p f_p o_p / sum_p f_p l_p. A part without a visible key has
+// l_p = 0 and is left out. Rows past the last sequence have no entry in the directory and are not read.
+template <class E, int DH>
+__global__ __launch_bounds__(256) void packed_attn_merge_kernel(PackedAttn a, int R) {
+  constexpr int CPR = DH / 8, PL = 64 / CPR, U = 4;
+  const int Hq = a.Hk * a.G;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int row = (int)(unit / Hq), head = (int)(unit - (int64_t)row * Hq);
+  if (row >= a.rows || row >= load_idx(a.cu_q, a.S, a.cu_wide, 0, a.rows) || row < load_idx(a.cu_q, 0, a.cu_wide, 0, a.rows))
+    return;
+  const int2 d = a.dir[unit];
+  const int parts = d.y & 0xffff, r = d.y >> 16;
+  // (offsets that do not rise leave rows without an entry: whatever lies there is not followed out of the workspace)
+  if (parts <= 1 || d.x < 0 || d.x > a.items - parts || r < 0 || r >= R) return;
+  const int lane = threadIdx.x & 63, c = lane % CPR, pl = lane / CPR;
+  const int64_t stride = a.Hk * part_floats(R, DH);
+  const float* base = a.ws + ((int64_t)d.x * a.Hk + head / a.G) * part_floats(R, DH);
+  float m = -INFINITY, l = 0.0f, x[8] = {};
+  for (int p0 = pl; p0 < parts; p0 += PL * U) {
+    float mp[U], lp[U];
+    f32x4_t y[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* b = base + min(p0 + u * PL, parts - 1) * stride;
+      mp[u] = b[r];
+      lp[u] = p0 + u * PL < parts ? b[R + r] : 0.0f;
+      const f32x4_t* src = reinterpret_cast<const f32x4_t*>(b + 2 * R + (int64_t)r * DH + 8 * c);
+      y[u][0] = src[0];
+      y[u][1] = src[1];
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (lp[u] != 0.0f) top = fmaxf(top, mp[u]);
+    const float tc = ref_shift(top, a.scale_log2);
+    const float keep = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= keep;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (lp[u] != 0.0f) {
+        const float f = __builtin_amdgcn_exp2f(fmaf(mp[u], a.scale_log2, -tc));
+        l = fmaf(lp[u], f, l);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(y[u][e >> 2][e & 3], f, x[e]);
+      }
+  }
+#pragma unroll
+  for (int s = CPR; s < 64; s <<= 1) {
+    const float m2 = __shfl_xor(m, s, 64), top = fmaxf(m, m2), tc = ref_shift(top, a.scale_log2);
+    const float f = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
+    const float f2 = __builtin_amdgcn_exp2f(fmaf(m2, a.scale_log2, -tc));
+    m = top;
+    l = l * f + __shfl_xor(l, s, 64) * f2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * f + __shfl_xor(x[e], s, 64) * f2;
+  }
+  if (pl) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= inv;
+  typename E::v8 y = round8<E>(x);
+  *reinterpret_cast<typename E::v8*>(a.out + (int64_t)row * a.o_rs + (int64_t)head * DH + 8 * c) = y;
 }
 
 }  // namespace oudjat
 
 using namespace oudjat;
 
+static constexpr int kPackedCus = 256;
+
+// How a call is dealt, from what the host knows: rows per tile (16: the keys kernel), the most items of a key head,
+// and how many parts at the most its items are cut into beside their own number (0: never, no workspace).
+struct PackedShape {
+  int R, target, min_tiles;
+  int64_t items;
+};
+
+static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh) {
+  PackedShape s{};
+  const int64_t G = Hq / Hk, seqs = std::max<int64_t>(1, std::min(S, rows));
+  const int64_t mean = cdiv(rows * G, seqs);  // packed rows of a sequence
+  if (mean <= 32) {
+    s.R = 16;
+    s.min_tiles = 2;   // of 128 keys
+  } else {
+    s.R = Dh == 128 && mean > 128 ? 256 : 128;
+    s.min_tiles = 4;   // of 64 keys
+  }
+  const int64_t tiles = std::max(rows * G / s.R, seqs);  // about as many as there are
+  const int64_t want = 2 * kPackedCus;
+  s.target = tiles * Hk < 2 * want ? (int)cdiv(want, Hk) : 0;
+  // ceil of the sequences' tiles: one more than the rows' own for each that has rows; and the parts, with room for
+  // the rounding of the units' fp32 sum.
+  s.items = rows * G / s.R + seqs + (s.target ? s.target + s.target / 16 + 1 : 0);
+  return s;
+}
+
+static int64_t packed_part_elems(const PackedShape& s, int64_t Hk, int64_t Dh) {
+  return s.items * Hk * part_floats(s.R, (int)Dh);
+}
+
 extern "C" int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh) {
-  return 0;
+  if (rows <= 0 || S <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || (Dh != 64 && Dh != 128) || rows * (Hq / Hk) >= 1 << 30)
+    return 0;
+  const PackedShape s = packed_shape(rows, S, Hq, Hk, Dh);
+  return s.target ? packed_part_elems(s, Hk, Dh) + rows * Hq * 2 : 0;
+}
+
+// Allows a kernel `lds` bytes of dynamic LDS on the current device, once.
+static int allow_lds(const void* fn, int lds, std::atomic<uint64_t>& done, const char* what) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return set_error(OUDJAT_ERR_HIP, "%s: hipGetDevice: %s", what, hipGetErrorString(e));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return OUDJAT_OK;
+  e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e != hipSuccess) return set_error(OUDJAT_ERR_HIP, "%s: hipFuncSetAttribute: %s", what, hipGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_release);
+  return OUDJAT_OK;
+}
+
+template <class E, int DH, int W>
+static int launch_rows(const PackedAttn& a, hipStream_t st, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int lds = 4 * 2 * kKeyTile * 2 * DH;
+  const int rc = allow_lds((const void*)packed_attn_rows_kernel<E, DH, W>, lds, done, what);
+  if (rc != OUDJAT_OK) return rc;
+  packed_attn_rows_kernel<E, DH, W><<<(unsigned)a.items * a.Hk, W * 64, lds, st>>>(a);
+  return check_launch(what);
+}
+
+template <class E, int DH>
+static int launch_keys(const PackedAttn& a, hipStream_t st, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int NS = DH == 128 ? 2 : 4, lds = 4 * 2 * NS * 32 * 2 * DH;  // 128 KB
+  const int rc = allow_lds((const void*)packed_attn_keys_kernel<E, DH, NS>, lds, done, what);
+  if (rc != OUDJAT_OK) return rc;
+  packed_attn_keys_kernel<E, DH, NS><<<(unsigned)a.items * a.Hk, 256, lds, st>>>(a);
+  return check_launch(what);
+}
+
+template <class E, int DH>
+static int launch_packed(const PackedAttn& a, int R, hipStream_t st, const char* what) {
+  int rc;
+  if (R == 16) rc = launch_keys<E, DH>(a, st, what);
+  else if constexpr (DH == 128) rc = R == 256 ? launch_rows<E, DH, 8>(a, st, what) : launch_rows<E, DH, 4>(a, st, what);
+  else rc = launch_rows<E, DH, 4>(a, st, what);
+  if (rc != OUDJAT_OK || !a.target) return rc;
+  const unsigned grid = (unsigned)cdiv((int64_t)a.rows * a.Hk * a.G, 4);
+  packed_attn_merge_kernel<E, DH><<<grid, 256, 0, st>>>(a, R);
+  return check_launch("packed_attention (merge)");
 }
 
 extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64_t rows, int64_t Hq, int64_t Dh,
@@ -124,18 +932,25 @@ extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t 
   OUDJAT_REQUIRE(q_rs >= 0 && q_hs >= 0 && k_bs >= 0 && k_rs >= 0 && k_hs >= 0 && v_bs >= 0 && v_rs >= 0 && v_hs >= 0 &&
                      out_rs >= 0,
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: negative stride", what);
-  OUDJAT_REQUIRE(((q_rs | q_hs | k_bs | k_rs | k_hs | v_bs | v_rs | v_hs) % 8) == 0 && out_rs % 4 == 0 && aligned(q, 16) &&
-                     aligned(k, 16) && aligned(v, 16) && aligned(out, 8) && aligned(cu_q, cu_wide ? 8 : 4) &&
+  OUDJAT_REQUIRE(((q_rs | q_hs | k_bs | k_rs | k_hs | v_bs | v_rs | v_hs) % 8) == 0 && out_rs % 8 == 0 && aligned(q, 16) &&
+                     aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, cu_wide ? 8 : 4) &&
                      aligned(keys, keys_wide ? 8 : 4),
-                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned q, k and v rows and heads required", what);
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned q, k, v and out rows and heads required", what);
   OUDJAT_REQUIRE(rows * (Hq / Hk) < (1 << 30) && Hq <= 65535 && S < (1 << 24) && key_cap < (1 << 30) &&
                      k_rs < (1 << 24) && v_rs < (1 << 24),
                  OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
-  PackedAttn a{q, q_rs, q_hs, k, v, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, cu_q, keys, out, out_rs, (int)rows, (int)S,
-               (int)Hq, (int)(Hq / Hk), (int)key_cap, cu_wide != 0, keys_wide != 0, batched != 0, causal != 0,
-               dtype == OUDJAT_FP16, scale * 1.4426950408889634f};
-  const unsigned grid = (unsigned)cdiv(rows * Hq, 4);
-  if (Dh == 64) packed_attn_kernel<64><<<grid, 256, 0, as_stream(stream)>>>(a);
-  else packed_attn_kernel<128><<<grid, 256, 0, as_stream(stream)>>>(a);
-  return check_launch(what);
+  const PackedShape s = packed_shape(rows, S, Hq, Hk, Dh);
+  OUDJAT_REQUIRE(s.items * Hk < (1 << 23), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
+  const int64_t parts = s.target ? packed_part_elems(s, Hk, Dh) : 0;
+  OUDJAT_REQUIRE(!s.target || (workspace && aligned(workspace, 16) && workspace_elems >= parts + rows * Hq * 2),
+                 OUDJAT_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld elements is needed", what,
+                 (long long)(parts + rows * Hq * 2));
+  const PackedAttn a{q, q_rs, q_hs, k, v, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, cu_q, keys, out, out_rs, (int)rows, (int)S,
+                     (int)Hk, (int)(Hq / Hk), (int)key_cap, cu_wide != 0, keys_wide != 0, batched != 0, causal != 0,
+                     scale * 1.4426950408889634f, s.target, s.min_tiles, (int)s.items, workspace,
+                     s.target ? reinterpret_cast<int2*>(workspace + parts) : nullptr};
+  hipStream_t st = as_stream(stream);
+  if (dtype == OUDJAT_BF16)
+    return Dh == 64 ? launch_packed<AttnBf16, 64>(a, s.R, st, what) : launch_packed<AttnBf16, 128>(a, s.R, st, what);
+  return Dh == 64 ? launch_packed<AttnFp16, 64>(a, s.R, st, what) : launch_packed<AttnFp16, 128>(a, s.R, st, what);
 }

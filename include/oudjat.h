@@ -797,7 +797,7 @@ int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t rows, int6
  * Where one workgroup per tile of query rows would leave CUs idle, the keys are split over several and merged by a
  * second launch (in part order): workspace of oudjat_packed_attention_workspace_elems fp32 elements, 16-byte
  * aligned, else OUDJAT_ERR_INVALID_ARGUMENT. Deterministic. Dh 64 or 128; scale > 0 and finite; 16-byte aligned
- * rows and heads of q, k, v, 8-byte aligned of out; strides not negative. */
+ * rows and heads of q, k, v and out; strides not negative. */
 int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64_t rows, int64_t Hq, int64_t Dh,
                             const uint16_t* k, int64_t k_bs, int64_t k_rs, int64_t k_hs, const uint16_t* v,
                             int64_t v_bs, int64_t v_rs, int64_t v_hs, int64_t Hk, int64_t key_cap, int batched,
