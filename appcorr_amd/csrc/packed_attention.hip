@@ -240,7 +240,7 @@ __device__ __forceinline__ float ref_shift(float m, float scale_log2) { return m
 // that takes such values out of the product and adds them to the rows that see them.
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int W>
-__global__ __launch_bounds__(W * 64) void packed_attn_rows_kernel(PackedAttn a) {
+__global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn a) {
   constexpr int R = 32 * W, QK_STEPS = DH / 16, OB = DH / 32, NST = 4;
   constexpr int ROWB = 2 * DH, CPR = DH / 8, TILEB = kKeyTile * ROWB, RPI = 1024 / ROWB, STAGE = 2 * TILEB;
   constexpr int LPW = kKeyTile / (RPI * W);
@@ -516,7 +516,7 @@ __global__ __launch_bounds__(W * 64) void packed_attn_rows_kernel(PackedAttn a) 
 // (keys 4 G + {0..3} and 16 + 4 G + {0..3} per lane, V^T by the transposing LDS read).
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int NS>
-__global__ __launch_bounds__(256) void packed_attn_keys_kernel(PackedAttn a) {
+__global__ __launch_bounds__(256, 2) void packed_attn_keys_kernel(PackedAttn a) {
   constexpr int R = 16, WAVES = 4, KEYS = 32, QK_STEPS = DH / 32, DB = DH / 16;
   constexpr int ROWB = 2 * DH, CPR = DH / 8, TILEB = KEYS * ROWB, RPI = 1024 / ROWB, L = KEYS / RPI;
   typedef typename E::v8 v8;
