@@ -34,6 +34,16 @@ namespace oudjat {
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x8_t __attribute__((ext_vector_type(8)));
 
+// Division of 0 .. 2^31 - 1 by a number that the launch fixes: x / d = x * ceil(2^(31 + b) / d) >> (31 + b), 2^b >= d.
+struct Divisor {
+  uint32_t d, mul, shift;
+  explicit Divisor(uint32_t n) : d(n), shift(0) {
+    while ((1u << shift) < n) ++shift;
+    mul = (uint32_t)(((1ull << (31 + shift)) + n - 1) / n);
+  }
+  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * mul) >> (31 + shift)); }
+};
+
 struct PackedAttn {
   const uint16_t* q;
   int64_t q_rs, q_hs;
@@ -43,6 +53,7 @@ struct PackedAttn {
   uint16_t* out;
   int64_t o_rs;
   int rows, S, Hk, G;
+  Divisor by_hk, by_g;
   int key_cap;
   bool cu_wide, keys_wide, batched, causal;
   float scale_log2;
@@ -50,8 +61,8 @@ struct PackedAttn {
   // their own number, and the fewest key tiles of a part.
   int target, min_tiles;
   int items;      // items a key head has at the most (the grid)
-  float* ws;      // parts, then the directory
-  int2* dir;      // [rows][Hq]: first item of the row's tile, its parts | row in the tile << 16
+  float* ws;      // the items' partial results
+  int4* heads;    // per (item, key head): parts to merge from this item on (0: none), first row, packed row, rows
 };
 
 // Element types on the matrix cores.
@@ -128,61 +139,97 @@ __device__ __forceinline__ void load_seq(const PackedAttn& a, int s, Item& t) {
   }
 }
 
+// Wave-wide sums and maxima by data-parallel moves (no LDS round trips): value of every lane combined with those of
+// all lanes before it; lane 63 has the whole.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T x, F&& f) {
+  auto from = [&](auto ctrl, auto rows) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                             decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  x = f(x, from(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{}));  // row_shr:1
+  x = f(x, from(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{}));  // row_shr:2
+  x = f(x, from(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{}));  // row_shr:4
+  x = f(x, from(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{}));  // row_shr:8
+  x = f(x, from(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{}));  // row_bcast:15 to rows 1 and 3
+  x = f(x, from(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{}));  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
+__device__ __forceinline__ float last_lane(float x) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
+}
+
+static constexpr int kSortedSeqs = 256;
+
 // Item number `item` of a key head, tiles of R packed rows and KT keys; false past the last. Parts of a sequence's
 // tiles: ceil(its key tiles / C), with C = max(min_tiles, units / target) and units the key tiles of all tiles, so
-// that a key head has at most its own tiles + target items.
+// that a key head has at most its own tiles + target items. Up to kSortedSeqs sequences the items of the longer ones
+// (more than half of the longest's keys, then more than a quarter) come first, so that the last workgroups are short.
 template <int R, int KT>
 __device__ __forceinline__ bool find_item(const PackedAttn& a, int item, Item& w) {
   const int lane = threadIdx.x & 63;
   Item t;
-  int chunk = 1 << 30;
-  auto tiles = [&](const Item& x) { return (int)(((int64_t)x.m * a.G + R - 1) / R); };
-  auto key_tiles = [&](const Item& x) { return (x.n + KT - 1) / KT; };
+  int chunk = 1 << 30, top = 0;
+  auto tiles = [&]() { return (int)(((int64_t)t.m * a.G + R - 1) / R); };
+  auto key_tiles = [&]() { return (t.n + KT - 1) / KT; };
   auto load = [&](int s0) {
     t.q0 = t.m = t.n = t.k0 = 0;
     if (s0 + lane < a.S) load_seq(a, s0 + lane, t);
   };
   load(0);
-  if (a.target) {
-    float units = (float)tiles(t) * (float)key_tiles(t);
+  const bool sorted = a.S <= kSortedSeqs;
+  if (a.target || sorted) {
+    float units = (float)tiles() * (float)key_tiles();
+    top = key_tiles();
     for (int s0 = 64; s0 < a.S; s0 += 64) {
       load(s0);
-      units += (float)tiles(t) * (float)key_tiles(t);
+      units += (float)tiles() * (float)key_tiles();
+      top = max(top, key_tiles());
     }
-    units = wave_sum(units);
-    chunk = max(a.min_tiles, (int)ceilf(units / (float)a.target));
+    if (a.target) {
+      units = last_lane(wave_scan(units, [](float x, float y) { return x + y; }));
+      chunk = max(a.min_tiles, (int)ceilf(units / (float)a.target));
+    }
+    top = last_lane(wave_scan(top, [](int x, int y) { return max(x, y); }));
     if (a.S > 64) load(0);
   }
   int base = 0;
-  for (int s0 = 0; s0 < a.S; s0 += 64) {
-    if (s0) load(s0);
-    const int nt = tiles(t), kt = key_tiles(t);
-    const int parts = max(1, (kt + chunk - 1) / chunk);
-    const int mine = nt * parts;
-    int incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += up;
+  for (int cls = 0; cls < (sorted ? 3 : 1); ++cls) {
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+      if (a.S > 64 && (s0 || cls)) load(s0);
+      const int nt = tiles(), kt = key_tiles(), parts = a.target ? max(1, (kt + chunk - 1) / chunk) : 1;
+      const int mine = !sorted || (2 * kt > top ? 0 : 4 * kt > top ? 1 : 2) == cls ? nt * parts : 0;
+      const int incl = wave_scan(mine, [](int x, int y) { return x + y; });
+      const int total = last_lane(incl);
+      if (item < base + total) {
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + incl > item));
+        const int within = item - base - __builtin_amdgcn_readlane(incl - mine, l);
+        w.seq = s0 + l;
+        w.q0 = __builtin_amdgcn_readlane(t.q0, l);
+        w.m = __builtin_amdgcn_readlane(t.m, l);
+        w.n = __builtin_amdgcn_readlane(t.n, l);
+        w.k0 = __builtin_amdgcn_readlane(t.k0, l);
+        w.parts = __builtin_amdgcn_readlane(parts, l);
+        const int from_last = w.parts == 1 ? within : within / w.parts;
+        w.part = within - from_last * w.parts;
+        w.tile = __builtin_amdgcn_readlane(nt, l) - 1 - from_last;
+        return true;
+      }
+      base += total;
     }
-    const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (item < base + total) {
-      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + incl > item));
-      const int within = item - base - __builtin_amdgcn_readlane(incl - mine, l);
-      w.seq = s0 + l;
-      w.q0 = __builtin_amdgcn_readlane(t.q0, l);
-      w.m = __builtin_amdgcn_readlane(t.m, l);
-      w.n = __builtin_amdgcn_readlane(t.n, l);
-      w.k0 = __builtin_amdgcn_readlane(t.k0, l);
-      w.parts = __builtin_amdgcn_readlane(parts, l);
-      const int from_last = within / w.parts;
-      w.part = within - from_last * w.parts;
-      w.tile = __builtin_amdgcn_readlane(nt, l) - 1 - from_last;
-      return true;
-    }
-    base += total;
   }
   return false;
+}
+
+// What the merge has to do from this item on (every workgroup of the grid says it, those without an item too).
+template <int R>
+__device__ __forceinline__ void note_merge(const PackedAttn& a, int item, int h, bool found, const Item& w) {
+  if (!a.target || threadIdx.x) return;
+  int4 x = make_int4(0, 0, 0, 0);
+  if (found && w.part == 0 && w.parts > 1) x = make_int4(w.parts, w.q0, w.tile * R, min(R, w.m * a.G - w.tile * R));
+  a.heads[(int64_t)item * a.Hk + h] = x;
 }
 
 // Keys that token i of the sequence sees.
@@ -248,24 +295,26 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
   typedef typename E::v8 v8;
   extern __shared__ __align__(16) unsigned char smem[];
 
-  const int item = blockIdx.x / a.Hk, h = blockIdx.x - item * a.Hk;
+  const int item = a.by_hk(blockIdx.x), h = blockIdx.x - item * a.Hk;
   Item w;
-  if (!find_item<R, kKeyTile>(a, item, w)) return;
+  const bool found = find_item<R, kKeyTile>(a, item, w);
+  note_merge<R>(a, item, h, found, w);
+  if (!found) return;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int total = w.m * a.G;                       // packed rows of the sequence
   const int r0 = w.tile * R, rw = r0 + wave * 32;    // first row of the tile and of this wave
   const int row = rw + l32;
   const bool active = rw < total, mine = row < total;
-  const int tok = row / a.G, head = row - tok * a.G;
+  const int tok = a.by_g(row), head = row - tok * a.G;
   const int lim = mine ? seen_keys(a, w, tok) : w.n;
   // Keys: the tile's last row sees kend, its first lim_tile (all full tiles below need no mask); the same per wave.
-  const int kend = seen_keys(a, w, (min(r0 + R, total) - 1) / a.G);
-  const int lim_tile = seen_keys(a, w, r0 / a.G);
-  const int kend_wave = active ? seen_keys(a, w, (min(rw + 32, total) - 1) / a.G) : 0;
-  const int lim_wave = active ? seen_keys(a, w, rw / a.G) : w.n;
+  const int kend = seen_keys(a, w, a.by_g(min(r0 + R, total) - 1));
+  const int lim_tile = seen_keys(a, w, a.by_g(r0));
+  const int kend_wave = active ? seen_keys(a, w, a.by_g(min(rw + 32, total) - 1)) : 0;
+  const int lim_wave = active ? seen_keys(a, w, a.by_g(rw)) : w.n;
   const int all_tiles = (kend + kKeyTile - 1) / kKeyTile;
-  const int per = (all_tiles + w.parts - 1) / w.parts;
+  const int per = w.parts == 1 ? all_tiles : (all_tiles + w.parts - 1) / w.parts;
   const int tb = w.part * per;                       // first key tile of this part; tiles are numbered from it below
   const int ntiles = max(0, min(per, all_tiles - tb));
   const int nfull = lim_tile / kKeyTile - tb;
@@ -287,16 +336,34 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
   const int lrow = RPI * wave + lane / CPR;  // tile row that this lane loads, and rows RPI W further on
   const uint32_t chunk = (uint32_t)(((lane % CPR) ^ tile_swz<DH>(lrow)) << 4);
   const uint32_t koff0 = (uint32_t)lrow * (uint32_t)a.k_rs * 2u + chunk, voff0 = (uint32_t)lrow * (uint32_t)a.v_rs * 2u + chunk;
-  auto issue = [&](int stage, int t) __attribute__((always_inline)) {
-    const int key0 = (tb + t) * kKeyTile, last = min(kKeyTile, w.n - key0) - 1;
-    const i32x4_t rk = make_buffer_rsrc(kbase + (int64_t)key0 * a.k_rs, (uint32_t)last * (uint32_t)a.k_rs * 2u + ROWB);
-    const i32x4_t rv = make_buffer_rsrc(vbase + (int64_t)key0 * a.v_rs, (uint32_t)last * (uint32_t)a.v_rs * 2u + ROWB);
+  // Tiles are issued in order: the next one's addresses and the keys left from it on (uniform).
+  const uint16_t *knext, *vnext;
+  int left;
+  const int64_t kstep = kKeyTile * a.k_rs, vstep = kKeyTile * a.v_rs;
+  const uint32_t kfull = (uint32_t)(kKeyTile - 1) * (uint32_t)a.k_rs * 2u + ROWB;
+  const uint32_t vfull = (uint32_t)(kKeyTile - 1) * (uint32_t)a.v_rs * 2u + ROWB;
+  auto rewind = [&]() {
+    knext = kbase + (int64_t)tb * kstep;
+    vnext = vbase + (int64_t)tb * vstep;
+    left = w.n - tb * kKeyTile;
+  };
+  rewind();
+  auto issue = [&](int stage) __attribute__((always_inline)) {
+    uint32_t kb = kfull, vb = vfull;
+    if (left < kKeyTile) {
+      kb = (uint32_t)(left - 1) * (uint32_t)a.k_rs * 2u + ROWB;
+      vb = (uint32_t)(left - 1) * (uint32_t)a.v_rs * 2u + ROWB;
+    }
+    const i32x4_t rk = make_buffer_rsrc(knext, kb), rv = make_buffer_rsrc(vnext, vb);
     unsigned char* base = smem + stage * STAGE + wave * 1024;
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
       buffer_load_lds16(rk, base + i * W * 1024, koff0 + (uint32_t)(i * RPI * W) * (uint32_t)a.k_rs * 2u);
       buffer_load_lds16(rv, base + i * W * 1024 + TILEB, voff0 + (uint32_t)(i * RPI * W) * (uint32_t)a.v_rs * 2u);
     }
+    knext += kstep;
+    vnext += vstep;
+    left -= kKeyTile;
   };
   auto wait_tiles = [&](int n) __attribute__((always_inline)) {  // tiles that may stay in flight
     if (n <= 0) wait_vmcnt<0>();
@@ -420,7 +487,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
       if (!MODE || t + 1 < ntiles) {
         wait_tiles(min(NST - 3, ntiles - 2 - t));
         block_barrier();
-        if (t + NST - 1 < ntiles) issue((SG + NST - 1) % NST, t + NST - 1);
+        if (t + NST - 1 < ntiles) issue((SG + NST - 1) % NST);
         if (MODE ? sees(t + 1) : WORK) scores(nxt, smem + ((SG + 1) % NST) * STAGE);
       }
       if (MODE ? sees(t) : WORK) finish(cur, smem + SG * STAGE, t, mode);
@@ -442,7 +509,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
   if (ntiles > 0) {
 #pragma unroll
     for (int st = 0; st < NST - 1; ++st)
-      if (st < ntiles) issue(st, st);
+      if (st < ntiles) issue(st);
     wait_tiles(min(NST - 2, ntiles - 1));
     block_barrier();
     if (active) pipeline(std::true_type{});
@@ -454,6 +521,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 #pragma unroll
         for (int v = 0; v < 16; ++v) z = fmaf(o[d][v], 0.0f, z);
       if (__syncthreads_or(mine && z != 0.0f)) {
+        rewind();
         m_i = -INFINITY;
         l_i = 0.0f;
 #pragma unroll
@@ -463,7 +531,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 #pragma unroll 1
         for (int t = 0; t < ntiles; ++t) {
           __syncthreads();
-          issue(0, t);
+          issue(0);
           wait_vmcnt<0>();
           __syncthreads();
           if ((tb + t) * kKeyTile < kend_wave) {
@@ -479,8 +547,6 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
   // O^T: lane l, register v of block db -> dim 32 db + 8 (v / 4) + 4 g + v % 4 of row l32.
   if (!mine) return;
   const int orow = w.q0 + tok, ohead = h * a.G + head;
-  if (a.target && w.part == 0 && g == 0)
-    a.dir[(int64_t)orow * a.Hk * a.G + ohead] = make_int2(item, w.parts | (row - r0) << 16);
   if (w.parts > 1) {
     float* ws = a.ws + ((int64_t)item * a.Hk + h) * part_floats(R, DH);
     const int r = row - r0;
@@ -522,19 +588,21 @@ __global__ __launch_bounds__(256, 2) void packed_attn_keys_kernel(PackedAttn a) 
   typedef typename E::v8 v8;
   extern __shared__ __align__(16) unsigned char smem[];
 
-  const int item = blockIdx.x / a.Hk, h = blockIdx.x - item * a.Hk;
+  const int item = a.by_hk(blockIdx.x), h = blockIdx.x - item * a.Hk;
   Item w;
-  if (!find_item<R, WAVES * KEYS>(a, item, w)) return;
+  const bool found = find_item<R, WAVES * KEYS>(a, item, w);
+  note_merge<R>(a, item, h, found, w);
+  if (!found) return;
   const int lane = threadIdx.x & 63, l16 = lane & 15, G = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int total = w.m * a.G, r0 = w.tile * R, row = r0 + l16;
   const bool mine = row < total;
-  const int tok = row / a.G, head = row - tok * a.G;
+  const int tok = a.by_g(row), head = row - tok * a.G;
   const int lim = mine ? seen_keys(a, w, tok) : w.n;
-  const int kend = seen_keys(a, w, (min(r0 + R, total) - 1) / a.G);
-  const int lim_tile = seen_keys(a, w, r0 / a.G);
+  const int kend = seen_keys(a, w, a.by_g(min(r0 + R, total) - 1));
+  const int lim_tile = seen_keys(a, w, a.by_g(r0));
   constexpr int KT = WAVES * KEYS;
-  const int all_tiles = (kend + KT - 1) / KT, per = (all_tiles + w.parts - 1) / w.parts;
+  const int all_tiles = (kend + KT - 1) / KT, per = w.parts == 1 ? all_tiles : (all_tiles + w.parts - 1) / w.parts;
   const int kfirst = w.part * per * KT, klast = min(kend, kfirst + per * KT);  // this part's keys
   const int n32 = max(0, (klast - kfirst + KEYS - 1) / KEYS);
   const int cnt = (n32 - wave + WAVES - 1) / WAVES;  // tiles of this wave: wave, wave + 4, ...
@@ -733,9 +801,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_keys_kernel(PackedAttn a) 
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fmaf(src[e], f, x[e]);
   }
-  const int otok = (r0 + r) / a.G, orow = w.q0 + otok, ohead = h * a.G + (r0 + r - otok * a.G);
-  if (a.target && w.part == 0 && c == 0)
-    a.dir[(int64_t)orow * a.Hk * a.G + ohead] = make_int2(item, w.parts | r << 16);
+  const int otok = a.by_g(r0 + r), orow = w.q0 + otok, ohead = h * a.G + (r0 + r - otok * a.G);
   if (w.parts > 1) {
     float* ws = a.ws + ((int64_t)item * a.Hk + h) * part_floats(R, DH);
     if (c == 0) {
@@ -754,72 +820,78 @@ __global__ __launch_bounds__(256, 2) void packed_attn_keys_kernel(PackedAttn a) 
   *reinterpret_cast<v8*>(a.out + (int64_t)orow * a.o_rs + (int64_t)ohead * DH + 8 * c) = y;
 }
 
-// Merge of the key parts: a wave per (row, query head), DH / 8 lanes of 8 dims by 64 / (DH / 8) parts at a time.
-// With m = max_p m_p and f_p = 2^(c (m_p - m)): out = sum_p f_p o_p / sum_p f_p l_p. A part without a visible key has
-// l_p = 0 and is left out. Rows past the last sequence have no entry in the directory and are not read.
-template <class E, int DH>
-__global__ __launch_bounds__(256) void packed_attn_merge_kernel(PackedAttn a, int R) {
-  constexpr int CPR = DH / 8, PL = 64 / CPR, U = 4;
-  const int Hq = a.Hk * a.G;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int row = (int)(unit / Hq), head = (int)(unit - (int64_t)row * Hq);
-  if (row >= a.rows || row >= load_idx(a.cu_q, a.S, a.cu_wide, 0, a.rows) || row < load_idx(a.cu_q, 0, a.cu_wide, 0, a.rows))
-    return;
-  const int2 d = a.dir[unit];
-  const int parts = d.y & 0xffff, r = d.y >> 16;
-  // (offsets that do not rise leave rows without an entry: whatever lies there is not followed out of the workspace)
-  if (parts <= 1 || d.x < 0 || d.x > a.items - parts || r < 0 || r >= R) return;
-  const int lane = threadIdx.x & 63, c = lane % CPR, pl = lane / CPR;
+// Merge of the key parts of the items whose tile was split (workgroups of the others leave at once). With
+// m = max_p m_p and f_p = 2^(c (m_p - m)): out = sum_p f_p o_p / sum_p f_p l_p; a part without a visible key has l_p = 0
+// and is left out. DH / 8 lanes hold a row's dims; the other lanes of a wave take further parts of it (PL at a time,
+// tiles of few rows and many parts) or further rows (PL = 1). A part's order in the sums is fixed.
+static constexpr int kMergeRows = 32;  // rows of a workgroup
+template <class E, int DH, int R>
+__global__ __launch_bounds__(256) void packed_attn_merge_kernel(PackedAttn a) {
+  constexpr int CPR = DH / 8, LANES = 64 / CPR, PL = R == 16 ? LANES : 1, U = 4;
+  const int4 todo = a.heads[blockIdx.x];
+  const int parts = todo.x;
+  if (parts <= 1) return;
+  const int item = a.by_hk(blockIdx.x), h = blockIdx.x - item * a.Hk;
+  const int lane = threadIdx.x & 63, c = lane % CPR, pl = PL > 1 ? lane / CPR : 0;
   const int64_t stride = a.Hk * part_floats(R, DH);
-  const float* base = a.ws + ((int64_t)d.x * a.Hk + head / a.G) * part_floats(R, DH);
-  float m = -INFINITY, l = 0.0f, x[8] = {};
-  for (int p0 = pl; p0 < parts; p0 += PL * U) {
-    float mp[U], lp[U];
-    f32x4_t y[U][2];
+  const float* base = a.ws + ((int64_t)item * a.Hk + h) * part_floats(R, DH);
+  constexpr int STEP = 4 * (LANES / PL);  // rows of a workgroup at a time
+  const int first = blockIdx.y * kMergeRows, end = min(todo.w, first + kMergeRows);
+  for (int r0 = first; r0 < end; r0 += STEP) {
+    const int rr = r0 + (threadIdx.x / 64) * (LANES / PL) + (PL > 1 ? 0 : lane / CPR);
+    const int r = min(rr, end - 1);  // lanes past the end repeat the last row, for the exchanges below
+    float m = -INFINITY, l = 0.0f, x[8] = {};
+    for (int p0 = pl; p0 < parts; p0 += PL * U) {
+      float mp[U], lp[U];
+      f32x4_t y[U][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float* b = base + min(p0 + u * PL, parts - 1) * stride;
-      mp[u] = b[r];
-      lp[u] = p0 + u * PL < parts ? b[R + r] : 0.0f;
-      const f32x4_t* src = reinterpret_cast<const f32x4_t*>(b + 2 * R + (int64_t)r * DH + 8 * c);
-      y[u][0] = src[0];
-      y[u][1] = src[1];
-    }
-    float top = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (lp[u] != 0.0f) top = fmaxf(top, mp[u]);
-    const float tc = ref_shift(top, a.scale_log2);
-    const float keep = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
-    m = top;
-    l *= keep;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= keep;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (lp[u] != 0.0f) {
-        const float f = __builtin_amdgcn_exp2f(fmaf(mp[u], a.scale_log2, -tc));
-        l = fmaf(lp[u], f, l);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(y[u][e >> 2][e & 3], f, x[e]);
+      for (int u = 0; u < U; ++u) {
+        const float* b = base + min(p0 + u * PL, parts - 1) * stride;
+        mp[u] = b[r];
+        lp[u] = p0 + u * PL < parts ? b[R + r] : 0.0f;
+        const f32x4_t* src = reinterpret_cast<const f32x4_t*>(b + 2 * R + (int64_t)r * DH + 8 * c);
+        y[u][0] = src[0];
+        y[u][1] = src[1];
       }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (lp[u] != 0.0f) top = fmaxf(top, mp[u]);
+      const float tc = ref_shift(top, a.scale_log2);
+      const float keep = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= keep;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (lp[u] != 0.0f) {
+          const float f = __builtin_amdgcn_exp2f(fmaf(mp[u], a.scale_log2, -tc));
+          l = fmaf(lp[u], f, l);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = fmaf(y[u][e >> 2][e & 3], f, x[e]);
+        }
+    }
+    if constexpr (PL > 1) {
+#pragma unroll
+      for (int s = CPR; s < 64; s <<= 1) {
+        const float m2 = __shfl_xor(m, s, 64), top = fmaxf(m, m2), tc = ref_shift(top, a.scale_log2);
+        const float f = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
+        const float f2 = __builtin_amdgcn_exp2f(fmaf(m2, a.scale_log2, -tc));
+        m = top;
+        l = l * f + __shfl_xor(l, s, 64) * f2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * f + __shfl_xor(x[e], s, 64) * f2;
+      }
+    }
+    if (rr >= end || pl) continue;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= inv;
+    const int tok = a.by_g(todo.z + r), qh = todo.z + r - tok * a.G;
+    *reinterpret_cast<typename E::v8*>(a.out + (int64_t)(todo.y + tok) * a.o_rs + (int64_t)(h * a.G + qh) * DH + 8 * c) =
+        round8<E>(x);
   }
-#pragma unroll
-  for (int s = CPR; s < 64; s <<= 1) {
-    const float m2 = __shfl_xor(m, s, 64), top = fmaxf(m, m2), tc = ref_shift(top, a.scale_log2);
-    const float f = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
-    const float f2 = __builtin_amdgcn_exp2f(fmaf(m2, a.scale_log2, -tc));
-    m = top;
-    l = l * f + __shfl_xor(l, s, 64) * f2;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * f + __shfl_xor(x[e], s, 64) * f2;
-  }
-  if (pl) return;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] *= inv;
-  typename E::v8 y = round8<E>(x);
-  *reinterpret_cast<typename E::v8*>(a.out + (int64_t)row * a.o_rs + (int64_t)head * DH + 8 * c) = y;
 }
 
 }  // namespace oudjat
@@ -835,35 +907,32 @@ struct PackedShape {
   int64_t items;
 };
 
-static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh) {
+static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh, int64_t key_cap) {
   PackedShape s{};
   const int64_t G = Hq / Hk, seqs = std::max<int64_t>(1, std::min(S, rows));
   const int64_t mean = cdiv(rows * G, seqs);  // packed rows of a sequence
-  if (mean <= 32) {
-    s.R = 16;
-    s.min_tiles = 2;   // of 128 keys
-  } else {
-    s.R = Dh == 128 && mean > 128 ? 256 : 128;
-    s.min_tiles = 4;   // of 64 keys
-  }
+  s.R = mean <= 32 ? 16 : Dh == 128 && mean > 192 ? 256 : 128;
+  s.min_tiles = s.R == 16 ? 2 : 12;                      // of 128 and 64 keys
   const int64_t tiles = std::max(rows * G / s.R, seqs);  // about as many as there are
-  const int64_t want = 2 * kPackedCus;
-  s.target = tiles * Hk < 2 * want ? (int)cdiv(want, Hk) : 0;
-  // ceil of the sequences' tiles: one more than the rows' own for each that has rows; and the parts, with room for
-  // the rounding of the units' fp32 sum.
-  s.items = rows * G / s.R + seqs + (s.target ? s.target + s.target / 16 + 1 : 0);
+  const int64_t fill = s.R == 16 ? 4 * kPackedCus : kPackedCus;
+  if (tiles * Hk < fill && key_cap > 2048) s.target = (int)cdiv(kPackedCus, Hk);
+  // The most items: the ceil of every sequence's tiles is at most one more than its rows have; and the parts, with
+  // room for the rounding of the units' fp32 sum, but no tile has more than the cache's length allows.
+  const int64_t most = rows * G / s.R + seqs, most_parts = cdiv(cdiv(key_cap, s.R == 16 ? 128 : kKeyTile), s.min_tiles);
+  s.items = s.target ? std::min(most + s.target + s.target / 16 + 1, most * most_parts) : most;
   return s;
 }
 
 static int64_t packed_part_elems(const PackedShape& s, int64_t Hk, int64_t Dh) {
-  return s.items * Hk * part_floats(s.R, (int)Dh);
+  return s.items * Hk * (part_floats(s.R, (int)Dh) + 4);  // the results, then four ints each for the merge
 }
 
-extern "C" int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh) {
+extern "C" int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh,
+                                                           int64_t key_cap) {
   if (rows <= 0 || S <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || (Dh != 64 && Dh != 128) || rows * (Hq / Hk) >= 1 << 30)
     return 0;
-  const PackedShape s = packed_shape(rows, S, Hq, Hk, Dh);
-  return s.target ? packed_part_elems(s, Hk, Dh) + rows * Hq * 2 : 0;
+  const PackedShape s = packed_shape(rows, S, Hq, Hk, Dh, key_cap);
+  return s.target ? packed_part_elems(s, Hk, Dh) : 0;
 }
 
 // Allows a kernel `lds` bytes of dynamic LDS on the current device, once.
@@ -892,7 +961,7 @@ static int launch_rows(const PackedAttn& a, hipStream_t st, const char* what) {
 template <class E, int DH>
 static int launch_keys(const PackedAttn& a, hipStream_t st, const char* what) {
   static std::atomic<uint64_t> done{0};
-  constexpr int NS = DH == 128 ? 2 : 4, lds = 4 * 2 * NS * 32 * 2 * DH;  // 128 KB
+  constexpr int NS = 2, lds = 4 * 2 * NS * 32 * 2 * DH;
   const int rc = allow_lds((const void*)packed_attn_keys_kernel<E, DH, NS>, lds, done, what);
   if (rc != OUDJAT_OK) return rc;
   packed_attn_keys_kernel<E, DH, NS><<<(unsigned)a.items * a.Hk, 256, lds, st>>>(a);
@@ -903,11 +972,12 @@ template <class E, int DH>
 static int launch_packed(const PackedAttn& a, int R, hipStream_t st, const char* what) {
   int rc;
   if (R == 16) rc = launch_keys<E, DH>(a, st, what);
-  else if constexpr (DH == 128) rc = R == 256 ? launch_rows<E, DH, 8>(a, st, what) : launch_rows<E, DH, 4>(a, st, what);
-  else rc = launch_rows<E, DH, 4>(a, st, what);
+  else rc = R == 256 ? launch_rows<E, DH, 8>(a, st, what) : launch_rows<E, DH, 4>(a, st, what);
   if (rc != OUDJAT_OK || !a.target) return rc;
-  const unsigned grid = (unsigned)cdiv((int64_t)a.rows * a.Hk * a.G, 4);
-  packed_attn_merge_kernel<E, DH><<<grid, 256, 0, st>>>(a, R);
+  const dim3 grid((unsigned)a.items * a.Hk, (unsigned)cdiv(R, kMergeRows));
+  if (R == 16) packed_attn_merge_kernel<E, DH, 16><<<grid, 256, 0, st>>>(a);
+  else if (R == 128) packed_attn_merge_kernel<E, DH, 128><<<grid, 256, 0, st>>>(a);
+  else packed_attn_merge_kernel<E, DH, 256><<<grid, 256, 0, st>>>(a);
   return check_launch("packed_attention (merge)");
 }
 
@@ -939,16 +1009,16 @@ extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t 
   OUDJAT_REQUIRE(rows * (Hq / Hk) < (1 << 30) && Hq <= 65535 && S < (1 << 24) && key_cap < (1 << 30) &&
                      k_rs < (1 << 24) && v_rs < (1 << 24),
                  OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
-  const PackedShape s = packed_shape(rows, S, Hq, Hk, Dh);
+  const PackedShape s = packed_shape(rows, S, Hq, Hk, Dh, key_cap);
   OUDJAT_REQUIRE(s.items * Hk < (1 << 23), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   const int64_t parts = s.target ? packed_part_elems(s, Hk, Dh) : 0;
-  OUDJAT_REQUIRE(!s.target || (workspace && aligned(workspace, 16) && workspace_elems >= parts + rows * Hq * 2),
+  OUDJAT_REQUIRE(!s.target || (workspace && aligned(workspace, 16) && workspace_elems >= parts),
                  OUDJAT_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld elements is needed", what,
-                 (long long)(parts + rows * Hq * 2));
+                 (long long)parts);
   const PackedAttn a{q, q_rs, q_hs, k, v, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, cu_q, keys, out, out_rs, (int)rows, (int)S,
-                     (int)Hk, (int)(Hq / Hk), (int)key_cap, cu_wide != 0, keys_wide != 0, batched != 0, causal != 0,
+                     (int)Hk, (int)(Hq / Hk), Divisor((uint32_t)Hk), Divisor((uint32_t)(Hq / Hk)), (int)key_cap, cu_wide != 0, keys_wide != 0, batched != 0, causal != 0,
                      scale * 1.4426950408889634f, s.target, s.min_tiles, (int)s.items, workspace,
-                     s.target ? reinterpret_cast<int2*>(workspace + parts) : nullptr};
+                     s.target ? reinterpret_cast<int4*>(workspace + s.items * Hk * part_floats(s.R, (int)Dh)) : nullptr};
   hipStream_t st = as_stream(stream);
   if (dtype == OUDJAT_BF16)
     return Dh == 64 ? launch_packed<AttnBf16, 64>(a, s.R, st, what) : launch_packed<AttnBf16, 128>(a, s.R, st, what);

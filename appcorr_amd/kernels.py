@@ -1334,25 +1334,36 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16}
 _POS_TYPES = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32}
 
 
-def _launch_on(tag: str, t: torch.Tensor, name: str, *args) -> None:
-    """_launch with the tensor's device as the current one (its stream is that device's)."""
-    if t.device.index == torch.cuda.current_device():
+def _gpu_of(*tensors: torch.Tensor | None) -> int:
+    """The device index that all given tensors share; raises as _require_cuda does."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            _require_cuda(*tensors)
+    return dev
+
+
+def _launch_on(tag: str, dev: int, t: torch.Tensor, name: str, *args) -> None:
+    """_launch with the tensors' device as the current one (its stream is that device's)."""
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            _launch(tag, t, name, *args)
+    elif tag in _probe["tags"]:
         _launch(tag, t, name, *args)
     else:
-        with torch.cuda.device(t.device):
-            _launch(tag, t, name, *args)
+        call(name, *args)
 
 
-def _stride(t: torch.Tensor, *dims: int) -> tuple:
-    """Strides of the dims as the kernels see them: 0 where there is only one entry (torch keeps any number)."""
-    return tuple(0 if t.shape[d] == 1 else t.stride(d) for d in dims)
+def _strides(t: torch.Tensor, n: int):
+    """Strides of the first n dims as the kernels see them: 0 where there is only one entry (torch keeps any number)."""
+    shape, stride = t.shape, t.stride()
+    if 1 not in shape:
+        return stride[:n]
+    return [0 if shape[d] == 1 else stride[d] for d in range(n)]
 
 
-def _lengths(t: torch.Tensor, n: int | None, what: str) -> torch.Tensor:
-    _require(t.dtype in (torch.int32, torch.int64) and t.dim() == 1 and t.is_contiguous()
-             and (n is None or t.numel() == n), f"{what} must be contiguous 1-D int32 or int64" +
-             ("" if n is None else f" of {n} entries"))
-    return t
+def _is_lengths(t: torch.Tensor, n: int) -> bool:
+    return t.dim() == 1 and t.dtype in (torch.int32, torch.int64) and t.is_contiguous() and t.numel() == n
 
 
 @dataclass
@@ -1375,34 +1386,43 @@ def packed_plan(q_lens: torch.Tensor, k_lens: torch.Tensor, rows: int, *, cache_
     key_rows (keys packed like the queries in that many rows) is given. Row r of sequence s is token_idx[r] of
     batch_idx[r] = s, which is also its position there; rows behind the last sequence and rows that come before
     token 0 have -1, -1. Lengths below 0 count as 0; rows past `rows` are cut off. At most 4096 sequences."""
-    _require_cuda(q_lens, k_lens)
+    dev = _gpu_of(q_lens, k_lens)
     S = q_lens.numel()
-    _lengths(q_lens, None, "packed_plan: q_lens")
-    _lengths(k_lens, S, "packed_plan: k_lens")
+    _require(_is_lengths(q_lens, S) and _is_lengths(k_lens, S),
+             "packed_plan: q_lens and k_lens must be contiguous 1-D int32 or int64 of one length")
     _require((cache_len is None) != (key_rows is None), "packed_plan: one of cache_len and key_rows")
-    dev = q_lens.device
-    plan = PackedPlan(cu_q=torch.empty(S + 1, device=dev, dtype=torch.int32),
-                      k_lens=torch.empty(S, device=dev, dtype=torch.int32),
-                      cu_k=torch.empty(S + 1, device=dev, dtype=torch.int64),
-                      batch_idx=torch.empty(rows, device=dev, dtype=torch.int64),
-                      token_idx=torch.empty(rows, device=dev, dtype=torch.int64))
-    _launch_on("packed_plan", q_lens, "oudjat_packed_plan", _ptr(q_lens), int(q_lens.dtype == torch.int64), _ptr(k_lens),
-               int(k_lens.dtype == torch.int64), S, rows, key_rows if cache_len is None else cache_len,
-               int(cache_len is None), _ptr(plan.cu_q), _ptr(plan.k_lens), _ptr(plan.cu_k), _ptr(plan.batch_idx),
-               _ptr(plan.token_idx), _stream(q_lens))
+    _require(rows >= 0, "packed_plan: negative number of rows")
+    device = q_lens.device
+    plan = PackedPlan(torch.empty(S + 1, device=device, dtype=torch.int32),
+                      torch.empty(S, device=device, dtype=torch.int32),
+                      torch.empty(S + 1, device=device, dtype=torch.int64),
+                      torch.empty(rows, device=device, dtype=torch.int64),
+                      torch.empty(rows, device=device, dtype=torch.int64))
+    _launch_on("packed_plan", dev, q_lens, "oudjat_packed_plan", q_lens.data_ptr(), q_lens.dtype == torch.int64,
+               k_lens.data_ptr(), k_lens.dtype == torch.int64, S, rows, key_rows if cache_len is None else cache_len,
+               cache_len is None, plan.cu_q.data_ptr(), plan.k_lens.data_ptr(), plan.cu_k.data_ptr(),
+               plan.batch_idx.data_ptr(), plan.token_idx.data_ptr(), _lib.stream_of(q_lens))
     return plan
 
 
-def _axis_rope(positions: torch.Tensor, inv_freq: torch.Tensor, sections, rows: int, what: str):
-    """The position arguments of the C entry points, and the host array that they point to."""
-    _require(positions.dim() == 2 and positions.shape[0] == rows and positions.dtype in _POS_TYPES,
-             f"{what}: positions must be [rows, axes] int32, int64 or fp32")
-    _require(len(sections) == positions.shape[1], f"{what}: one section per axis of positions")
-    _require(inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
-             and inv_freq.numel() == sum(sections), f"{what}: inv_freq must be contiguous fp32 [sum(sections)]")
-    host = (ctypes.c_int64 * max(1, len(sections)))(*sections)
-    return host, (_ptr(positions), _POS_TYPES[positions.dtype], positions.stride(0), positions.stride(1),
-                  len(sections), _ptr(inv_freq), ctypes.addressof(host))
+_SECTIONS: dict = {}
+
+
+def _axis_rope(positions: torch.Tensor, inv_freq: torch.Tensor, sections, rows: int, what: str) -> tuple:
+    """The position arguments of the C entry points."""
+    sections = tuple(sections)
+    host = _SECTIONS.get(sections)
+    if host is None:  # the host array that the call reads: one per distinct sections, kept
+        host = _SECTIONS[sections] = ((ctypes.c_int64 * max(1, len(sections)))(*sections), sum(sections))
+    if positions.dim() != 2 or positions.shape[0] != rows or positions.dtype not in _POS_TYPES:
+        raise ValueError(f"{what}: positions must be [rows, axes] int32, int64 or fp32")
+    if len(sections) != positions.shape[1]:
+        raise ValueError(f"{what}: one section per axis of positions")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
+            or inv_freq.numel() != host[1]:
+        raise ValueError(f"{what}: inv_freq must be contiguous fp32 [sum(sections)]")
+    return (positions.data_ptr(), _POS_TYPES[positions.dtype], *positions.stride(), len(sections), inv_freq.data_ptr(),
+            ctypes.addressof(host[0]))
 
 
 def apply_rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections,
@@ -1414,19 +1434,24 @@ def apply_rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, i
     inv_freq[i] radians, formed in 64 bits; dims from R on stay. Position 0 leaves a row as it is (cls and
     register tokens). bf16 or fp16; q and k may be views of a qkv row with packed heads' last dim. `out` =
     (q_out, k_out) receives the result and may be (q, k): in place."""
-    what = "apply_rope_axes"
-    oq, ok = out if out is not None else (torch.empty_like(q, memory_format=torch.contiguous_format),
-                                          torch.empty_like(k, memory_format=torch.contiguous_format))
-    _require_cuda(q, k, positions, inv_freq, oq, ok)
     _require(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
-             f"{what}: q [M, Hq, Dh] and k [M, Hk, Dh]")
-    _require(q.dtype in _DTYPES and q.dtype == k.dtype == oq.dtype == ok.dtype, f"{what}: bf16 or fp16, one type")
-    _require(oq.shape == q.shape and ok.shape == k.shape, f"{what}: out must have the shapes of q and k")
-    _require(all(t.stride(2) == 1 for t in (q, k, oq, ok)), f"{what}: the head dim must be contiguous")
-    host, pos = _axis_rope(positions, inv_freq, sections, q.shape[0], what)
-    _launch_on("rope_axes", q, "oudjat_rope_axes", _ptr(q), *_stride(q, 0, 1), _ptr(k), *_stride(k, 0, 1), q.shape[0],
-               q.shape[1], k.shape[1], q.shape[2], _DTYPES[q.dtype], *pos, _ptr(oq), *_stride(oq, 0, 1), _ptr(ok),
-               *_stride(ok, 0, 1), _stream(q))
+             "apply_rope_axes: q [M, Hq, Dh] and k [M, Hk, Dh]")
+    if out is None:
+        oq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        ok = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    else:
+        oq, ok = out
+        _require(oq.shape == q.shape and ok.shape == k.shape, "apply_rope_axes: out must have the shapes of q and k")
+    dev = _gpu_of(q, k, positions, inv_freq, oq, ok)
+    _require(q.dtype in _DTYPES and q.dtype == k.dtype == oq.dtype == ok.dtype,
+             "apply_rope_axes: bf16 or fp16, one type")
+    _require(q.stride(2) == 1 and k.stride(2) == 1 and oq.stride(2) == 1 and ok.stride(2) == 1,
+             "apply_rope_axes: the head dim must be contiguous")
+    M, Hq, Dh = q.shape
+    pos = _axis_rope(positions, inv_freq, sections, M, "apply_rope_axes")
+    _launch_on("rope_axes", dev, q, "oudjat_rope_axes", q.data_ptr(), *_strides(q, 2), k.data_ptr(), *_strides(k, 2), M,
+               Hq, k.shape[1], Dh, _DTYPES[q.dtype], *pos, oq.data_ptr(), *_strides(oq, 2), ok.data_ptr(),
+               *_strides(ok, 2), _lib.stream_of(q))
     return oq, ok
 
 
@@ -1440,30 +1465,32 @@ def qk_norm_rope_kv(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm, k_norm
     (x / sqrt(mean(x^2) + eps) * weight), or LayerNorm with layer_norm=True. Positions, inv_freq and sections as in
     apply_rope_axes. fp32 arithmetic, rounded once. Rows with a slot outside the cache (packed_plan's -1) are
     skipped: q_out and the cache keep what they held. The other rows' slots must be unique. Dh 64 or 128."""
-    what = "qk_norm_rope_kv"
     qw, qb = q_norm
     kw, kb = k_norm
-    _require_cuda(qkv, qw, qb, kw, kb, positions, inv_freq, batch_idx, token_idx, kv_cache, q_out)
+    dev = _gpu_of(qkv, qw, qb, kw, kb, positions, inv_freq, batch_idx, token_idx, kv_cache, q_out)
+    dtype = qkv.dtype
     _require(heads > 0 and kv_heads > 0 and qkv.dim() == 3 and qkv.shape[1] == heads + 2 * kv_heads
-             and qkv.dtype in _DTYPES and trailing_is_packed(qkv, 1),
-             f"{what}: qkv must be [M, heads + 2 kv_heads, Dh] bf16 or fp16 with packed rows")
+             and dtype in _DTYPES and trailing_is_packed(qkv, 1),
+             "qk_norm_rope_kv: qkv must be [M, heads + 2 kv_heads, Dh] bf16 or fp16 with packed rows")
     M, _, Dh = qkv.shape
     for w in (qw, qb, kw, kb):
-        _require(w is None or (w.dtype == qkv.dtype and w.numel() == Dh and w.is_contiguous()),
-                 f"{what}: norm weights must be contiguous [Dh] of qkv's type")
-    _require(layer_norm or (qb is None and kb is None), f"{what}: a bias needs layer_norm=True")
-    _require(kv_cache.dim() == 5 and kv_cache.shape[2:] == (2, kv_heads, Dh) and kv_cache.dtype == qkv.dtype
-             and trailing_is_packed(kv_cache, 3), f"{what}: kv_cache must be [B, N, 2, kv_heads, Dh] of qkv's type "
-             "with packed heads")
-    _require(q_out.shape == (M, heads, Dh) and q_out.dtype == qkv.dtype and trailing_is_packed(q_out, 1),
-             f"{what}: q_out must be [M, heads, Dh] of qkv's type with packed rows")
+        _require(w is None or (w.dtype == dtype and w.numel() == Dh and w.is_contiguous()),
+                 "qk_norm_rope_kv: norm weights must be contiguous [Dh] of qkv's type")
+    _require(layer_norm or (qb is None and kb is None), "qk_norm_rope_kv: a bias needs layer_norm=True")
+    _require(kv_cache.dim() == 5 and kv_cache.shape[2:] == (2, kv_heads, Dh) and kv_cache.dtype == dtype
+             and trailing_is_packed(kv_cache, 3),
+             "qk_norm_rope_kv: kv_cache must be [B, N, 2, kv_heads, Dh] of qkv's type with packed heads")
+    _require(q_out.shape == (M, heads, Dh) and q_out.dtype == dtype and trailing_is_packed(q_out, 1),
+             "qk_norm_rope_kv: q_out must be [M, heads, Dh] of qkv's type with packed rows")
     bi, ti = _index(batch_idx, "batch_idx"), _index(token_idx, "token_idx")
-    _require(bi.numel() == M and ti.numel() == M, f"{what}: one slot per row")
-    host, pos = _axis_rope(positions, inv_freq, sections, M, what)
-    _launch_on("qkv_post", qkv, "oudjat_qk_norm_rope_kv", _ptr(qkv), *_stride(qkv, 0), M, heads, kv_heads, Dh,
-               _DTYPES[qkv.dtype], int(layer_norm), _ptr(qw), _ptr(qb), _ptr(kw), _ptr(kb), float(eps), *pos, _ptr(bi),
-               _ptr(ti), _ptr(kv_cache), *_stride(kv_cache, 0, 1, 2), kv_cache.shape[0], kv_cache.shape[1], _ptr(q_out),
-               *_stride(q_out, 0), _stream(qkv))
+    _require(bi.numel() == M and ti.numel() == M, "qk_norm_rope_kv: one slot per row")
+    pos = _axis_rope(positions, inv_freq, sections, M, "qk_norm_rope_kv")
+    _launch_on("qkv_post", dev, qkv, "oudjat_qk_norm_rope_kv", qkv.data_ptr(), *_strides(qkv, 1), M, heads, kv_heads, Dh,
+               _DTYPES[dtype], layer_norm, qw.data_ptr() if qw is not None else 0,
+               qb.data_ptr() if qb is not None else 0, kw.data_ptr() if kw is not None else 0,
+               kb.data_ptr() if kb is not None else 0, eps, *pos, bi.data_ptr(), ti.data_ptr(), kv_cache.data_ptr(),
+               *_strides(kv_cache, 3), kv_cache.shape[0], kv_cache.shape[1], q_out.data_ptr(), *_strides(q_out, 1),
+               _lib.stream_of(qkv))
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, keys: torch.Tensor,
@@ -1478,33 +1505,35 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     A row without keys gives 0; hidden keys have no influence, NaN or infinite ones neither. Rows of `out` behind
     the last sequence stay as they were (undefined in a new tensor). scale must be positive. bf16 or fp16; Dh 64
     or 128. With few query rows the keys of a sequence are split over workgroups and merged, in a fixed order."""
-    what = "packed_attention"
-    _require_cuda(q, k, v, cu_q, keys, out)
     _require(q.dim() == 3 and k.dim() in (3, 4) and k.shape == v.shape and k.shape[-1] == q.shape[2],
-             f"{what}: q [M, Hq, Dh], k and v [Mk, Hk, Dh] or [B, N, Hk, Dh]")
-    _require(q.dtype in _DTYPES and q.dtype == k.dtype == v.dtype, f"{what}: bf16 or fp16, one type")
-    _require(all(t.stride(-1) == 1 for t in (q, k, v)), f"{what}: the head dim must be contiguous")
+             "packed_attention: q [M, Hq, Dh], k and v [Mk, Hk, Dh] or [B, N, Hk, Dh]")
     M, Hq, Dh = q.shape
-    batched = k.dim() == 4
-    Hk = k.shape[-2]
-    _lengths(cu_q, None, f"{what}: cu_q")
-    S = cu_q.numel() - 1
-    _require(S >= 0, f"{what}: cu_q must have one entry more than sequences")
-    _lengths(keys, S if batched else S + 1, f"{what}: keys")
-    _require(not batched or k.shape[0] >= S, f"{what}: the cache has fewer batches than sequences")
+    dtype = q.dtype
     if out is None:
-        out = torch.empty((M, Hq * Dh), device=q.device, dtype=q.dtype)
-    _require(out.shape == (M, Hq * Dh) and out.dtype == q.dtype and out.stride(1) == 1,
-             f"{what}: out must be [M, Hq * Dh] of q's type with contiguous rows")
-    wkey = ("packed_attention", M, S, Hq, Hk, Dh)
+        out = torch.empty((M, Hq * Dh), device=q.device, dtype=dtype)
+    dev = _gpu_of(q, k, v, cu_q, keys, out)
+    _require(dtype in _DTYPES and dtype == k.dtype == v.dtype == out.dtype,
+             "packed_attention: bf16 or fp16, one type")
+    _require(q.stride(2) == 1 and k.stride(-1) == 1 and v.stride(-1) == 1 and out.shape == (M, Hq * Dh)
+             and out.stride(1) == 1, "packed_attention: contiguous head dims, out [M, Hq * Dh] with contiguous rows")
+    batched = k.dim() == 4
+    cap, Hk = k.shape[-3], k.shape[-2]
+    S = cu_q.numel() - 1
+    _require(S >= 0 and _is_lengths(cu_q, S + 1) and _is_lengths(keys, S if batched else S + 1),
+             "packed_attention: cu_q [S + 1] and keys ([S] of a cache, [S + 1] packed) must be contiguous int32 or int64")
+    _require(not batched or k.shape[0] >= S, "packed_attention: the cache has fewer batches than sequences")
+    wkey = ("packed_attention", M, S, Hq, Hk, Dh, cap)
     elems = _WS_ELEMS.get(wkey)
     if elems is None:
-        elems = int(_lib.load().oudjat_packed_attention_workspace_elems(M, S, Hq, Hk, Dh))
+        elems = int(_lib.load().oudjat_packed_attention_workspace_elems(*wkey[1:]))
         _WS_ELEMS[wkey] = elems
     ws = _stream_workspace(q, elems) if elems > 0 else None
-    sk, sv = (_stride(t, 0, 1, 2) if batched else (0, *_stride(t, 0, 1)) for t in (k, v))
-    _launch_on("attention", q, "oudjat_packed_attention", _ptr(q), *_stride(q, 0, 1), M, Hq, Dh, _ptr(k), *sk,
-               _ptr(v), *sv, Hk, k.shape[-3], int(batched), _ptr(cu_q), int(cu_q.dtype == torch.int64), _ptr(keys),
-               int(keys.dtype == torch.int64), S, float(scale), int(causal), _DTYPES[q.dtype], _ptr(out), *_stride(out, 0),
-               _ptr(ws), 0 if ws is None else ws.numel(), _stream(q))
+    if batched:
+        sk, sv = _strides(k, 3), _strides(v, 3)
+    else:
+        sk, sv = (0, *_strides(k, 2)), (0, *_strides(v, 2))
+    _launch_on("attention", dev, q, "oudjat_packed_attention", q.data_ptr(), *_strides(q, 2), M, Hq, Dh, k.data_ptr(),
+               *sk, v.data_ptr(), *sv, Hk, cap, batched, cu_q.data_ptr(), cu_q.dtype == torch.int64, keys.data_ptr(),
+               keys.dtype == torch.int64, S, scale, causal, _DTYPES[dtype], out.data_ptr(), *_strides(out, 1),
+               0 if ws is None else ws.data_ptr(), elems, _lib.stream_of(q))
     return out

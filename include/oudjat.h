@@ -804,7 +804,8 @@ int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64
                             const void* cu_q, int cu_wide, const void* keys, int keys_wide, int64_t S, float scale,
                             int causal, int dtype, uint16_t* out, int64_t out_rs, float* workspace,
                             int64_t workspace_elems, oudjat_stream_t stream);
-int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh);
+int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh,
+                                                int64_t key_cap);
 
 #ifdef __cplusplus
 }
