@@ -55,7 +55,7 @@ struct PackedAttn {
   int rows, S, Hk, G;
   Divisor by_hk, by_g;
   int key_cap;
-  bool cu_wide, keys_wide, batched, causal;
+  bool cu_wide, keys_wide, batched, causal, search;
   float scale_log2;
   // Key parts: 0 = never split; else the number of parts that a key head's items are cut into at the most, beside
   // their own number, and the fewest key tiles of a part.
@@ -116,8 +116,11 @@ __device__ __forceinline__ typename E::v8 round8(const float* f) {
 }
 
 __device__ __forceinline__ int load_idx(const void* p, int i, bool wide, int lo, int hi) {
-  const int64_t v = wide ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
-  return v < lo ? lo : (v > hi ? hi : (int)v);
+  if (wide) {
+    const int64_t v = static_cast<const int64_t*>(p)[i];
+    return v < lo ? lo : (v > hi ? hi : (int)v);
+  }
+  return max(lo, min(hi, static_cast<const int32_t*>(p)[i]));
 }
 
 // A sequence's rows and keys, and the item that a workgroup takes of it. Uniform over the wave.
@@ -161,45 +164,68 @@ __device__ __forceinline__ float last_lane(float x) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), 63));
 }
 
-static constexpr int kSortedSeqs = 256;
-
-// Item number `item` of a key head, tiles of R packed rows and KT keys; false past the last. Parts of a sequence's
-// tiles: ceil(its key tiles / C), with C = max(min_tiles, units / target) and units the key tiles of all tiles, so
-// that a key head has at most its own tiles + target items. Up to kSortedSeqs sequences the items of the longer ones
-// (more than half of the longest's keys, then more than a quarter) come first, so that the last workgroups are short.
+// Item number `item` of a key head, tiles of R packed rows and KT keys; false if there is none. Two numberings:
+//
+// Scan (up to 64 sequences, or any number if keys are split): the sequences' items one after another, 64 sequences at
+// a time. Parts of a sequence's tiles: its key tiles / C, rounded, with C = max(min_tiles, units / target) and units the
+// key tiles of all tiles, so that a key head has at most its own tiles + target items. Up to 64 sequences the items of the
+// longer ones (more than half of the longest's keys, then more than a quarter) come first, so that the last
+// workgroups are short.
+//
+// Search (more sequences, no split): sequence s starts at number floor(cu_q[s] G / R) + s, which leaves room for all
+// its tiles, so that the sequence of a number is found by a 64-way search in cu_q, two loads up to 4096 sequences
+// (one token each of 4096 sequences, 16 over 4 heads of 64, 200 keys: SEARCHMEAS).
 template <int R, int KT>
-__device__ __forceinline__ bool find_item(const PackedAttn& a, int item, Item& w) {
+__device__ __forceinline__ bool search_item(const PackedAttn& a, int item, Item& w) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = a.S;
+  while (true) {  // the last s of lo .. lo + n - 1 that starts at or before the item
+    const int step = (n + 63) / 64, s = lo + lane * step;
+    const bool before = s < lo + n && load_idx(a.cu_q, s, a.cu_wide, 0, a.rows) * a.G / R + s <= item;
+    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
+    if (c == 0) return false;
+    lo += (c - 1) * step;
+    if (step == 1) break;
+    n = min(step, a.S - lo);
+  }
+  load_seq(a, lo, w);
+  const int tiles = (w.m * a.G + R - 1) / R, from_first = item - (w.q0 * a.G / R + lo);
+  w.seq = lo;
+  w.part = 0;
+  w.parts = 1;
+  w.tile = tiles - 1 - from_first;
+  return from_first >= 0 && w.tile >= 0;
+}
+
+template <int R, int KT>
+__device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w) {
   const int lane = threadIdx.x & 63;
   Item t;
-  int chunk = 1 << 30, top = 0;
-  auto tiles = [&]() { return (int)(((int64_t)t.m * a.G + R - 1) / R); };
+  int chunk = 1, top = 0;
+  auto tiles = [&]() { return (t.m * a.G + R - 1) / R; };
   auto key_tiles = [&]() { return (t.n + KT - 1) / KT; };
   auto load = [&](int s0) {
     t.q0 = t.m = t.n = t.k0 = 0;
     if (s0 + lane < a.S) load_seq(a, s0 + lane, t);
   };
   load(0);
-  const bool sorted = a.S <= kSortedSeqs;
-  if (a.target || sorted) {
+  const bool sorted = a.S <= 64;
+  if (a.target) {
     float units = (float)tiles() * (float)key_tiles();
-    top = key_tiles();
     for (int s0 = 64; s0 < a.S; s0 += 64) {
       load(s0);
       units += (float)tiles() * (float)key_tiles();
-      top = max(top, key_tiles());
     }
-    if (a.target) {
-      units = last_lane(wave_scan(units, [](float x, float y) { return x + y; }));
-      chunk = max(a.min_tiles, (int)ceilf(units / (float)a.target));
-    }
-    top = last_lane(wave_scan(top, [](int x, int y) { return max(x, y); }));
-    if (a.S > 64) load(0);
+    units = last_lane(wave_scan(units, [](float x, float y) { return x + y; }));
+    chunk = max(a.min_tiles, (int)ceilf(units / (float)a.target));
+    if (!sorted) load(0);
   }
+  if (sorted) top = last_lane(wave_scan(key_tiles(), [](int x, int y) { return max(x, y); }));
   int base = 0;
   for (int cls = 0; cls < (sorted ? 3 : 1); ++cls) {
     for (int s0 = 0; s0 < a.S; s0 += 64) {
-      if (a.S > 64 && (s0 || cls)) load(s0);
-      const int nt = tiles(), kt = key_tiles(), parts = a.target ? max(1, (kt + chunk - 1) / chunk) : 1;
+      if (s0) load(s0);
+      const int nt = tiles(), kt = key_tiles(), parts = a.target ? max(1, (2 * kt + chunk) / (2 * chunk)) : 1;
       const int mine = !sorted || (2 * kt > top ? 0 : 4 * kt > top ? 1 : 2) == cls ? nt * parts : 0;
       const int incl = wave_scan(mine, [](int x, int y) { return x + y; });
       const int total = last_lane(incl);
@@ -223,13 +249,37 @@ __device__ __forceinline__ bool find_item(const PackedAttn& a, int item, Item& w
   return false;
 }
 
-// What the merge has to do from this item on (every workgroup of the grid says it, those without an item too).
-template <int R>
-__device__ __forceinline__ void note_merge(const PackedAttn& a, int item, int h, bool found, const Item& w) {
-  if (!a.target || threadIdx.x) return;
-  int4 x = make_int4(0, 0, 0, 0);
-  if (found && w.part == 0 && w.parts > 1) x = make_int4(w.parts, w.q0, w.tile * R, min(R, w.m * a.G - w.tile * R));
-  a.heads[(int64_t)item * a.Hk + h] = x;
+// The workgroup's item, found by its first wave (the others wait: the search is instructions that a neighbour on the
+// CU could issue); false past the last. And what the merge has to do from this item on, which every workgroup of the
+// grid says, those without an item too.
+template <int R, int KT>
+__device__ __forceinline__ bool take_item(const PackedAttn& a, int item, int h, Item& w) {
+  __shared__ int shared[9];
+  if (threadIdx.x < 64) {
+    w = Item{};
+    const bool found = a.search ? search_item<R, KT>(a, item, w) : scan_item<R, KT>(a, item, w);
+    if (threadIdx.x == 0) {
+      if (a.target) {
+        int4 x = make_int4(0, 0, 0, 0);
+        if (found && w.part == 0 && w.parts > 1)
+          x = make_int4(w.parts, w.q0, w.tile * R, min(R, w.m * a.G - w.tile * R));
+        a.heads[(int64_t)item * a.Hk + h] = x;
+      }
+      shared[0] = w.seq;
+      shared[1] = w.q0;
+      shared[2] = w.m;
+      shared[3] = w.n;
+      shared[4] = w.k0;
+      shared[5] = w.tile;
+      shared[6] = w.part;
+      shared[7] = w.parts;
+      shared[8] = found;
+    }
+  }
+  __syncthreads();
+  auto get = [&](int i) { return __builtin_amdgcn_readfirstlane(shared[i]); };
+  w = Item{get(0), get(1), get(2), get(3), get(4), get(5), get(6), get(7)};
+  return get(8) != 0;
 }
 
 // Keys that token i of the sequence sees.
@@ -297,9 +347,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 
   const int item = a.by_hk(blockIdx.x), h = blockIdx.x - item * a.Hk;
   Item w;
-  const bool found = find_item<R, kKeyTile>(a, item, w);
-  note_merge<R>(a, item, h, found, w);
-  if (!found) return;
+  if (!take_item<R, kKeyTile>(a, item, h, w)) return;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int total = w.m * a.G;                       // packed rows of the sequence
@@ -340,8 +388,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
   const uint16_t *knext, *vnext;
   int left;
   const int64_t kstep = kKeyTile * a.k_rs, vstep = kKeyTile * a.v_rs;
-  const uint32_t kfull = (uint32_t)(kKeyTile - 1) * (uint32_t)a.k_rs * 2u + ROWB;
-  const uint32_t vfull = (uint32_t)(kKeyTile - 1) * (uint32_t)a.v_rs * 2u + ROWB;
+  const uint32_t krow = (uint32_t)a.k_rs * 2u, vrow = (uint32_t)a.v_rs * 2u;
   auto rewind = [&]() {
     knext = kbase + (int64_t)tb * kstep;
     vnext = vbase + (int64_t)tb * vstep;
@@ -349,17 +396,13 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
   };
   rewind();
   auto issue = [&](int stage) __attribute__((always_inline)) {
-    uint32_t kb = kfull, vb = vfull;
-    if (left < kKeyTile) {
-      kb = (uint32_t)(left - 1) * (uint32_t)a.k_rs * 2u + ROWB;
-      vb = (uint32_t)(left - 1) * (uint32_t)a.v_rs * 2u + ROWB;
-    }
-    const i32x4_t rk = make_buffer_rsrc(knext, kb), rv = make_buffer_rsrc(vnext, vb);
+    const uint32_t last = (uint32_t)(min(left, kKeyTile) - 1);
+    const i32x4_t rk = make_buffer_rsrc(knext, last * krow + ROWB), rv = make_buffer_rsrc(vnext, last * vrow + ROWB);
     unsigned char* base = smem + stage * STAGE + wave * 1024;
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
-      buffer_load_lds16(rk, base + i * W * 1024, koff0 + (uint32_t)(i * RPI * W) * (uint32_t)a.k_rs * 2u);
-      buffer_load_lds16(rv, base + i * W * 1024 + TILEB, voff0 + (uint32_t)(i * RPI * W) * (uint32_t)a.v_rs * 2u);
+      buffer_load_lds16(rk, base + i * W * 1024, koff0 + (uint32_t)(i * RPI * W) * krow);
+      buffer_load_lds16(rv, base + i * W * 1024 + TILEB, voff0 + (uint32_t)(i * RPI * W) * vrow);
     }
     knext += kstep;
     vnext += vstep;
@@ -485,15 +528,16 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
     auto step = [&](auto stage_c, int t, Scores& cur, Scores& nxt, auto mode) __attribute__((always_inline)) {
       constexpr int SG = decltype(stage_c)::value, MODE = decltype(mode)::value;
       if (!MODE || t + 1 < ntiles) {
-        wait_tiles(min(NST - 3, ntiles - 2 - t));
+        if (MODE) wait_tiles(min(NST - 3, ntiles - 2 - t));
+        else wait_vmcnt<2 * LPW * (NST - 3)>();
         block_barrier();
-        if (t + NST - 1 < ntiles) issue((SG + NST - 1) % NST);
+        if (!MODE || t + NST - 1 < ntiles) issue((SG + NST - 1) % NST);
         if (MODE ? sees(t + 1) : WORK) scores(nxt, smem + ((SG + 1) % NST) * STAGE);
       }
       if (MODE ? sees(t) : WORK) finish(cur, smem + SG * STAGE, t, mode);
     };
     int t = 0;
-    for (; t + NST < ntiles && t + NST < nfull; t += NST) {  // nothing hidden in tiles t .. t + 4
+    for (; t + 2 * NST - 2 < ntiles && t + NST <= nfull; t += NST) {  // nothing hidden in tiles t .. t + 3
       step(I0{}, t, sa, sb, I0{});
       step(I1{}, t + 1, sb, sa, I0{});
       step(I2{}, t + 2, sa, sb, I0{});
@@ -581,18 +625,16 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 // S^T per 16-key block on v_mfma_f32_16x16x32 (lane l, G = l / 16: keys 4 G + v of row l % 16), O^T per 16 dims
 // (keys 4 G + {0..3} and 16 + 4 G + {0..3} per lane, V^T by the transposing LDS read).
 // ------------------------------------------------------------------------------------------------
-template <class E, int DH, int NS>
-__global__ __launch_bounds__(256, 2) void packed_attn_keys_kernel(PackedAttn a) {
-  constexpr int R = 16, WAVES = 4, KEYS = 32, QK_STEPS = DH / 32, DB = DH / 16;
+template <class E, int DH, int NS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedAttn a) {
+  constexpr int R = 16, KEYS = 32, QK_STEPS = DH / 32, DB = DH / 16;
   constexpr int ROWB = 2 * DH, CPR = DH / 8, TILEB = KEYS * ROWB, RPI = 1024 / ROWB, L = KEYS / RPI;
   typedef typename E::v8 v8;
   extern __shared__ __align__(16) unsigned char smem[];
 
   const int item = a.by_hk(blockIdx.x), h = blockIdx.x - item * a.Hk;
   Item w;
-  const bool found = find_item<R, WAVES * KEYS>(a, item, w);
-  note_merge<R>(a, item, h, found, w);
-  if (!found) return;
+  if (!take_item<R, WAVES * KEYS>(a, item, h, w)) return;
   const int lane = threadIdx.x & 63, l16 = lane & 15, G = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int total = w.m * a.G, r0 = w.tile * R, row = r0 + l16;
@@ -903,7 +945,8 @@ static constexpr int kPackedCus = 256;
 // How a call is dealt, from what the host knows: rows per tile (16: the keys kernel), the most items of a key head,
 // and how many parts at the most its items are cut into beside their own number (0: never, no workspace).
 struct PackedShape {
-  int R, target, min_tiles;
+  int R, waves, target, min_tiles;
+  bool search;
   int64_t items;
 };
 
@@ -912,13 +955,16 @@ static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk,
   const int64_t G = Hq / Hk, seqs = std::max<int64_t>(1, std::min(S, rows));
   const int64_t mean = cdiv(rows * G, seqs);  // packed rows of a sequence
   s.R = mean <= 32 ? 16 : Dh == 128 && mean > 192 ? 256 : 128;
-  s.min_tiles = s.R == 16 ? 2 : 12;                      // of 128 and 64 keys
+  s.min_tiles = s.R == 16 ? 2 : 6;
   const int64_t tiles = std::max(rows * G / s.R, seqs);  // about as many as there are
+  s.waves = Dh == 64 && tiles * Hk <= kPackedCus ? 8 : 4;
+  const int keys = s.R == 16 ? 32 * s.waves : kKeyTile;  // of a key tile
   const int64_t fill = s.R == 16 ? 4 * kPackedCus : kPackedCus;
   if (tiles * Hk < fill && key_cap > 2048) s.target = (int)cdiv(kPackedCus, Hk);
   // The most items: the ceil of every sequence's tiles is at most one more than its rows have; and the parts, with
   // room for the rounding of the units' fp32 sum, but no tile has more than the cache's length allows.
-  const int64_t most = rows * G / s.R + seqs, most_parts = cdiv(cdiv(key_cap, s.R == 16 ? 128 : kKeyTile), s.min_tiles);
+  s.search = S > 64 && !s.target;
+  const int64_t most = rows * G / s.R + (s.search ? S : seqs), most_parts = cdiv(cdiv(key_cap, keys), s.min_tiles);
   s.items = s.target ? std::min(most + s.target + s.target / 16 + 1, most * most_parts) : most;
   return s;
 }
@@ -958,20 +1004,23 @@ static int launch_rows(const PackedAttn& a, hipStream_t st, const char* what) {
   return check_launch(what);
 }
 
-template <class E, int DH>
+template <class E, int DH, int WAVES>
 static int launch_keys(const PackedAttn& a, hipStream_t st, const char* what) {
   static std::atomic<uint64_t> done{0};
-  constexpr int NS = 2, lds = 4 * 2 * NS * 32 * 2 * DH;
-  const int rc = allow_lds((const void*)packed_attn_keys_kernel<E, DH, NS>, lds, done, what);
+  constexpr int NS = 2, lds = WAVES * 2 * NS * 32 * 2 * DH;
+  const int rc = allow_lds((const void*)packed_attn_keys_kernel<E, DH, NS, WAVES>, lds, done, what);
   if (rc != OUDJAT_OK) return rc;
-  packed_attn_keys_kernel<E, DH, NS><<<(unsigned)a.items * a.Hk, 256, lds, st>>>(a);
+  packed_attn_keys_kernel<E, DH, NS, WAVES><<<(unsigned)a.items * a.Hk, WAVES * 64, lds, st>>>(a);
   return check_launch(what);
 }
 
 template <class E, int DH>
-static int launch_packed(const PackedAttn& a, int R, hipStream_t st, const char* what) {
+static int launch_packed(const PackedAttn& a, int R, int waves, hipStream_t st, const char* what) {
   int rc;
-  if (R == 16) rc = launch_keys<E, DH>(a, st, what);
+  if (R == 16) {
+    if constexpr (DH == 64) rc = waves == 8 ? launch_keys<E, DH, 8>(a, st, what) : launch_keys<E, DH, 4>(a, st, what);
+    else rc = launch_keys<E, DH, 4>(a, st, what);
+  }
   else rc = R == 256 ? launch_rows<E, DH, 8>(a, st, what) : launch_rows<E, DH, 4>(a, st, what);
   if (rc != OUDJAT_OK || !a.target) return rc;
   const dim3 grid((unsigned)a.items * a.Hk, (unsigned)cdiv(R, kMergeRows));
@@ -1016,11 +1065,11 @@ extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t 
                  OUDJAT_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld elements is needed", what,
                  (long long)parts);
   const PackedAttn a{q, q_rs, q_hs, k, v, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, cu_q, keys, out, out_rs, (int)rows, (int)S,
-                     (int)Hk, (int)(Hq / Hk), Divisor((uint32_t)Hk), Divisor((uint32_t)(Hq / Hk)), (int)key_cap, cu_wide != 0, keys_wide != 0, batched != 0, causal != 0,
+                     (int)Hk, (int)(Hq / Hk), Divisor((uint32_t)Hk), Divisor((uint32_t)(Hq / Hk)), (int)key_cap, cu_wide != 0, keys_wide != 0, batched != 0, causal != 0, s.search,
                      scale * 1.4426950408889634f, s.target, s.min_tiles, (int)s.items, workspace,
                      s.target ? reinterpret_cast<int4*>(workspace + s.items * Hk * part_floats(s.R, (int)Dh)) : nullptr};
   hipStream_t st = as_stream(stream);
   if (dtype == OUDJAT_BF16)
-    return Dh == 64 ? launch_packed<AttnBf16, 64>(a, s.R, st, what) : launch_packed<AttnBf16, 128>(a, s.R, st, what);
-  return Dh == 64 ? launch_packed<AttnFp16, 64>(a, s.R, st, what) : launch_packed<AttnFp16, 128>(a, s.R, st, what);
+    return Dh == 64 ? launch_packed<AttnBf16, 64>(a, s.R, s.waves, st, what) : launch_packed<AttnBf16, 128>(a, s.R, s.waves, st, what);
+  return Dh == 64 ? launch_packed<AttnFp16, 64>(a, s.R, s.waves, st, what) : launch_packed<AttnFp16, 128>(a, s.R, s.waves, st, what);
 }

@@ -397,6 +397,26 @@ def test_attention_long(dev, m, n, Hq, Hk, Dh, causal):
         check_attention(q, k, v, m, n, Dh ** -0.5, causal, got, str(dtype))
 
 
+@pytest.mark.parametrize("S,longest,Hq,Hk,Dh", [(65, 200, 4, 1, 64), (130, 40, 3, 3, 128), (300, 90, 8, 2, 64),
+                                                (700, 3, 40, 4, 128), (5000, 2, 2, 1, 64)])
+def test_attention_many_sequences(dev, S, longest, Hq, Hk, Dh):
+    """Ragged lengths with empty sequences among them, the offsets starting inside the row buffer."""
+    rng = random.Random(S)
+    m = [rng.choice([0, 1, rng.randrange(longest + 1)]) for _ in range(S)]
+    n = [a + rng.randrange(60) for a in m]
+    q, k, v, cu, keys = packed_case(dev, m, n, Hq, Hk, Dh, BF, False, S)
+    got = K.packed_attention(q, k, v, cu, keys, Dh ** -0.5, causal=True)
+    some = rng.sample(range(S), 40)
+    for s in some:
+        at, ak = sum(m[:s]), sum(n[:s])
+        ref, slack = attention64(q[at:at + m[s]], k[ak:ak + n[s]], v[ak:ak + n[s]], m[s], n[s], Dh ** -0.5, True)
+        near(got[at:at + m[s]].view(m[s], Hq, Dh), ref, slack, f"sequence {s}")
+    wide = torch.cat([q[:7], q, q[:9]])
+    out = torch.full((wide.shape[0], Hq * Dh), 3.0, device=dev, dtype=BF)
+    K.packed_attention(wide, k, v, cu + 7, keys, Dh ** -0.5, causal=True, out=out)
+    assert torch.equal(out[7:-9], got) and (out[:7] == 3).all() and (out[-9:] == 3).all()
+
+
 @pytest.mark.parametrize("scale", [1e-3, 0.6, 3.0])
 def test_attention_sharp_and_flat_scores(dev, scale):
     m, n = [3, 200, 1], [400, 200, 3000]
