@@ -160,6 +160,17 @@ __device__ __forceinline__ void axis_sincos(const AxisRope& a, int64_t row, int 
   sincospif(half_turns, sn, cs);
 }
 
+// Cosines and sines of rows row0 .. row0 + n - 1 to lds [n][2][half], one (row, pair) per thread.
+__device__ __forceinline__ void fill_rope_table(const AxisRope& a, float* lds, int64_t row0, int n) {
+  for (int i = threadIdx.x; i < n * a.half; i += kRopeThreads) {
+    const int r = i / a.half, p = i - r * a.half;
+    float sn, cs;
+    axis_sincos(a, row0 + r, p, &sn, &cs);
+    lds[(2 * r) * a.half + p] = cs;
+    lds[(2 * r + 1) * a.half + p] = sn;
+  }
+}
+
 // 16-bit element types: E::to8 / E::from8 between a 16-byte chunk and eight floats.
 struct ElemBf16 {
   static __device__ __forceinline__ void to8(const uint4& v, float* f) { unpack8(v, f); }
@@ -183,51 +194,64 @@ struct ElemFp16 {
 __device__ __forceinline__ uint4 load16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ void store16(uint16_t* p, const uint4& v) { *reinterpret_cast<uint4*>(p) = v; }
 
-// A workgroup takes `per_wg` rows: the rows' sines and cosines first, then (row, head, 16 dims) items, one per
-// thread: chunk pair c < R/16 holds dims 8c .. and R/2 + 8c .., the others 16 dims that are copied. Every q and k
-// element is read and written once. An item's loads and stores do not depend on another's, so in place is fine.
-template <class E>
+// A workgroup takes `per_wg` rows: (row, head, 16 dims) items, one per thread: chunk pair c < R/16 holds dims 8c .. and
+// R/2 + 8c .., the others 16 dims that are copied. Every q and k element is read and written once; an item's loads
+// and stores do not depend on another's, so in place is fine. Bound by HBM: a thread has U items' loads in flight,
+// the first of them while the rows' sines and cosines are computed (16404 rows, 32 + 8 heads of 128, 336 MB: U = 1
+// 76 us, 4 70 us, 4.8 TB/s, 6 71 us; a copy of 2 GB runs at 4.9). U = 1 where a workgroup has one item per thread.
+template <class E, int U>
 __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(
     AxisRope a, const uint16_t* q, int64_t q_rs, int64_t q_hs, const uint16_t* k, int64_t k_rs, int64_t k_hs,
     uint16_t* qo, int64_t qo_rs, int64_t qo_hs, uint16_t* ko, int64_t ko_rs, int64_t ko_hs, int64_t rows, int Hq,
     int Hk, int Dh, int per_wg) {
-  extern __shared__ __align__(16) float rope_lds[];  // [per_wg][2][half]: cosines, sines
+  extern __shared__ __align__(16) float rope_lds[];
   const int half = a.half, tid = threadIdx.x;
   const int64_t row0 = (int64_t)blockIdx.x * per_wg;
   const int n = (int)min((int64_t)per_wg, rows - row0);
-  for (int i = tid; i < n * half; i += kRopeThreads) {
-    const int r = i / half, p = i - r * half;
-    float sn, cs;
-    axis_sincos(a, row0 + r, p, &sn, &cs);
-    rope_lds[(2 * r) * half + p] = cs;
-    rope_lds[(2 * r + 1) * half + p] = sn;
-  }
-  __syncthreads();
   const int cph = Dh / 16, H = Hq + Hk, items = n * H * cph, rot = half / 8;
-  for (int i = tid; i < items; i += kRopeThreads) {
-    const int rh = i / cph, c = i - rh * cph;
-    const int r = rh / H, h = rh - r * H;
-    const int64_t row = row0 + r;
-    const bool is_q = h < Hq;
-    const uint16_t* src = is_q ? q + row * q_rs + h * q_hs : k + row * k_rs + (h - Hq) * k_hs;
-    uint16_t* dst = is_q ? qo + row * qo_rs + h * qo_hs : ko + row * ko_rs + (h - Hq) * ko_hs;
-    const int d0 = c < rot ? 8 * c : 16 * c, d1 = c < rot ? half + 8 * c : 16 * c + 8;
-    uint4 x0 = load16(src + d0), x1 = load16(src + d1);
-    if (c < rot) {
-      const float* cs = rope_lds + (2 * r) * half + 8 * c;
-      const float* sn = cs + half;
-      float l[8], g[8];
-      E::to8(x0, l);
-      E::to8(x1, g);
-      float cv[8], sv[8];
-      load8f(cs, cv);
-      load8f(sn, sv);
-      rope8(l, g, cv, cv, sv, sv);
-      x0 = E::from8(l);
-      x1 = E::from8(g);
+  uint4 x0[U], x1[U];
+  uint16_t* dst[U];
+  int r[U], c[U];
+  auto first = [&](int u) { return c[u] < rot ? 8 * c[u] : 16 * c[u]; };
+  auto second = [&](int u) { return c[u] < rot ? half + 8 * c[u] : 16 * c[u] + 8; };
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * kRopeThreads, items - 1);
+      const int rh = i / cph;
+      c[u] = i - rh * cph;
+      r[u] = rh / H;
+      const int h = rh - r[u] * H;
+      const int64_t row = row0 + r[u];
+      const bool is_q = h < Hq;
+      const uint16_t* src = is_q ? q + row * q_rs + h * q_hs : k + row * k_rs + (h - Hq) * k_hs;
+      dst[u] = is_q ? qo + row * qo_rs + h * qo_hs : ko + row * ko_rs + (h - Hq) * ko_hs;
+      x0[u] = load16(src + first(u));
+      x1[u] = load16(src + second(u));
     }
-    store16(dst + d0, x0);
-    store16(dst + d1, x1);
+  };
+  load(tid);
+  fill_rope_table(a, rope_lds, row0, n);
+  __syncthreads();
+  for (int i0 = tid; i0 < items; i0 += kRopeThreads * U) {
+    if (i0 != tid) load(i0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * kRopeThreads >= items) break;
+      if (c[u] < rot) {
+        const float* cs = rope_lds + (2 * r[u]) * half + 8 * c[u];
+        float l[8], g[8], cv[8], sv[8];
+        E::to8(x0[u], l);
+        E::to8(x1[u], g);
+        load8f(cs, cv);
+        load8f(cs + half, sv);
+        rope8(l, g, cv, cv, sv, sv);
+        x0[u] = E::from8(l);
+        x1[u] = E::from8(g);
+      }
+      store16(dst[u] + first(u), x0[u]);
+      store16(dst[u] + second(u), x1[u]);
+    }
   }
 }
 
@@ -236,7 +260,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(
 // RMS: y = x / sqrt(mean(x^2) + eps) * w;  LayerNorm: the same of x - mean(x), plus b. Then the rotation, then one
 // rounding to the type; values are copied. Dh / 16 lanes hold a head, 16 dims each (as above), so that its sums
 // are two to three lane exchanges, and a thread keeps the weights of its dims for all heads it takes. A row whose
-// slot lies outside the cache is skipped.
+// slot lies outside the cache is skipped. Bound by HBM: 16404 rows, 32 + 2 x 8 heads of 128, 398 MB, 83.7 us
+// (4.75 TB/s); one token of 32 streams 4.8 us, a launch and two dependent rounds of loads.
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, bool LAYER>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kv_kernel(
@@ -250,13 +275,6 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kv_kernel(
   const int half = a.half, tid = threadIdx.x;
   const int64_t row0 = (int64_t)blockIdx.x * per_wg;
   const int n = (int)min((int64_t)per_wg, rows - row0);
-  for (int i = tid; i < n * half; i += kRopeThreads) {
-    const int r = i / half, p = i - r * half;
-    float sn, cs;
-    axis_sincos(a, row0 + r, p, &sn, &cs);
-    rope_lds[(2 * r) * half + p] = cs;
-    rope_lds[(2 * r + 1) * half + p] = sn;
-  }
   const int c = tid % L, rot = half / 8;
   const bool turned = c < rot;
   const int d0 = turned ? 8 * c : 16 * c, d1 = turned ? half + 8 * c : 16 * c + 8;
@@ -272,15 +290,27 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kv_kernel(
     b[1][0] = kb ? load16(kb + d0) : zero;
     b[1][1] = kb ? load16(kb + d1) : zero;
   }
-  __syncthreads();
   const int H = Hq + 2 * Hk, heads = n * H;
-  for (int i = tid / L; i < heads; i += kRopeThreads / L) {  // the L lanes of a head stay together
-    const int r = i / H, h = i - r * H;
-    const int64_t row = row0 + r;
-    const int64_t bi = batch_idx[row], ti = token_idx[row];
-    if (bi < 0 || bi >= B || ti < 0 || ti >= N) continue;
+  int r, h;
+  int64_t row, bi, ti;
+  uint4 x0, x1;
+  auto load = [&](int i) {  // (head i of the workgroup's rows, the last one where there is none)
+    i = min(i, heads - 1);
+    r = i / H;
+    h = i - r * H;
+    row = row0 + r;
     const uint16_t* src = qkv + row * x_rs + (int64_t)h * DH;
-    uint4 x0 = load16(src + d0), x1 = load16(src + d1);
+    x0 = load16(src + d0);
+    x1 = load16(src + d1);
+    bi = batch_idx[row];
+    ti = token_idx[row];
+  };
+  load(tid / L);
+  fill_rope_table(a, rope_lds, row0, n);
+  __syncthreads();
+  for (int i = tid / L; i < heads; i += kRopeThreads / L) {  // the L lanes of a head stay together
+    if (i != tid / L) load(i);
+    if (bi < 0 || bi >= B || ti < 0 || ti >= N) continue;
     uint16_t* dst;
     if (h < Hq) dst = qo + row * qo_rs + (int64_t)h * DH;
     else {
@@ -332,9 +362,11 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kv_kernel(
   }
 }
 
-// Rows a workgroup takes: one while that leaves CUs free (latency), else as many as its threads have pairs for.
+// Rows a workgroup takes: one while few (latency), else as many as its threads have pairs for. Measured (us, one row a
+// workgroup -> 256 / half rows; 32 + 8 heads of 128, rope and norm): 512 rows 5.7 -> 7.1 and 6.1 -> 10.1, 2048 rows
+// 12.9 -> 11.0 and 13.7 -> 15.2, 16404 rows 77 -> 72 and 82 -> 83; 6 + 6 heads of 64, 16404 rows 24 -> 15 and 30 -> 19.
 static int rope_rows_per_wg(int64_t rows, int half) {
-  return rows < 1024 ? 1 : std::max(1, kRopeThreads / half);
+  return rows < 2048 ? 1 : std::max(1, kRopeThreads / half);
 }
 
 static int make_axis_rope(AxisRope* a, const void* pos, int pos_kind, int64_t pos_rs, int64_t pos_as, int64_t axes,
@@ -407,13 +439,18 @@ extern "C" int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, c
   const int per = rope_rows_per_wg(rows, a.half);
   OUDJAT_REQUIRE(cdiv(rows, per) < INT32_MAX && (Hq + Hk) * Dh * per < INT32_MAX, OUDJAT_ERR_TOO_LARGE, "%s: too large",
                  what);
-  auto go = [&](auto e) {
-    rope_axes_kernel<decltype(e)><<<(unsigned)cdiv(rows, per), kRopeThreads, (size_t)per * 2 * a.half * 4,
-                                    as_stream(stream)>>>(a, q, q_rs, q_hs, k, k_rs, k_hs, q_out, qo_rs, qo_hs, k_out,
-                                                         ko_rs, ko_hs, rows, (int)Hq, (int)Hk, (int)Dh, per);
+  auto go = [&](auto e, auto u) {
+    rope_axes_kernel<decltype(e), decltype(u)::value>
+        <<<(unsigned)cdiv(rows, per), kRopeThreads, (size_t)per * 2 * a.half * 4, as_stream(stream)>>>(
+            a, q, q_rs, q_hs, k, k_rs, k_hs, q_out, qo_rs, qo_hs, k_out, ko_rs, ko_hs, rows, (int)Hq, (int)Hk, (int)Dh,
+            per);
   };
-  if (dtype == 0) go(ElemBf16{});
-  else go(ElemFp16{});
+  auto by_items = [&](auto e) {
+    if (per * (Hq + Hk) * Dh / 16 > kRopeThreads) go(e, std::integral_constant<int, 4>{});
+    else go(e, std::integral_constant<int, 1>{});
+  };
+  if (dtype == 0) by_items(ElemBf16{});
+  else by_items(ElemFp16{});
   return check_launch(what);
 }
 
