@@ -10,17 +10,19 @@
 // r % G of the group, so that one pass over a key head's K and V serves the whole group, a single token fills G rows
 // of a tile, and a causal tile spans few tokens.
 //
-// Work is dealt by the sequences' lengths, which only the device knows: a workgroup is one (item, key head), item = (tile of
-// R packed rows, part of its keys); the items of all sequences are numbered one after another, a sequence's last tile
-// (the one with the most keys) first, and every wave finds its item by a scan over the lengths, 64 sequences at a
-// time (about a microsecond up to some hundreds of sequences, against a plan launch of 3 us per layer). The grid
-// is an upper bound from the numbers of rows and sequences; workgroups past the last item leave.
+// Work is dealt by the sequences' lengths, which only the device knows: a workgroup is one (item, key head), item =
+// (tile of R packed rows, part of its keys), and finds its item from the lengths itself (scan_item, search_item: 1.2 us
+// of an idle CU, 2 beside a busy neighbour; a launch that laid the items out would cost every call 3 us and more).
+// Tiles are numbered from a sequence's last, the one with the most keys under causality. The grid is an upper bound
+// from the numbers of rows and sequences; workgroups without an item leave.
 //
-// Few items are split by keys (`split`): every part is left with about units / target key tiles, parts write their running
-// reference, sum and unnormalised rows to the workspace, and a second launch merges them in part order.
+// Few items are split by keys: parts of about units / target key tiles write their running reference, sum and
+// unnormalised rows to the workspace, and a second launch merges them in part order.
 //
 // Two kernels. packed_attn_rows: R = 32 W rows, a wave owns 32, all waves of the workgroup share K/V tiles of 64 keys.
-// packed_attn_keys, for few rows: R = 16, the four waves share the rows and take 32 keys each in turn.
+// packed_attn_keys, for few rows: R = 16, the waves share the rows and take 32 keys each in turn. Measured:
+// prompts of up to 16384 tokens, 32 over 8 heads of 128, 3.36 ms (1020 TF/s; a 16384^3 product of the library 1360);
+// 32 tokens over caches of up to 16385 keys 155 us (5.0 TB/s); 24 crops of up to 1029 tokens, 16 heads of 64, 44 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -115,13 +117,14 @@ __device__ __forceinline__ typename E::v8 round8(const float* f) {
   return __builtin_convertvector(v, typename E::v8);
 }
 
-__device__ __forceinline__ int load_idx(const void* p, int i, bool wide, int lo, int hi) {
-  if (wide) {
-    const int64_t v = static_cast<const int64_t*>(p)[i];
-    return v < lo ? lo : (v > hi ? hi : (int)v);
-  }
-  return max(lo, min(hi, static_cast<const int32_t*>(p)[i]));
+// Entry i of an int32 or int64 tensor, cut to 32 bits. Without branches, so that the loads of several entries overlap
+// (a branch on the width put a wait behind every one).
+__device__ __forceinline__ int load_idx(const void* p, int i, bool wide) {
+  const int32_t* w = static_cast<const int32_t*>(p) + ((int64_t)i << (wide ? 1 : 0));
+  const int lo = w[0], hi = w[wide ? 1 : 0];
+  return wide && hi != lo >> 31 ? (hi < 0 ? INT32_MIN : INT32_MAX) : lo;
 }
+__device__ __forceinline__ int clamp_idx(int v, int lo, int hi) { return max(lo, min(hi, v)); }
 
 // A sequence's rows and keys, and the item that a workgroup takes of it. Uniform over the wave.
 struct Item {
@@ -131,15 +134,12 @@ struct Item {
 
 // Sequence s: rows and keys, cut to the buffers.
 __device__ __forceinline__ void load_seq(const PackedAttn& a, int s, Item& t) {
-  t.q0 = load_idx(a.cu_q, s, a.cu_wide, 0, a.rows);
-  t.m = load_idx(a.cu_q, s + 1, a.cu_wide, t.q0, a.rows) - t.q0;
-  t.k0 = 0;
-  if (a.batched) {
-    t.n = load_idx(a.keys, s, a.keys_wide, 0, a.key_cap);
-  } else {
-    t.k0 = load_idx(a.keys, s, a.keys_wide, 0, a.key_cap);
-    t.n = load_idx(a.keys, s + 1, a.keys_wide, t.k0, a.key_cap) - t.k0;
-  }
+  const int c0 = load_idx(a.cu_q, s, a.cu_wide), c1 = load_idx(a.cu_q, s + 1, a.cu_wide);
+  const int k0 = load_idx(a.keys, s, a.keys_wide), k1 = load_idx(a.keys, s + (a.batched ? 0 : 1), a.keys_wide);
+  t.q0 = clamp_idx(c0, 0, a.rows);
+  t.m = clamp_idx(c1, t.q0, a.rows) - t.q0;
+  t.k0 = a.batched ? 0 : clamp_idx(k0, 0, a.key_cap);
+  t.n = clamp_idx(k1, t.k0, a.key_cap) - t.k0;
 }
 
 // Wave-wide sums and maxima by data-parallel moves (no LDS round trips): value of every lane combined with those of
@@ -174,14 +174,14 @@ __device__ __forceinline__ float last_lane(float x) {
 //
 // Search (more sequences, no split): sequence s starts at number floor(cu_q[s] G / R) + s, which leaves room for all
 // its tiles, so that the sequence of a number is found by a 64-way search in cu_q, two loads up to 4096 sequences
-// (one token each of 4096 sequences, 16 over 4 heads of 64, 200 keys: SEARCHMEAS).
+// (one token each of 4096 sequences, 16 over 4 heads of 64, 200 keys: 956 us by the scan, 222 by the search; of 256 26, 17).
 template <int R, int KT>
 __device__ __forceinline__ bool search_item(const PackedAttn& a, int item, Item& w) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = a.S;
   while (true) {  // the last s of lo .. lo + n - 1 that starts at or before the item
     const int step = (n + 63) / 64, s = lo + lane * step;
-    const bool before = s < lo + n && load_idx(a.cu_q, s, a.cu_wide, 0, a.rows) * a.G / R + s <= item;
+    const bool before = s < lo + n && clamp_idx(load_idx(a.cu_q, s, a.cu_wide), 0, a.rows) * a.G / R + s <= item;
     const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
     if (c == 0) return false;
     lo += (c - 1) * step;
@@ -331,7 +331,11 @@ __device__ __forceinline__ float ref_shift(float m, float scale_log2) { return m
 // HBM to LDS by buffer loads, four stages deep, each through a descriptor of exactly the keys that its tile has
 // left (built per tile from 64-bit addresses, so that a sequence may span more than 4 GiB): keys past the
 // sequence's last load as zeros, whatever lies there. The scores of the next tile are issued before the softmax of
-// this one.
+// this one. Bound by the softmax's VALU work and the matrix cores in about equal parts (about 140 VALU instructions per
+// 32 x 64 scores, half of a tile's cycles), as the rectangular attention's kernels are; two waves per SIMD are stated in the
+// launch bounds, without which the compiler keeps accumulators in the second register file and moves them (Dh = 64:
+// 96 of 269 VALU instructions, 24 crops 92 -> 69 us). Three stages and three waves per SIMD at Dh = 64 spill (24 crops
+// 46 -> 60 us). Beside the tiles a workgroup pays 4 to 5 us: its item, queries, first tiles and the output.
 // Hidden keys inside a sequence (causal) have score -inf, weight 0; a non-finite value among them would still give
 // 0 * inf = NaN in the second product. Only where a row came out non-finite is the item done again on a slow path
 // that takes such values out of the product and adds them to the rows that see them.
@@ -619,9 +623,10 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Keys kernel, for sequences of few packed rows (single tokens): 16 rows per workgroup, whose four waves take 32 keys
-// each in turn through rings of their own in LDS, so that no barrier holds a wave and the loads of a CU (up to 96 KB)
-// are never drained; the waves' results meet in LDS at the end. Bound by reading K and V once.
+// Keys kernel, for sequences of few packed rows (single tokens): 16 rows per workgroup, whose waves take 32 keys each
+// in turn through rings of their own in LDS (two tiles of K and two of V, each refilled as soon as it is read), so that
+// no barrier holds a wave and the loads of a CU (up to 96 KB) are never drained; the waves' results meet in LDS at the
+// end. Bound by reading K and V once: 512 tokens over 1000 keys each, 32 over 8 heads of 128, 370 us, 5.7 TB/s.
 // S^T per 16-key block on v_mfma_f32_16x16x32 (lane l, G = l / 16: keys 4 G + v of row l % 16), O^T per 16 dims
 // (keys 4 G + {0..3} and 16 + 4 G + {0..3} per lane, V^T by the transposing LDS read).
 // ------------------------------------------------------------------------------------------------
@@ -812,7 +817,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
     }
   }
 
-  // The four waves' results: references and sums, then rows of DH + 4 floats (conflict-free writes of 16 rows).
+  // The waves' results: references and sums, then rows of DH + 4 floats (conflict-free writes of 16 rows).
   constexpr int OROW = DH + 4, WROWS = 2 * R + R * OROW;
   float* park = reinterpret_cast<float*>(smem);
   __syncthreads();
@@ -942,14 +947,27 @@ using namespace oudjat;
 
 static constexpr int kPackedCus = 256;
 
-// How a call is dealt, from what the host knows: rows per tile (16: the keys kernel), the most items of a key head,
-// and how many parts at the most its items are cut into beside their own number (0: never, no workspace).
+// How a call is dealt, from what the host knows: rows per tile (16: the keys kernel, with its waves), the most items of
+// a key head, and how many parts at the most its items are cut into beside their own number (0: never, no workspace).
 struct PackedShape {
   int R, waves, target, min_tiles;
   bool search;
   int64_t items;
 };
 
+// Measured on one card, graphs of ten calls, us:
+// R: up to 32 packed rows a sequence on the mean the keys kernel (4 x 12 rows of 4 heads each over 8 k keys: 17 by it, 32
+//   by 128-row tiles with the limit at 16; 32 crops of 201 tokens: 8.7 by rows, 15.6 by keys with the limit at 64). Dh =
+//   128: tiles of 256 rows, whose eight waves fill a CU (its LDS holds one workgroup), above 192 rows (4 x 32 heads,
+//   414 of 4101: 142, by 128 rows 209; 64 tokens of 4 heads each over 8 k keys, 256 rows: 36, by 128 rows 33). Dh = 64: 128
+//   rows, two workgroups on a CU (24 crops: 46, by 256 rows 52; causal 4101 of 16 heads: 61, 82).
+// waves of the keys kernel at Dh = 64: eight, one workgroup on a CU, while there are no more tiles than CUs (4 tokens
+//   over 1 k keys: 9.2 -> 7.9), else two workgroups of four (64 tokens, 16 heads: 18.6, by eight 26.7).
+// target: with as many tiles as CUs (rows) or four times that (keys) nothing is split (64 tokens over 8 k keys, 8
+//   key heads: 118 split, 139 not; 16 crops of up to 1029 tokens: 26 unsplit, 47 with twice the target and splits), nor
+//   below 2049 keys (8 x 201 tokens of 6 heads: 8.7 unsplit, 10.6 with the merge launch). One part per CU: 1 token over 16 k
+//   keys, 8 key heads: 19.2, two per CU 24.7.
+// min_tiles: 6 x 100 rows over 3 k keys: 15.5 from 6, 20.8 from 12; 2 x 16 rows over 2 k keys: 9.8 from 2, 11.3 from 4.
 static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh, int64_t key_cap) {
   PackedShape s{};
   const int64_t G = Hq / Hk, seqs = std::max<int64_t>(1, std::min(S, rows));

@@ -13,6 +13,7 @@ synchronising.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -1405,24 +1406,24 @@ def packed_plan(q_lens: torch.Tensor, k_lens: torch.Tensor, rows: int, *, cache_
     return plan
 
 
-_SECTIONS: dict = {}
+@functools.lru_cache(maxsize=64)
+def _sections(sections: tuple):
+    """(host array of the sections that a call reads, their sum)."""
+    return (ctypes.c_int64 * max(1, len(sections)))(*sections), sum(sections)
 
 
 def _axis_rope(positions: torch.Tensor, inv_freq: torch.Tensor, sections, rows: int, what: str) -> tuple:
     """The position arguments of the C entry points."""
-    sections = tuple(sections)
-    host = _SECTIONS.get(sections)
-    if host is None:  # the host array that the call reads: one per distinct sections, kept
-        host = _SECTIONS[sections] = ((ctypes.c_int64 * max(1, len(sections)))(*sections), sum(sections))
+    host, half = _sections(tuple(sections))
     if positions.dim() != 2 or positions.shape[0] != rows or positions.dtype not in _POS_TYPES:
         raise ValueError(f"{what}: positions must be [rows, axes] int32, int64 or fp32")
     if len(sections) != positions.shape[1]:
         raise ValueError(f"{what}: one section per axis of positions")
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
-            or inv_freq.numel() != host[1]:
+            or inv_freq.numel() != half:
         raise ValueError(f"{what}: inv_freq must be contiguous fp32 [sum(sections)]")
     return (positions.data_ptr(), _POS_TYPES[positions.dtype], *positions.stride(), len(sections), inv_freq.data_ptr(),
-            ctypes.addressof(host[0]))
+            ctypes.byref(host))
 
 
 def apply_rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections,
@@ -1493,6 +1494,11 @@ def qk_norm_rope_kv(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm, k_norm
                _lib.stream_of(qkv))
 
 
+@functools.lru_cache(maxsize=4096)  # (row counts change from call to call: no table that only grows)
+def _packed_attention_workspace(rows: int, S: int, Hq: int, Hk: int, Dh: int, cap: int) -> int:
+    return int(_lib.load().oudjat_packed_attention_workspace_elems(rows, S, Hq, Hk, Dh, cap))
+
+
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, keys: torch.Tensor,
                      scale: float, *, causal: bool, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of packed rows over the keys of their own sequences, grouped heads -> [M, Hq * Dh].
@@ -1522,11 +1528,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     _require(S >= 0 and _is_lengths(cu_q, S + 1) and _is_lengths(keys, S if batched else S + 1),
              "packed_attention: cu_q [S + 1] and keys ([S] of a cache, [S + 1] packed) must be contiguous int32 or int64")
     _require(not batched or k.shape[0] >= S, "packed_attention: the cache has fewer batches than sequences")
-    wkey = ("packed_attention", M, S, Hq, Hk, Dh, cap)
-    elems = _WS_ELEMS.get(wkey)
-    if elems is None:
-        elems = int(_lib.load().oudjat_packed_attention_workspace_elems(*wkey[1:]))
-        _WS_ELEMS[wkey] = elems
+    elems = _packed_attention_workspace(M, S, Hq, Hk, Dh, cap)
     ws = _stream_workspace(q, elems) if elems > 0 else None
     if batched:
         sk, sv = _strides(k, 3), _strides(v, 3)

@@ -385,7 +385,9 @@ def test_attention(dev, m, n, Hq, Hk, Dh, causal):
 @pytest.mark.parametrize("m,n,Hq,Hk,Dh", [
     ([1000, 3, 700], [1000, 3, 700], 4, 4, 64), ([1, 1], [9000, 40], 8, 2, 128), ([600], [4101], 16, 4, 128),
     ([1029] * 4, [1029] * 4, 16, 16, 64), ([2000], [2000], 32, 8, 128), ([90, 4], [5000, 5000], 12, 12, 64),
-    ([1] * 70, list(range(1, 71)), 4, 2, 128), ([1] * 300, [200 + i for i in range(300)], 8, 8, 64),
+    ([1] * 70, list(range(1, 71)), 4, 2, 128), ([40] * 70, [40 + 37 * i for i in range(70)], 2, 2, 64),
+    ([1] * 100, [29 * i for i in range(1, 101)], 4, 2, 64), ([2] * 100, [2 + 29 * i for i in range(100)], 2, 1, 128),
+    ([100, 30], [2600, 100], 2, 1, 64), ([1] * 300, [200 + i for i in range(300)], 8, 8, 64),
     ([33], [20000], 1, 1, 64), ([1], [50000], 4, 1, 128),
 ])
 @pytest.mark.parametrize("causal", [False, True])
@@ -425,7 +427,9 @@ def test_attention_sharp_and_flat_scores(dev, scale):
 
 
 @pytest.mark.parametrize("m,n,Hq,Hk,Dh", [([200, 7], [200, 7], 4, 4, 64), ([150, 60], [190, 333], 8, 1, 128),
-                                          ([5, 1], [700, 90], 4, 2, 128), ([300], [300], 2, 2, 64)])
+                                          ([5, 1], [700, 90], 4, 2, 128), ([300], [300], 2, 2, 64),
+                                          ([7, 3], [2500, 64], 4, 2, 64), ([6], [2400], 2, 1, 128),
+                                          ([200], [2500], 4, 2, 64), ([150], [2600], 4, 2, 128)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_hidden_keys_and_values_have_no_influence(dev, m, n, Hq, Hk, Dh, bad):
     """A NaN or infinite key or value is met by the rows that see it, and by no others: keys behind a sequence's
