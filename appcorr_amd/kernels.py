@@ -1339,14 +1339,16 @@ def _gpu_of(*tensors: torch.Tensor | None) -> int:
     """The device index that all given tensors share; raises as _require_cuda does."""
     dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (t.get_device() != dev or dev < 0):
+        if t is not None and t.get_device() != dev:
             _require_cuda(*tensors)
+    if dev < 0:
+        _require_cuda(*tensors)
     return dev
 
 
 def _launch_on(tag: str, dev: int, t: torch.Tensor, name: str, *args) -> None:
     """_launch with the tensors' device as the current one (its stream is that device's)."""
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             _launch(tag, t, name, *args)
     elif tag in _probe["tags"]:
@@ -1363,8 +1365,16 @@ def _strides(t: torch.Tensor, n: int):
     return [0 if shape[d] == 1 else stride[d] for d in range(n)]
 
 
+_LENGTH_TYPES = (torch.int32, torch.int64)
+
+
 def _is_lengths(t: torch.Tensor, n: int) -> bool:
-    return t.dim() == 1 and t.dtype in (torch.int32, torch.int64) and t.is_contiguous() and t.numel() == n
+    return t.shape == (n,) and t.dtype in _LENGTH_TYPES and t.is_contiguous()
+
+
+def _rows_packed(t: torch.Tensor, inner: int) -> bool:
+    """[..., n, inner] with its last two dims packed."""
+    return t.stride(-1) == 1 and (t.stride(-2) == inner or t.shape[-2] == 1)
 
 
 @dataclass
@@ -1415,15 +1425,13 @@ def _sections(sections: tuple):
 def _axis_rope(positions: torch.Tensor, inv_freq: torch.Tensor, sections, rows: int, what: str) -> tuple:
     """The position arguments of the C entry points."""
     host, half = _sections(tuple(sections))
-    if positions.dim() != 2 or positions.shape[0] != rows or positions.dtype not in _POS_TYPES:
-        raise ValueError(f"{what}: positions must be [rows, axes] int32, int64 or fp32")
-    if len(sections) != positions.shape[1]:
-        raise ValueError(f"{what}: one section per axis of positions")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
-            or inv_freq.numel() != half:
+    kind = _POS_TYPES.get(positions.dtype)
+    if kind is None or positions.shape != (rows, len(sections)):
+        raise ValueError(f"{what}: positions must be [rows, axes] int32, int64 or fp32, with one section per axis")
+    if inv_freq.dtype != torch.float32 or inv_freq.shape != (half,) or not inv_freq.is_contiguous():
         raise ValueError(f"{what}: inv_freq must be contiguous fp32 [sum(sections)]")
-    return (positions.data_ptr(), _POS_TYPES[positions.dtype], *positions.stride(), len(sections), inv_freq.data_ptr(),
-            ctypes.byref(host))
+    row_stride, axis_stride = positions.stride()
+    return positions.data_ptr(), kind, row_stride, axis_stride, len(sections), inv_freq.data_ptr(), ctypes.byref(host)
 
 
 def apply_rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections,
@@ -1435,23 +1443,27 @@ def apply_rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, i
     inv_freq[i] radians, formed in 64 bits; dims from R on stay. Position 0 leaves a row as it is (cls and
     register tokens). bf16 or fp16; q and k may be views of a qkv row with packed heads' last dim. `out` =
     (q_out, k_out) receives the result and may be (q, k): in place."""
-    _require(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    kind = _DTYPES.get(dtype)
+    _require(len(qs) == len(ks) == 3 and qs[0] == ks[0] and qs[2] == ks[2],
              "apply_rope_axes: q [M, Hq, Dh] and k [M, Hk, Dh]")
+    _require(kind is not None and k.dtype == dtype, "apply_rope_axes: bf16 or fp16, one type")
+    M, Hq, Dh = qs
     if out is None:
-        oq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        ok = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        oq = torch.empty(qs, device=q.device, dtype=dtype)
+        ok = torch.empty(ks, device=q.device, dtype=dtype)
+        dev = _gpu_of(q, k, positions, inv_freq)
+        _require(q.stride(2) == 1 and k.stride(2) == 1, "apply_rope_axes: the head dim must be contiguous")
     else:
         oq, ok = out
-        _require(oq.shape == q.shape and ok.shape == k.shape, "apply_rope_axes: out must have the shapes of q and k")
-    dev = _gpu_of(q, k, positions, inv_freq, oq, ok)
-    _require(q.dtype in _DTYPES and q.dtype == k.dtype == oq.dtype == ok.dtype,
-             "apply_rope_axes: bf16 or fp16, one type")
-    _require(q.stride(2) == 1 and k.stride(2) == 1 and oq.stride(2) == 1 and ok.stride(2) == 1,
-             "apply_rope_axes: the head dim must be contiguous")
-    M, Hq, Dh = q.shape
+        dev = _gpu_of(q, k, positions, inv_freq, oq, ok)
+        _require(oq.shape == qs and ok.shape == ks and oq.dtype == dtype and ok.dtype == dtype,
+                 "apply_rope_axes: out must have the shapes and the type of q and k")
+        _require(q.stride(2) == 1 and k.stride(2) == 1 and oq.stride(2) == 1 and ok.stride(2) == 1,
+                 "apply_rope_axes: the head dim must be contiguous")
     pos = _axis_rope(positions, inv_freq, sections, M, "apply_rope_axes")
     _launch_on("rope_axes", dev, q, "oudjat_rope_axes", q.data_ptr(), *_strides(q, 2), k.data_ptr(), *_strides(k, 2), M,
-               Hq, k.shape[1], Dh, _DTYPES[q.dtype], *pos, oq.data_ptr(), *_strides(oq, 2), ok.data_ptr(),
+               Hq, ks[1], Dh, kind, *pos, oq.data_ptr(), *_strides(oq, 2), ok.data_ptr(),
                *_strides(ok, 2), _lib.stream_of(q))
     return oq, ok
 
@@ -1470,27 +1482,30 @@ def qk_norm_rope_kv(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm, k_norm
     kw, kb = k_norm
     dev = _gpu_of(qkv, qw, qb, kw, kb, positions, inv_freq, batch_idx, token_idx, kv_cache, q_out)
     dtype = qkv.dtype
-    _require(heads > 0 and kv_heads > 0 and qkv.dim() == 3 and qkv.shape[1] == heads + 2 * kv_heads
-             and dtype in _DTYPES and trailing_is_packed(qkv, 1),
+    kind = _DTYPES.get(dtype)
+    shape = qkv.shape
+    _require(heads > 0 and kv_heads > 0 and len(shape) == 3 and shape[1] == heads + 2 * kv_heads and kind is not None
+             and _rows_packed(qkv, shape[2]),
              "qk_norm_rope_kv: qkv must be [M, heads + 2 kv_heads, Dh] bf16 or fp16 with packed rows")
-    M, _, Dh = qkv.shape
+    M, _, Dh = shape
     for w in (qw, qb, kw, kb):
-        _require(w is None or (w.dtype == dtype and w.numel() == Dh and w.is_contiguous()),
-                 "qk_norm_rope_kv: norm weights must be contiguous [Dh] of qkv's type")
+        if w is not None and (w.dtype != dtype or w.shape != (Dh,) or not w.is_contiguous()):
+            raise ValueError("qk_norm_rope_kv: norm weights must be contiguous [Dh] of qkv's type")
     _require(layer_norm or (qb is None and kb is None), "qk_norm_rope_kv: a bias needs layer_norm=True")
-    _require(kv_cache.dim() == 5 and kv_cache.shape[2:] == (2, kv_heads, Dh) and kv_cache.dtype == dtype
-             and trailing_is_packed(kv_cache, 3),
+    cache = kv_cache.shape
+    _require(len(cache) == 5 and cache == (cache[0], cache[1], 2, kv_heads, Dh) and kv_cache.dtype == dtype
+             and _rows_packed(kv_cache, Dh),
              "qk_norm_rope_kv: kv_cache must be [B, N, 2, kv_heads, Dh] of qkv's type with packed heads")
-    _require(q_out.shape == (M, heads, Dh) and q_out.dtype == dtype and trailing_is_packed(q_out, 1),
+    _require(q_out.shape == (M, heads, Dh) and q_out.dtype == dtype and _rows_packed(q_out, Dh),
              "qk_norm_rope_kv: q_out must be [M, heads, Dh] of qkv's type with packed rows")
     bi, ti = _index(batch_idx, "batch_idx"), _index(token_idx, "token_idx")
-    _require(bi.numel() == M and ti.numel() == M, "qk_norm_rope_kv: one slot per row")
+    _require(bi.shape == (M,) and ti.shape == (M,), "qk_norm_rope_kv: one slot per row")
     pos = _axis_rope(positions, inv_freq, sections, M, "qk_norm_rope_kv")
     _launch_on("qkv_post", dev, qkv, "oudjat_qk_norm_rope_kv", qkv.data_ptr(), *_strides(qkv, 1), M, heads, kv_heads, Dh,
-               _DTYPES[dtype], layer_norm, qw.data_ptr() if qw is not None else 0,
+               kind, layer_norm, qw.data_ptr() if qw is not None else 0,
                qb.data_ptr() if qb is not None else 0, kw.data_ptr() if kw is not None else 0,
                kb.data_ptr() if kb is not None else 0, eps, *pos, bi.data_ptr(), ti.data_ptr(), kv_cache.data_ptr(),
-               *_strides(kv_cache, 3), kv_cache.shape[0], kv_cache.shape[1], q_out.data_ptr(), *_strides(q_out, 1),
+               *_strides(kv_cache, 3), cache[0], cache[1], q_out.data_ptr(), *_strides(q_out, 1),
                _lib.stream_of(qkv))
 
 
@@ -1511,23 +1526,27 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     A row without keys gives 0; hidden keys have no influence, NaN or infinite ones neither. Rows of `out` behind
     the last sequence stay as they were (undefined in a new tensor). scale must be positive. bf16 or fp16; Dh 64
     or 128. With few query rows the keys of a sequence are split over workgroups and merged, in a fixed order."""
-    _require(q.dim() == 3 and k.dim() in (3, 4) and k.shape == v.shape and k.shape[-1] == q.shape[2],
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    _require(len(qs) == 3 and len(ks) in (3, 4) and ks == v.shape and ks[-1] == qs[2],
              "packed_attention: q [M, Hq, Dh], k and v [Mk, Hk, Dh] or [B, N, Hk, Dh]")
-    M, Hq, Dh = q.shape
-    dtype = q.dtype
+    M, Hq, Dh = qs
+    kind = _DTYPES.get(dtype)
+    _require(kind is not None and k.dtype == dtype and v.dtype == dtype, "packed_attention: bf16 or fp16, one type")
+    _require(q.stride(2) == 1 and k.stride(-1) == 1 and v.stride(-1) == 1,
+             "packed_attention: the head dims must be contiguous")
     if out is None:
+        dev = _gpu_of(q, k, v, cu_q, keys)
         out = torch.empty((M, Hq * Dh), device=q.device, dtype=dtype)
-    dev = _gpu_of(q, k, v, cu_q, keys, out)
-    _require(dtype in _DTYPES and dtype == k.dtype == v.dtype == out.dtype,
-             "packed_attention: bf16 or fp16, one type")
-    _require(q.stride(2) == 1 and k.stride(-1) == 1 and v.stride(-1) == 1 and out.shape == (M, Hq * Dh)
-             and out.stride(1) == 1, "packed_attention: contiguous head dims, out [M, Hq * Dh] with contiguous rows")
-    batched = k.dim() == 4
-    cap, Hk = k.shape[-3], k.shape[-2]
+    else:
+        dev = _gpu_of(q, k, v, cu_q, keys, out)
+        _require(out.shape == (M, Hq * Dh) and out.dtype == dtype and out.stride(1) == 1,
+                 "packed_attention: out must be [M, Hq * Dh] of q's type with contiguous rows")
+    batched = len(ks) == 4
+    cap, Hk = ks[-3], ks[-2]
     S = cu_q.numel() - 1
     _require(S >= 0 and _is_lengths(cu_q, S + 1) and _is_lengths(keys, S if batched else S + 1),
              "packed_attention: cu_q [S + 1] and keys ([S] of a cache, [S + 1] packed) must be contiguous int32 or int64")
-    _require(not batched or k.shape[0] >= S, "packed_attention: the cache has fewer batches than sequences")
+    _require(not batched or ks[0] >= S, "packed_attention: the cache has fewer batches than sequences")
     elems = _packed_attention_workspace(M, S, Hq, Hk, Dh, cap)
     ws = _stream_workspace(q, elems) if elems > 0 else None
     if batched:
@@ -1536,6 +1555,6 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         sk, sv = (0, *_strides(k, 2)), (0, *_strides(v, 2))
     _launch_on("attention", dev, q, "oudjat_packed_attention", q.data_ptr(), *_strides(q, 2), M, Hq, Dh, k.data_ptr(),
                *sk, v.data_ptr(), *sv, Hk, cap, batched, cu_q.data_ptr(), cu_q.dtype == torch.int64, keys.data_ptr(),
-               keys.dtype == torch.int64, S, scale, causal, _DTYPES[dtype], out.data_ptr(), *_strides(out, 1),
+               keys.dtype == torch.int64, S, scale, causal, kind, out.data_ptr(), *_strides(out, 1),
                0 if ws is None else ws.data_ptr(), elems, _lib.stream_of(q))
     return out
