@@ -437,7 +437,7 @@ extern "C" int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, c
   const int rc = make_axis_rope(&a, pos, pos_kind, pos_rs, pos_as, axes, inv_freq, sections, Dh, what);
   if (rc != OUDJAT_OK) return rc;
   const int per = rope_rows_per_wg(rows, a.half);
-  OUDJAT_REQUIRE(cdiv(rows, per) < INT32_MAX && (Hq + Hk) * Dh * per < INT32_MAX, OUDJAT_ERR_TOO_LARGE, "%s: too large",
+  OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24) && (Hq + Hk) * Dh * per < INT32_MAX, OUDJAT_ERR_TOO_LARGE, "%s: too large",
                  what);
   auto go = [&](auto e, auto u) {
     rope_axes_kernel<decltype(e), decltype(u)::value>
@@ -478,7 +478,7 @@ extern "C" int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t
   const int rc = make_axis_rope(&a, pos, pos_kind, pos_rs, pos_as, axes, inv_freq, sections, Dh, what);
   if (rc != OUDJAT_OK) return rc;
   const int per = rope_rows_per_wg(rows, a.half);
-  OUDJAT_REQUIRE(cdiv(rows, per) < INT32_MAX && (Hq + 2 * Hk) * Dh * per < INT32_MAX, OUDJAT_ERR_TOO_LARGE,
+  OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24) && (Hq + 2 * Hk) * Dh * per < INT32_MAX, OUDJAT_ERR_TOO_LARGE,
                  "%s: too large", what);
   auto go = [&](auto e, auto dh, auto layer) {
     qk_norm_rope_kv_kernel<decltype(e), decltype(dh)::value, decltype(layer)::value>

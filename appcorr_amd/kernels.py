@@ -1419,7 +1419,7 @@ def packed_plan(q_lens: torch.Tensor, k_lens: torch.Tensor, rows: int, *, cache_
 @functools.lru_cache(maxsize=64)
 def _sections(sections: tuple):
     """(host array of the sections that a call reads, their sum)."""
-    return (ctypes.c_int64 * max(1, len(sections)))(*sections), sum(sections)
+    return (ctypes.c_int64 * max(1, len(sections)))(*map(int, sections)), int(sum(sections))
 
 
 def _axis_rope(positions: torch.Tensor, inv_freq: torch.Tensor, sections, rows: int, what: str) -> tuple:

@@ -426,6 +426,38 @@ def test_attention_sharp_and_flat_scores(dev, scale):
     check_attention(q, k, v, m, n, scale, True, K.packed_attention(q, k, v, cu, keys, scale, causal=True))
 
 
+@pytest.mark.parametrize("m", [1, 50])
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_attention_of_many_small_weights(dev, m, Dh, dtype):
+    """One key far above 20000 equal ones, whose weights (2^-15 and 2^-20 of its own, subnormal in fp16) add up to a
+    large and to a small part of the sum."""
+    n = 20001
+    for octaves, at in ((15, 0), (15, n - 1), (20, 9000)):
+        g = gen(dev, octaves)
+        k = torch.zeros(1, n, 1, Dh, device=dev, dtype=dtype)
+        k[0, at, 0, 0] = octaves
+        v = torch.randn(1, n, 1, Dh, generator=g, device=dev).to(dtype) + 0.5
+        q = torch.zeros(m, 2, Dh, device=dev, dtype=dtype)
+        q[:, :, 0] = 1
+        got = K.packed_attention(q, k, v, offsets([m], dev), torch.tensor([n], device=dev), math.log(2), causal=False)
+        check_attention(q, k, v, [m], [n], math.log(2), False, got, f"{octaves} octaves")
+
+
+@pytest.mark.parametrize("m", [1, 70])
+@pytest.mark.parametrize("Dh", [64, 128])
+def test_attention_of_tiny_and_huge_fp16_values(dev, m, Dh):
+    """Values and keys below fp16's smallest normal number, and values near its largest."""
+    q, k, v, cu, keys = packed_case(dev, [m], [300], 2, 2, Dh, HF, True, 6)
+    for factor in (1e-5, 1.5e4):
+        vf = (v.float() * factor).clamp(-65504, 65504).to(HF)  # (a value of 4.4 times the deviation would be infinite)
+        got = K.packed_attention(q, k, vf, cu, keys, 0.1, causal=True)
+        check_attention(q, k, vf, [m], [300], 0.1, True, got, f"values {factor}")
+    small = (k.float() * 1e-5).to(HF)
+    got = K.packed_attention(q, small, v, cu, keys, 1e4, causal=True)
+    check_attention(q, small, v, [m], [300], 1e4, True, got, "keys")
+
+
 @pytest.mark.parametrize("m,n,Hq,Hk,Dh", [([200, 7], [200, 7], 4, 4, 64), ([150, 60], [190, 333], 8, 1, 128),
                                           ([5, 1], [700, 90], 4, 2, 128), ([300], [300], 2, 2, 64),
                                           ([7, 3], [2500, 64], 4, 2, 64), ([6], [2400], 2, 1, 128),
