@@ -166,15 +166,17 @@ __device__ __forceinline__ float last_lane(float x) {
 
 // Item number `item` of a key head, tiles of R packed rows and KT keys; false if there is none. Two numberings:
 //
-// Scan (up to 64 sequences, or any number if keys are split): the sequences' items one after another, 64 sequences at
-// a time. Parts of a sequence's tiles: its key tiles / C, rounded, with C = max(min_tiles, units / target) and units the
-// key tiles of all tiles, so that a key head has at most its own tiles + target items. Up to 64 sequences the items of the
-// longer ones (more than half of the longest's keys, then more than a quarter) come first, so that the last
-// workgroups are short.
+// Scan (up to 64 sequences, up to kSortedSeqs with long keys, any number if keys are split): the sequences' items one
+// after another, 64 sequences at a time. Parts of a sequence's tiles: its key tiles / C, rounded, with C = max(min_tiles, units / target) and units the
+// key tiles of all tiles, so that a key head has at most its own tiles + target items. Up to kSortedSeqs sequences the
+// items of the longer ones (more than half of the longest's keys, then more than a quarter) come first, so that the
+// last workgroups are short.
 //
 // Search (more sequences, no split): sequence s starts at number floor(cu_q[s] G / R) + s, which leaves room for all
 // its tiles, so that the sequence of a number is found by a 64-way search in cu_q, two loads up to 4096 sequences
 // (one token each of 4096 sequences, 16 over 4 heads of 64, 200 keys: 956 us by the scan, 222 by the search; of 256 26, 17).
+static constexpr int kSortedSeqs = 256;
+
 template <int R, int KT>
 __device__ __forceinline__ bool search_item(const PackedAttn& a, int item, Item& w) {
   const int lane = threadIdx.x & 63;
@@ -209,22 +211,23 @@ __device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w
     if (s0 + lane < a.S) load_seq(a, s0 + lane, t);
   };
   load(0);
-  const bool sorted = a.S <= 64;
+  const bool sorted = a.S <= kSortedSeqs;
+  float units = (float)tiles() * (float)key_tiles();
+  top = key_tiles();
+  for (int s0 = 64; s0 < a.S; s0 += 64) {
+    load(s0);
+    units += (float)tiles() * (float)key_tiles();
+    top = max(top, key_tiles());
+  }
   if (a.target) {
-    float units = (float)tiles() * (float)key_tiles();
-    for (int s0 = 64; s0 < a.S; s0 += 64) {
-      load(s0);
-      units += (float)tiles() * (float)key_tiles();
-    }
     units = last_lane(wave_scan(units, [](float x, float y) { return x + y; }));
     chunk = max(a.min_tiles, (int)ceilf(units / (float)a.target));
-    if (!sorted) load(0);
   }
-  if (sorted) top = last_lane(wave_scan(key_tiles(), [](int x, int y) { return max(x, y); }));
+  if (sorted) top = last_lane(wave_scan(top, [](int x, int y) { return max(x, y); }));
   int base = 0;
   for (int cls = 0; cls < (sorted ? 3 : 1); ++cls) {
     for (int s0 = 0; s0 < a.S; s0 += 64) {
-      if (s0) load(s0);
+      if (a.S > 64) load(s0);
       const int nt = tiles(), kt = key_tiles(), parts = a.target ? max(1, (2 * kt + chunk) / (2 * chunk)) : 1;
       const int mine = !sorted || (2 * kt > top ? 0 : 4 * kt > top ? 1 : 2) == cls ? nt * parts : 0;
       const int incl = wave_scan(mine, [](int x, int y) { return x + y; });
@@ -965,6 +968,7 @@ struct PackedShape {
 //   key heads: 118 split, 139 not; 16 crops of up to 1029 tokens: 26 unsplit, 47 with twice the target and splits), nor
 //   below 2049 keys (8 x 201 tokens of 6 heads: 8.7 unsplit, 10.6 with the merge launch). One part per CU: 1 token over 16 k
 //   keys, 8 key heads: 19.2, two per CU 24.7.
+// search (above): 256 tokens over 200 keys 17 by search, 26 by scan; 128 over up to 4 k keys 139 by search, 126 by scan.
 // min_tiles: 6 x 100 rows over 3 k keys: 15.5 from 6, 20.8 from 12; 2 x 16 rows over 2 k keys: 9.8 from 2, 11.3 from 4.
 static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh, int64_t key_cap) {
   PackedShape s{};
@@ -979,7 +983,7 @@ static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk,
   if (tiles * Hk < fill && key_cap > 2048) s.target = (int)cdiv(kPackedCus, Hk);
   // The most items: the ceil of every sequence's tiles is at most one more than its rows have; and the parts, with
   // room for the rounding of the units' fp32 sum, but no tile has more than the cache's length allows.
-  s.search = S > 64 && !s.target;
+  s.search = S > 64 && !s.target && (S > kSortedSeqs || key_cap <= 2048);
   const int64_t most = rows * G / s.R + (s.search ? S : seqs), most_parts = cdiv(cdiv(key_cap, keys), s.min_tiles);
   s.items = s.target ? std::min(most + s.target + s.target / 16 + 1, most * most_parts) : most;
   return s;
