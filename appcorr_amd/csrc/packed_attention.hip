@@ -167,14 +167,14 @@ __device__ __forceinline__ float last_lane(float x) {
 // Item number `item` of a key head, tiles of R packed rows and KT keys; false if there is none. Two numberings:
 //
 // Scan (up to 64 sequences, up to kSortedSeqs with long keys, any number if keys are split): the sequences' items one
-// after another, 64 sequences at a time. Parts of a sequence's tiles: its key tiles / C, rounded, with C = max(min_tiles, units / target) and units the
-// key tiles of all tiles, so that a key head has at most its own tiles + target items. Up to kSortedSeqs sequences the
-// items of the longer ones (more than half of the longest's keys, then more than a quarter) come first, so that the
-// last workgroups are short.
+// after another, 64 sequences at a time. Parts of a sequence's tiles: its key tiles / C, rounded, with C =
+// max(min_tiles, units / target) and units the key tiles of all tiles, so that a key head has at most its own tiles +
+// target items. Up to kSortedSeqs sequences the items of the longer ones (more than half of the longest's keys, then
+// more than a quarter) come first, so that the last workgroups are short.
 //
 // Search (more sequences, no split): sequence s starts at number floor(cu_q[s] G / R) + s, which leaves room for all
-// its tiles, so that the sequence of a number is found by a 64-way search in cu_q, two loads up to 4096 sequences
-// (one token each of 4096 sequences, 16 over 4 heads of 64, 200 keys: 956 us by the scan, 222 by the search; of 256 26, 17).
+// its tiles, so that the sequence of a number is found by a 64-way search in cu_q, two loads up to 4096 sequences (one
+// token each of 4096 sequences, 16 over 4 heads of 64, 200 keys: 956 us by the scan, 222 by the search; of 256 26, 17).
 static constexpr int kSortedSeqs = 256;
 
 template <int R, int KT>
@@ -221,7 +221,7 @@ __device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w
   }
   if (a.target) {
     units = last_lane(wave_scan(units, [](float x, float y) { return x + y; }));
-    chunk = max(a.min_tiles, (int)ceilf(units / (float)a.target));
+    chunk = max(a.min_tiles, (int)fminf(ceilf(units / (float)a.target), (float)(1 << 24)));
   }
   if (sorted) top = last_lane(wave_scan(top, [](int x, int y) { return max(x, y); }));
   int base = 0;
@@ -243,8 +243,9 @@ __device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w
         w.parts = __builtin_amdgcn_readlane(parts, l);
         const int from_last = w.parts == 1 ? within : within / w.parts;
         w.part = within - from_last * w.parts;
-        w.tile = __builtin_amdgcn_readlane(nt, l) - 1 - from_last;
-        return true;
+        const int last = __builtin_amdgcn_readlane(nt, l) - 1;
+        w.tile = last - from_last;
+        return from_last >= 0 && w.tile >= 0;  // (offsets that fall may let the counts wrap)
       }
       base += total;
     }
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
   const int lim_tile = seen_keys(a, w, a.by_g(r0));
   constexpr int KT = WAVES * KEYS;
   const int all_tiles = (kend + KT - 1) / KT, per = w.parts == 1 ? all_tiles : (all_tiles + w.parts - 1) / w.parts;
-  const int kfirst = w.part * per * KT, klast = min(kend, kfirst + per * KT);  // this part's keys
+  const int kfirst = min(w.part * per, all_tiles) * KT, klast = min(kend, kfirst + per * KT);  // this part's keys
   const int n32 = max(0, (klast - kfirst + KEYS - 1) / KEYS);
   const int cnt = (n32 - wave + WAVES - 1) / WAVES;  // tiles of this wave: wave, wave + 4, ...
 
@@ -1085,11 +1086,13 @@ extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t 
                  OUDJAT_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %lld elements is needed", what,
                  (long long)parts);
   const PackedAttn a{q, q_rs, q_hs, k, v, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, cu_q, keys, out, out_rs, (int)rows, (int)S,
-                     (int)Hk, (int)(Hq / Hk), Divisor((uint32_t)Hk), Divisor((uint32_t)(Hq / Hk)), (int)key_cap, cu_wide != 0, keys_wide != 0, batched != 0, causal != 0, s.search,
-                     scale * 1.4426950408889634f, s.target, s.min_tiles, (int)s.items, workspace,
+                     (int)Hk, (int)(Hq / Hk), Divisor((uint32_t)Hk), Divisor((uint32_t)(Hq / Hk)), (int)key_cap,
+                     cu_wide != 0, keys_wide != 0, batched != 0, causal != 0, s.search, scale * 1.4426950408889634f, s.target, s.min_tiles, (int)s.items, workspace,
                      s.target ? reinterpret_cast<int4*>(workspace + s.items * Hk * part_floats(s.R, (int)Dh)) : nullptr};
   hipStream_t st = as_stream(stream);
   if (dtype == OUDJAT_BF16)
-    return Dh == 64 ? launch_packed<AttnBf16, 64>(a, s.R, s.waves, st, what) : launch_packed<AttnBf16, 128>(a, s.R, s.waves, st, what);
-  return Dh == 64 ? launch_packed<AttnFp16, 64>(a, s.R, s.waves, st, what) : launch_packed<AttnFp16, 128>(a, s.R, s.waves, st, what);
+    return Dh == 64 ? launch_packed<AttnBf16, 64>(a, s.R, s.waves, st, what)
+                    : launch_packed<AttnBf16, 128>(a, s.R, s.waves, st, what);
+  return Dh == 64 ? launch_packed<AttnFp16, 64>(a, s.R, s.waves, st, what)
+                  : launch_packed<AttnFp16, 128>(a, s.R, s.waves, st, what);
 }

@@ -545,6 +545,20 @@ def test_attention_offsets_outside_the_buffers_are_cut(dev):
     assert not none.any()
 
 
+def test_attention_offsets_that_fall(dev):
+    """Offsets that rise and fall are no valid input: the call ends all the same and writes nothing outside `out`."""
+    for S, Hk, Dh, cap in ((3, 2, 64, 3000), (200, 1, 128, 3000), (300, 2, 64, 100)):
+        q, _, _, _, _ = packed_case(dev, [900], [900], 2 * Hk, Hk, Dh, BF, False, 14)
+        g = gen(dev, 15)
+        k = torch.randn(cap, Hk, Dh, generator=g, device=dev).to(BF)
+        cu = torch.tensor([0, 20] + [900 if i % 2 else 0 for i in range(S - 1)], device=dev)
+        cu_k = torch.tensor([0, 50] + [cap if i % 2 else 0 for i in range(S - 1)], device=dev)
+        out = torch.full((902, 2 * Hk * Dh), 5.0, device=dev, dtype=BF)
+        K.packed_attention(q, k, k, cu, cu_k, 0.1, causal=True, out=out[1:901])
+        torch.cuda.synchronize()
+        assert (out[0] == 5).all() and (out[901] == 5).all()
+
+
 def test_attention_empty(dev):
     q = torch.empty(0, 4, 64, device=dev, dtype=BF)
     k = torch.empty(0, 2, 64, device=dev, dtype=BF)
@@ -672,3 +686,106 @@ def test_layer_of_prompts_and_then_tokens(dev):
         have = total
     for s, n in enumerate(have):  # the cache holds the tokens that were given, and nothing else
         assert torch.isfinite(kv[s, :n]).all() and torch.isnan(kv[s, n:]).all()
+
+
+def test_layer_in_a_graph(dev):
+    """The three steps recorded once and replayed with other lengths, rows and caches, against eager calls."""
+    Hq, Hk, Dh, N, rows, S = 8, 2, 128, 2300, 40, 5
+    g = gen(dev, 50)
+    qkv = torch.zeros(rows, Hq + 2 * Hk, Dh, device=dev, dtype=BF)
+    new = torch.zeros(S, device=dev, dtype=torch.int64)
+    total = torch.zeros(S, device=dev, dtype=torch.int64)
+    w = torch.ones(Dh, device=dev, dtype=BF)
+    freq = (100.0 ** -(torch.arange(64, device=dev) / 64)).float()
+    pos = torch.randint(0, 1 << 20, (rows, 3), generator=g, device=dev)
+    kv = torch.randn(S, N, 2, Hk, Dh, generator=g, device=dev).to(BF)
+    q = torch.zeros(rows, Hq, Dh, device=dev, dtype=BF)
+    out = torch.zeros(rows, Hq * Dh, device=dev, dtype=BF)
+
+    def layer(kv, q, out):
+        plan = K.packed_plan(new, total, rows, cache_len=N)
+        K.qk_norm_rope_kv(qkv, Hq, Hk, (w, None), (w, None), 1e-6, pos, freq, (16, 24, 24), plan.batch_idx,
+                          plan.token_idx, kv, q)
+        K.packed_attention(q, kv[:, :, 0], kv[:, :, 1], plan.cu_q, plan.k_lens, Dh ** -0.5, causal=True, out=out)
+
+    replay = graphs.capture(lambda: layer(kv, q, out))
+    for turn, (a, b) in enumerate([([1] * 5, [2300, 1, 40, 700, 2000]), ([8, 0, 20, 3, 0], [8, 0, 2300, 1500, 9]),
+                                   ([0] * 5, [0] * 5), ([40, 0, 0, 0, 0], [41, 0, 0, 0, 0])]):
+        qkv.copy_(torch.randn(qkv.shape, generator=gen(dev, turn), device=dev))
+        new.copy_(torch.tensor(a, device=dev))
+        total.copy_(torch.tensor(b, device=dev))
+        kv2, q2, out2 = kv.clone(), q.clone(), out.clone()
+        layer(kv2, q2, out2)
+        torch.cuda.synchronize()
+        replay()
+        torch.cuda.synchronize()
+        assert torch.equal(kv, kv2) and torch.equal(q, q2) and torch.equal(out, out2), f"replay {turn}"
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q=(4, 4, 32)), dict(k=(9, 3, 64)), dict(v=(9, 2, 128)), dict(dtype=torch.float32), dict(cu=4), dict(keys=4),
+    dict(scale=0.0), dict(scale=-0.1), dict(scale=math.nan), dict(out=(4, 255)), dict(kdtype=HF), dict(heads_strided=True),
+    dict(k=(2, 9, 2, 64)), dict(cu_dtype=torch.float32), dict(odd=True),
+])
+def test_attention_refusals(dev, bad):
+    """Arguments that do not fit are refused before a launch, ValueError by the wrapper or the library's status."""
+    dtype = bad.get("dtype", BF)
+    q = torch.zeros(bad.get("q", (4, 4, 64)), device=dev, dtype=dtype)
+    k = torch.zeros(bad.get("k", (9, 2, 64)), device=dev, dtype=bad.get("kdtype", dtype))
+    v = torch.zeros(bad.get("v", k.shape), device=dev, dtype=bad.get("kdtype", dtype))
+    if bad.get("heads_strided"):
+        k = torch.zeros(9, 2, 128, device=dev, dtype=dtype)[..., ::2]
+    if bad.get("odd"):
+        q = torch.zeros(4 * 4 * 64 + 1, device=dev, dtype=dtype)[1:].view(4, 4, 64)
+    cu = torch.zeros(bad.get("cu", 4), device=dev, dtype=bad.get("cu_dtype", torch.int32))
+    keys = torch.zeros(bad.get("keys", 4), device=dev, dtype=torch.int32)
+    if bad.get("cu") == 4:
+        keys = keys[:3]
+    elif bad.get("keys") == 4:
+        cu = cu[:3]
+    out = torch.zeros(bad["out"], device=dev, dtype=dtype) if "out" in bad else None
+    from appcorr_amd._lib import OudjatKernelError
+    with pytest.raises((ValueError, OudjatKernelError)):
+        K.packed_attention(q, k, v, cu, keys, bad.get("scale", 0.1), causal=True, out=out)
+
+
+def test_row_operator_refusals(dev):
+    from appcorr_amd._lib import OudjatKernelError
+    x = torch.zeros(4, 6, 64, device=dev, dtype=BF)
+    pos, freq = torch.zeros(4, 2, device=dev), torch.zeros(32, device=dev)
+    n = torch.ones(3, device=dev, dtype=torch.int32)
+    for call in (
+        lambda: K.apply_rope_axes(x, x.to(HF), pos, freq, (16, 16)),
+        lambda: K.apply_rope_axes(x.float(), x.float(), pos, freq, (16, 16)),
+        lambda: K.apply_rope_axes(x, x[:3], pos, freq, (16, 16)),
+        lambda: K.apply_rope_axes(x, x, pos, freq, (16, 8)),
+        lambda: K.apply_rope_axes(x, x, pos, freq, (32,)),
+        lambda: K.apply_rope_axes(x, x, pos.double(), freq, (16, 16)),
+        lambda: K.apply_rope_axes(x, x, pos, freq.double(), (16, 16)),
+        lambda: K.apply_rope_axes(x, x, pos, torch.zeros(40, device=dev), (20, 20)),
+        lambda: K.apply_rope_axes(x, x, pos.cpu(), freq, (16, 16)),
+        lambda: K.apply_rope_axes(x, x, pos, freq, (16, 16), out=(x, x[:, :3])),
+        lambda: K.packed_plan(n, n[:2], 4, cache_len=4),
+        lambda: K.packed_plan(n, n, 4),
+        lambda: K.packed_plan(n, n, 4, cache_len=4, key_rows=4),
+        lambda: K.packed_plan(n.float(), n, 4, cache_len=4),
+        lambda: K.packed_plan(n, n, -1, cache_len=4),
+        lambda: K.packed_plan(n, n, 4, cache_len=-1),
+        lambda: K.packed_plan(torch.ones(4097, device=dev, dtype=torch.int32),
+                              torch.ones(4097, device=dev, dtype=torch.int32), 4, cache_len=4),
+    ):
+        with pytest.raises((ValueError, OudjatKernelError)):
+            call()
+    w = torch.ones(64, device=dev, dtype=BF)
+    slot = torch.zeros(4, device=dev, dtype=torch.int64)
+    kv, q = torch.zeros(1, 8, 2, 1, 64, device=dev, dtype=BF), torch.zeros(4, 4, 64, device=dev, dtype=BF)
+
+    def norm(qkv=x, heads=4, qn=(w, None), sections=(16, 16), bi=slot, ti=slot, kv=kv, q=q, eps=1e-6, **kw):
+        K.qk_norm_rope_kv(qkv, heads, 1, qn, (None, None), eps, pos, freq, sections, bi, ti, kv, q, **kw)
+
+    for kw in (dict(heads=5), dict(qkv=x.float()), dict(qn=(w[:32], None)), dict(qn=(w.float(), None)), dict(qn=(w, w)),
+               dict(sections=(16,)), dict(bi=slot.int()), dict(ti=slot[:3]), dict(kv=kv[:, :, :1]), dict(kv=kv.to(HF)),
+               dict(q=q[:3]), dict(q=q.to(HF)), dict(eps=-1.0), dict(eps=math.nan),
+               dict(qkv=x.transpose(0, 1).contiguous().transpose(0, 1))):
+        with pytest.raises((ValueError, OudjatKernelError)):
+            norm(**kw)

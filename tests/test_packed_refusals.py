@@ -118,6 +118,24 @@ def test_attention_refuses(status, kw):
     refused(status, "oudjat_packed_attention", *attn_args(**kw))
 
 
+def test_attention_refuses_a_missing_or_small_workspace():
+    """Few rows over a long cache: the keys may be split, and the call needs what the library asks for."""
+    shape = (4, 1, 4, 2, 64)
+    need = _lib.load().oudjat_packed_attention_workspace_elems(*shape, 5000)
+    assert need > 0 and _lib.load().oudjat_packed_attention_workspace_elems(*shape, 2048) == 0
+    for ws, elems in ((NULL, need), (P16, need - 1), (ctypes.c_void_p(24), need)):
+        refused("OUDJAT_ERR_INVALID_ARGUMENT", "oudjat_packed_attention", *attn_args(cap=5000, ws=ws, ws_elems=elems))
+
+
+@pytest.mark.parametrize("rows,S,Hq,Hk,Dh,cap", [(1, 1, 1, 1, 64, 1 << 29), (32, 32, 32, 8, 128, 16385), (700, 3, 32, 8, 128, 9000),
+                                                  (100, 70, 4, 1, 64, 4000), (1, 1, 64, 64, 128, 1 << 29)])
+def test_attention_workspace_is_bounded(rows, S, Hq, Hk, Dh, cap):
+    """A part is at most 256 rows of Dh + 2 floats and there are about as many as CUs and tiles together."""
+    need = _lib.load().oudjat_packed_attention_workspace_elems(rows, S, Hq, Hk, Dh, cap)
+    tiles = rows * (Hq // Hk) // 16 + min(S, rows)
+    assert 0 < need <= (tiles * Hk + 2 * 256 + 2 * Hk) * (256 * (Dh + 2) + 4)
+
+
 def test_nothing_to_do_is_no_error():
     _lib.call("oudjat_packed_attention", *attn_args(rows=0, q=NULL, out=NULL))
     _lib.call("oudjat_packed_attention", *attn_args(S=0, cu=NULL))
