@@ -388,7 +388,8 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 
   const int lrow = RPI * wave + lane / CPR;  // tile row that this lane loads, and rows RPI W further on
   const uint32_t chunk = (uint32_t)(((lane % CPR) ^ tile_swz<DH>(lrow)) << 4);
-  const uint32_t koff0 = (uint32_t)lrow * (uint32_t)a.k_rs * 2u + chunk, voff0 = (uint32_t)lrow * (uint32_t)a.v_rs * 2u + chunk;
+  const uint32_t koff0 = (uint32_t)lrow * (uint32_t)a.k_rs * 2u + chunk;
+  const uint32_t voff0 = (uint32_t)lrow * (uint32_t)a.v_rs * 2u + chunk;
   // Tiles are issued in order: the next one's addresses and the keys left from it on (uniform).
   const uint16_t *knext, *vnext;
   int left;
@@ -1087,7 +1088,8 @@ extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t 
                  (long long)parts);
   const PackedAttn a{q, q_rs, q_hs, k, v, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, cu_q, keys, out, out_rs, (int)rows, (int)S,
                      (int)Hk, (int)(Hq / Hk), Divisor((uint32_t)Hk), Divisor((uint32_t)(Hq / Hk)), (int)key_cap,
-                     cu_wide != 0, keys_wide != 0, batched != 0, causal != 0, s.search, scale * 1.4426950408889634f, s.target, s.min_tiles, (int)s.items, workspace,
+                     cu_wide != 0, keys_wide != 0, batched != 0, causal != 0, s.search, scale * 1.4426950408889634f,
+                     s.target, s.min_tiles, (int)s.items, workspace,
                      s.target ? reinterpret_cast<int4*>(workspace + s.items * Hk * part_floats(s.R, (int)Dh)) : nullptr};
   hipStream_t st = as_stream(stream);
   if (dtype == OUDJAT_BF16)
