@@ -1548,7 +1548,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
              "packed_attention: cu_q [S + 1] and keys ([S] of a cache, [S + 1] packed) must be contiguous int32 or int64")
     _require(not batched or ks[0] >= S, "packed_attention: the cache has fewer batches than sequences")
     elems = _packed_attention_workspace(M, S, Hq, Hk, Dh, cap)
-    ws = _stream_workspace(q, elems) if elems > 0 else None
+    # The parts of split keys, from the allocator and not _stream_workspace: two graphs that torch.cuda.graph records
+    # on its one capture stream would share that buffer, and may be replayed at once.
+    ws = q.new_empty(elems, dtype=torch.float32) if elems > 0 else None
     if batched:
         sk, sv = _strides(k, 3), _strides(v, 3)
     else:

@@ -635,6 +635,33 @@ def test_attention_on_another_stream_and_in_graphs(dev):
         torch.cuda.synchronize()
 
 
+def test_attention_graphs_recorded_by_torch_own_their_scratch(dev):
+    """torch records all its graphs on one stream; two of them, with split keys, replayed at once on two streams."""
+    cases, runs = [], []
+    for seed in (81, 82):
+        q, k, v, cu, keys = packed_case(dev, [2, 1, 3], [5000, 4100, 4900], 8, 2, 128, BF, True, seed)
+        out = torch.empty_like(q).flatten(1)
+        want = K.packed_attention(q, k, v, cu, keys, 0.1, causal=True)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            K.packed_attention(q, k, v, cu, keys, 0.1, causal=True, out=out)
+        cases.append((q, k, v, cu, keys, out, want))
+        runs.append((g, torch.cuda.Stream()))
+    for _ in range(4):
+        for case in cases:
+            case[5].fill_(7.0)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, stream in runs:
+                with torch.cuda.stream(stream):
+                    g.replay()
+        torch.cuda.synchronize()
+        for q, k, v, cu, keys, out, want in cases:
+            assert torch.equal(out, want)
+            assert torch.equal(K.packed_attention(q, k, v, cu, keys, 0.1, causal=True), want)
+
+
 def test_attention_agrees_with_sparse_query_attention(dev):
     """Equal lengths, equal heads, no mask: the rectangular attention of the correction pass."""
     g = gen(dev, 30)
