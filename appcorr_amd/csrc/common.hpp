@@ -106,6 +106,28 @@ inline hipStream_t as_stream(oudjat_stream_t s) { return reinterpret_cast<hipStr
 
 inline bool aligned(const void* p, int64_t a) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)a) == 0; }
 
+// Whether a buffer's entries are apart: `inner` elements each, dims given as (size, stride) in any order. A buffer that
+// is written must be (an expanded one has stride 0: its workgroups would race).
+struct BufferDim {
+  int64_t size, stride;
+};
+template <int N>
+inline bool entries_apart(const BufferDim (&dims)[N], int64_t inner) {
+  BufferDim d[N];
+  for (int i = 0; i < N; ++i) {  // by stride
+    int at = i;
+    for (; at > 0 && d[at - 1].stride > dims[i].stride; --at) d[at] = d[at - 1];
+    d[at] = dims[i];
+  }
+  __int128 end = inner;  // of the entries of the dims so far
+  for (int i = 0; i < N; ++i) {
+    if (d[i].size <= 1) continue;
+    if (d[i].stride < end) return false;
+    end += (__int128)(d[i].size - 1) * d[i].stride;
+  }
+  return true;
+}
+
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- direct-to-LDS loads and their waits (shared by the GEMM and attention kernels) ----------------

@@ -433,6 +433,8 @@ extern "C" int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, c
   OUDJAT_REQUIRE(((q_rs | q_hs | k_rs | k_hs | qo_rs | qo_hs | ko_rs | ko_hs) % 8) == 0 && aligned(q, 16) &&
                      aligned(k, 16) && aligned(q_out, 16) && aligned(k_out, 16),
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned rows and heads required", what);
+  OUDJAT_REQUIRE(entries_apart({{rows, qo_rs}, {Hq, qo_hs}}, Dh) && entries_apart({{rows, ko_rs}, {Hk, ko_hs}}, Dh),
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: the rows and heads of an output must not overlap", what);
   AxisRope a;
   const int rc = make_axis_rope(&a, pos, pos_kind, pos_rs, pos_as, axes, inv_freq, sections, Dh, what);
   if (rc != OUDJAT_OK) return rc;
@@ -474,6 +476,8 @@ extern "C" int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t
                      aligned(q_out, 16) && aligned(qw, 16) && aligned(qb, 16) && aligned(kw, 16) && aligned(kb, 16) &&
                      aligned(batch_idx, 8) && aligned(token_idx, 8),
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned rows and weights required", what);
+  OUDJAT_REQUIRE(entries_apart({{rows, qo_rs}}, Hq * Dh) && entries_apart({{B, kv_bs}, {N, kv_ns}, {2, kv_cs}}, Hk * Dh),
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: the rows of q_out and of the cache must not overlap", what);
   AxisRope a;
   const int rc = make_axis_rope(&a, pos, pos_kind, pos_rs, pos_as, axes, inv_freq, sections, Dh, what);
   if (rc != OUDJAT_OK) return rc;

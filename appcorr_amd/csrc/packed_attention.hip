@@ -1077,6 +1077,8 @@ extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t 
                      aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(cu_q, cu_wide ? 8 : 4) &&
                      aligned(keys, keys_wide ? 8 : 4),
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned q, k, v and out rows and heads required", what);
+  OUDJAT_REQUIRE(entries_apart({{rows, out_rs}}, Hq * Dh), OUDJAT_ERR_UNSUPPORTED_LAYOUT,
+                 "%s: the rows of out must not overlap", what);
   OUDJAT_REQUIRE(rows * (Hq / Hk) < (1 << 30) && Hq <= 65535 && S < (1 << 24) && key_cap < (1 << 30) &&
                      k_rs < (1 << 24) && v_rs < (1 << 24),
                  OUDJAT_ERR_TOO_LARGE, "%s: too large", what);

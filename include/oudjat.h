@@ -763,7 +763,8 @@ int oudjat_packed_plan(const void* q_lens, int q_wide, const void* k_lens, int k
  * has), dims (i, i + R/2), i < R/2, of row m turn by pos[m, axis of i] * inv_freq[i] radians (formed in 64 bits);
  * dims from R on are copied. fp32 arithmetic, one rounding. pos [rows, axes] with strides pos_rs, pos_as of type
  * oudjat_pos, 1 to 4 axes. The outputs may be the inputs (in place) but not overlap them otherwise. Hq or Hk may
- * be 0. Dh % 16 == 0, Dh <= 512; R / 2 a multiple of 8; 16-byte aligned rows and heads. */
+ * be 0. Dh % 16 == 0, Dh <= 512; R / 2 a multiple of 8; 16-byte aligned rows and heads, an output's rows and heads
+ * apart (any order of the two strides). */
 int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, const uint16_t* k, int64_t k_rs, int64_t k_hs,
                      int64_t rows, int64_t Hq, int64_t Hk, int64_t Dh, int dtype, const void* pos, int pos_kind,
                      int64_t pos_rs, int64_t pos_as, int64_t axes, const float* inv_freq, const int64_t* sections,
@@ -775,7 +776,8 @@ int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, const uint16
  * Dh values or NULL), rotated as in oudjat_rope_axes, rounded once; queries to q_out [rows, Hq, Dh] (row stride
  * qo_rs), keys and (unchanged) values to kv + batch * kv_bs + token * kv_ns (+ kv_cs for values), Hk x Dh packed.
  * Rows whose (batch, token) lies outside B x N are skipped: neither q_out nor the cache is written for them. The
- * slots of the other rows must be unique. Dh 64 or 128; 16-byte aligned rows. */
+ * slots of the other rows must be unique. Dh 64 or 128; 16-byte aligned rows, those of q_out and of the cache apart
+ * (any order of its strides). Neither output may overlap qkv. */
 int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t rows, int64_t Hq, int64_t Hk, int64_t Dh,
                            int dtype, int layer_norm, const uint16_t* q_weight, const uint16_t* q_bias,
                            const uint16_t* k_weight, const uint16_t* k_bias, float eps, const void* pos, int pos_kind,
@@ -797,7 +799,8 @@ int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t rows, int6
  * Where one workgroup per tile of query rows would leave CUs idle, the keys are split over several and merged by a
  * second launch (in part order): workspace of oudjat_packed_attention_workspace_elems fp32 elements, 16-byte
  * aligned, else OUDJAT_ERR_INVALID_ARGUMENT. Deterministic. Dh 64 or 128; scale > 0 and finite; 16-byte aligned
- * rows and heads of q, k, v and out; strides not negative. */
+ * rows and heads of q, k, v and out; strides not negative; the rows of out apart from one another
+ * and from q, k and v. Calls that may run at once need a workspace each. */
 int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64_t rows, int64_t Hq, int64_t Dh,
                             const uint16_t* k, int64_t k_bs, int64_t k_rs, int64_t k_hs, const uint16_t* v,
                             int64_t v_bs, int64_t v_rs, int64_t v_hs, int64_t Hk, int64_t key_cap, int batched,

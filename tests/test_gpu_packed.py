@@ -749,6 +749,30 @@ def test_layer_in_a_graph(dev):
         assert torch.equal(kv, kv2) and torch.equal(q, q2) and torch.equal(out, out2), f"replay {turn}"
 
 
+def test_outputs_in_other_orders(dev):
+    """Outputs whose entries are apart in any order of dims: heads outside rows, a cache with K and V outside, every
+    second row; what lies between stays."""
+    g, Hq, Hk, Dh, M, B, N = gen(dev, 93), 4, 2, 64, 9, 2, 5
+    pos, freq = torch.randint(0, 99, (M, 2), generator=g, device=dev), torch.rand(32, generator=g, device=dev)
+    q, k = (torch.randn(M, h, Dh, generator=g, device=dev).to(BF) for h in (Hq, Hk))
+    want = K.apply_rope_axes(q, k, pos, freq, (16, 16))
+    oq = torch.full((Hq, 2 * M, Dh), 3.0, device=dev, dtype=BF)
+    ok = torch.full((Hk, M, Dh), 3.0, device=dev, dtype=BF)
+    K.apply_rope_axes(q, k, pos, freq, (16, 16), out=(oq[:, ::2].transpose(0, 1), ok.transpose(0, 1)))
+    assert torch.equal(oq[:, ::2].transpose(0, 1), want[0]) and torch.equal(ok.transpose(0, 1), want[1])
+    assert (oq[:, 1::2] == 3.0).all()
+
+    qkv = torch.randn(M, Hq + 2 * Hk, Dh, generator=g, device=dev).to(BF)
+    slot = torch.randperm(B * N, generator=g, device=dev)[:M]
+    plain = torch.full((B, N, 2, Hk, Dh), 3.0, device=dev, dtype=BF)
+    other = torch.full((2, N, B, Hk, Dh), 3.0, device=dev, dtype=BF)
+    q1, q2 = torch.empty(M, Hq, Dh, device=dev, dtype=BF), torch.full((2 * M, Hq, Dh), 3.0, device=dev, dtype=BF)
+    for cache, qo in ((plain, q1), (other.permute(2, 1, 0, 3, 4), q2[::2])):
+        K.qk_norm_rope_kv(qkv, Hq, Hk, (None, None), (None, None), 1e-6, pos, freq, (16, 16), slot // N, slot % N, cache,
+                          qo)
+    assert torch.equal(other.permute(2, 1, 0, 3, 4), plain) and torch.equal(q2[::2], q1) and (q2[1::2] == 3.0).all()
+
+
 @pytest.mark.parametrize("bad", [
     dict(q=(4, 4, 32)), dict(k=(9, 3, 64)), dict(v=(9, 2, 128)), dict(dtype=torch.float32), dict(cu=4), dict(keys=4),
     dict(scale=0.0), dict(scale=-0.1), dict(scale=math.nan), dict(out=(4, 255)), dict(kdtype=HF), dict(heads_strided=True),

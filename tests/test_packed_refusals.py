@@ -68,6 +68,13 @@ def test_rope_refuses(status, kw):
     refused(status, "oudjat_rope_axes", *args)
 
 
+@pytest.mark.parametrize("kw", [dict(qo_rs=0), dict(ko_rs=0), dict(qo_hs=0), dict(qo_hs=56), dict(ko_rs=248),
+                                dict(qo_rs=64, qo_hs=248), dict(ko_rs=-256), dict(qo_rs=1 << 62, rows=1 << 20, qo_hs=0)])
+def test_rope_refuses_an_output_that_overlaps_itself(kw):
+    host, args = rope_args(**kw)
+    refused("OUDJAT_ERR_UNSUPPORTED_LAYOUT", "oudjat_rope_axes", *args)
+
+
 def norm_args(sections=(16, 16), **kw):
     host = (ctypes.c_int64 * len(sections))(*sections)
     a = dict(x=P16, x_rs=512, rows=4, Hq=4, Hk=2, Dh=64, dtype=0, layer=0, qw=P16, qb=NULL, kw_=P16, kb=NULL, eps=1e-6,
@@ -89,6 +96,13 @@ def norm_args(sections=(16, 16), **kw):
 def test_norm_refuses(status, kw):
     host, args = norm_args(**kw)
     refused(status, "oudjat_qk_norm_rope_kv", *args)
+
+
+@pytest.mark.parametrize("kw", [dict(qo_rs=0), dict(qo_rs=248), dict(kv_bs=0), dict(kv_ns=0), dict(kv_cs=0),
+                                dict(kv_cs=120), dict(kv_ns=248), dict(kv_bs=1016), dict(kv_bs=256, kv_ns=504, kv_cs=128)])
+def test_norm_refuses_outputs_that_overlap_themselves(kw):
+    host, args = norm_args(**kw)
+    refused("OUDJAT_ERR_UNSUPPORTED_LAYOUT", "oudjat_qk_norm_rope_kv", *args)
 
 
 def attn_args(**kw):
@@ -116,6 +130,11 @@ def attn_args(**kw):
 ])
 def test_attention_refuses(status, kw):
     refused(status, "oudjat_packed_attention", *attn_args(**kw))
+
+
+@pytest.mark.parametrize("out_rs", [0, 248])
+def test_attention_refuses_an_output_that_overlaps_itself(out_rs):
+    refused("OUDJAT_ERR_UNSUPPORTED_LAYOUT", "oudjat_packed_attention", *attn_args(out_rs=out_rs))
 
 
 def test_attention_refuses_a_missing_or_small_workspace():
