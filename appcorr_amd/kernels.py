@@ -1442,7 +1442,7 @@ def apply_rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, i
     inv_freq fp32 [sum(sections)]: dims (i, i + R/2) with R = 2 sum(sections) turn by positions[m, axis of i] *
     inv_freq[i] radians, formed in 64 bits; dims from R on stay. Position 0 leaves a row as it is (cls and
     register tokens). bf16 or fp16; q and k may be views of a qkv row with packed heads' last dim. `out` =
-    (q_out, k_out) receives the result and may be (q, k): in place."""
+    (q_out, k_out) receives the result and may be (q, k): in place; it must not overlap itself or them otherwise."""
     qs, ks, dtype = q.shape, k.shape, q.dtype
     kind = _DTYPES.get(dtype)
     _require(len(qs) == len(ks) == 3 and qs[0] == ks[0] and qs[2] == ks[2],
@@ -1477,7 +1477,8 @@ def qk_norm_rope_kv(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm, k_norm
     q_norm, k_norm: (weight, bias) of Dh values of qkv's type, each or both None. RMSNorm over a head
     (x / sqrt(mean(x^2) + eps) * weight), or LayerNorm with layer_norm=True. Positions, inv_freq and sections as in
     apply_rope_axes. fp32 arithmetic, rounded once. Rows with a slot outside the cache (packed_plan's -1) are
-    skipped: q_out and the cache keep what they held. The other rows' slots must be unique. Dh 64 or 128."""
+    skipped: q_out and the cache keep what they held. The other rows' slots must be unique. q_out and kv_cache may
+    be strided, but not overlap themselves (expanded) or qkv. Dh 64 or 128."""
     qw, qb = q_norm
     kw, kb = k_norm
     dev = _gpu_of(qkv, qw, qb, kw, kb, positions, inv_freq, batch_idx, token_idx, kv_cache, q_out)
@@ -1525,7 +1526,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     0 .. n - m + i of its n, so the last row sees all; else every row sees all n.
     A row without keys gives 0; hidden keys have no influence, NaN or infinite ones neither. Rows of `out` behind
     the last sequence stay as they were (undefined in a new tensor). scale must be positive. bf16 or fp16; Dh 64
-    or 128. With few query rows the keys of a sequence are split over workgroups and merged, in a fixed order."""
+    or 128. With few query rows the keys of a sequence are split over workgroups and merged, in a fixed order. `out`
+    must not overlap itself (expanded) or an input."""
     qs, ks, dtype = q.shape, k.shape, q.dtype
     _require(len(qs) == 3 and len(ks) in (3, 4) and ks == v.shape and ks[-1] == qs[2],
              "packed_attention: q [M, Hq, Dh], k and v [Mk, Hk, Dh] or [B, N, Hk, Dh]")
