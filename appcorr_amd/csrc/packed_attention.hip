@@ -245,7 +245,7 @@ __device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w
         w.part = within - from_last * w.parts;
         const int last = __builtin_amdgcn_readlane(nt, l) - 1;
         w.tile = last - from_last;
-        return from_last >= 0 && w.tile >= 0;  // (offsets that fall may let the counts wrap)
+        return within >= 0 && w.tile >= 0;  // (offsets that fall may let the counts wrap)
       }
       base += total;
     }
@@ -261,7 +261,10 @@ __device__ __forceinline__ bool take_item(const PackedAttn& a, int item, int h, 
   __shared__ int shared[9];
   if (threadIdx.x < 64) {
     w = Item{};
-    const bool found = a.search ? search_item<R, KT>(a, item, w) : scan_item<R, KT>(a, item, w);
+    bool found = a.search ? search_item<R, KT>(a, item, w) : scan_item<R, KT>(a, item, w);
+    // Offsets that fall may make more items than the grid has. A tile whose parts pass the last one is left out whole,
+    // since the merge would read results that nothing wrote, past the workspace.
+    found = found && w.parts - w.part <= a.items - item;
     if (threadIdx.x == 0) {
       if (a.target) {
         int4 x = make_int4(0, 0, 0, 0);
