@@ -798,7 +798,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
       issue(vring, vbase, a.v_rs, t + NS);
     }
   }
-  if (a.causal && klast > lim_tile) {  // keys were hidden by causality: see the rows kernel
+  // Keys were hidden by causality: see the rows kernel. The last tile of 32 loads keys past kend, which hide even where
+  // all rows of the tile see the same keys (16 query heads of one key head: one token).
+  if (a.causal && kfirst + n32 * KEYS > lim_tile) {
     float z = 0.0f;
 #pragma unroll
     for (int d = 0; d < DB; ++d)

@@ -8,7 +8,7 @@ import torch
 
 from appcorr_amd import _lib
 from appcorr_amd import kernels as K
-from tests.test_gpu_packed import BF, HF, attention64, gen, near
+from tests.test_gpu_packed import BF, HF, attention64, gen, near, packed_case
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,27 @@ def test_falling_offsets_leave_the_merge_inside_its_workspace(dev):
     torch.cuda.synchronize()
     assert torch.isfinite(out).all() and (out[0] == 5).all() and (out[-1] == 5).all()
     assert torch.isnan(ws[need:]).all()
+
+
+@pytest.mark.parametrize("m,n,Hq,Hk", [([2], [100], 16, 1), ([2], [100], 32, 2), ([3, 1], [70, 33], 16, 1),
+                                       ([2, 0], [41, 9], 32, 1), ([1, 1, 2], [5, 64, 2500], 16, 1), ([2, 0], [2601, 9], 32, 1),
+                                       ([2, 1], [3001, 2500], 16, 1)])
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_hidden_values_of_a_group_that_fills_the_tile(dev, m, n, Hq, Hk, Dh, bad):
+    """16 or 32 query heads of a key head, so that a tile of 16 rows is one token: the last token's value is not finite,
+    and the tokens before it do not see it. The keys of the longer ones are split."""
+    for dtype in (BF, HF):
+        q, k, v, cu, keys = packed_case(dev, m, n, Hq, Hk, Dh, dtype, True, 61)
+        v = v.clone()
+        for s, b in enumerate(n):
+            v[s, b - 1:] = bad
+        got = K.packed_attention(q, k, v, cu, keys, Dh ** -0.5, causal=True).view(-1, Hq, Dh)
+        at = 0
+        for s, (a, b) in enumerate(zip(m, n)):
+            if a:
+                ref, slack = attention64(q[at:at + a - 1], k[s, :b - 1], v[s, :b - 1], a - 1, b - 1, Dh ** -0.5, True)
+                near(got[at:at + a - 1], ref, slack, f"{dtype} sequence {s}")
+                last = got[at + a - 1]
+                assert (last.isnan() if math.isnan(bad) else last == bad).all()
+            at += a
