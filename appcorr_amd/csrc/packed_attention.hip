@@ -58,6 +58,7 @@ struct PackedAttn {
   Divisor by_hk, by_g;
   int key_cap;
   bool cu_wide, keys_wide, batched, causal, search;
+  bool values_overlap;  // value rows closer than one row: past a tile's last key its descriptor shows values again
   float scale_log2;
   // Key parts: 0 = never split; else the number of parts that a key head's items are cut into at the most, beside
   // their own number, and the fewest key tiles of a part.
@@ -345,7 +346,9 @@ __device__ __forceinline__ float ref_shift(float m, float scale_log2) { return m
 // 46 -> 60 us). Beside the tiles a workgroup pays 4 to 5 us: its item, queries, first tiles and the output.
 // Hidden keys inside a sequence (causal) have score -inf, weight 0; a non-finite value among them would still give
 // 0 * inf = NaN in the second product. Only where a row came out non-finite is the item done again on a slow path
-// that takes such values out of the product and adds them to the rows that see them.
+// that takes such values out of the product and adds them to the rows that see them. So are, without a mask too, value
+// rows that lie closer than a row (one value for all keys, a cache of one token): the descriptor of a sequence's last
+// tile shows visible values again behind the last key.
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int W>
 __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn a) {
@@ -567,7 +570,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
     block_barrier();
     if (active) pipeline(std::true_type{});
     else pipeline(std::false_type{});
-    if (a.causal && (tb + ntiles) * kKeyTile > lim_tile) {  // keys were hidden by causality
+    if ((a.causal || a.values_overlap) && (tb + ntiles) * kKeyTile > lim_tile) {  // keys were hidden
       float z = 0.0f;
 #pragma unroll
       for (int d = 0; d < OB; ++d)
@@ -798,9 +801,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
       issue(vring, vbase, a.v_rs, t + NS);
     }
   }
-  // Keys were hidden by causality: see the rows kernel. The last tile of 32 loads keys past kend, which hide even where
+  // Keys were hidden: see the rows kernel. The last tile of 32 loads keys past kend, which hide even where
   // all rows of the tile see the same keys (16 query heads of one key head: one token).
-  if (a.causal && kfirst + n32 * KEYS > lim_tile) {
+  if ((a.causal || a.values_overlap) && kfirst + n32 * KEYS > lim_tile) {
     float z = 0.0f;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -1095,7 +1098,7 @@ extern "C" int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t 
                  (long long)parts);
   const PackedAttn a{q, q_rs, q_hs, k, v, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, cu_q, keys, out, out_rs, (int)rows, (int)S,
                      (int)Hk, (int)(Hq / Hk), Divisor((uint32_t)Hk), Divisor((uint32_t)(Hq / Hk)), (int)key_cap,
-                     cu_wide != 0, keys_wide != 0, batched != 0, causal != 0, s.search, scale * 1.4426950408889634f,
+                     cu_wide != 0, keys_wide != 0, batched != 0, causal != 0, s.search, v_rs < Dh, scale * 1.4426950408889634f,
                      s.target, s.min_tiles, (int)s.items, workspace,
                      s.target ? reinterpret_cast<int4*>(workspace + s.items * Hk * part_floats(s.R, (int)Dh)) : nullptr};
   hipStream_t st = as_stream(stream);

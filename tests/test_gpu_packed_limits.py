@@ -57,3 +57,30 @@ def test_hidden_values_of_a_group_that_fills_the_tile(dev, m, n, Hq, Hk, Dh, bad
                 last = got[at + a - 1]
                 assert (last.isnan() if math.isnan(bad) else last == bad).all()
             at += a
+
+
+@pytest.mark.parametrize("m,Dh", [(1, 64), (1, 128), (100, 64), (40, 128), (300, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_values_closer_than_a_row(dev, m, Dh, causal, bad):
+    """A cache of one token, one value for every key and value rows that overlap: an infinite value that a row sees is
+    that infinity in its dim, not NaN by meeting the weight 0 of keys past the last."""
+    g = gen(dev, 62)
+    for dtype in (BF, HF):
+        q = torch.randn(m, 2, Dh, generator=g, device=dev).to(dtype)
+        cu = torch.tensor([0, m], device=dev)
+        k = torch.randn(1, 70, 2, Dh, generator=g, device=dev).to(dtype)
+        one = torch.randn(1, 1, 2, Dh, generator=g, device=dev).to(dtype)
+        overlapping = torch.randn(8 * 69 + 2 * Dh, generator=g, device=dev).to(dtype)
+        one.view(-1)[1] = overlapping[8 * 69 + Dh - 1] = bad
+        for n, v in ((1, one), (70, one.expand(1, 70, 2, Dh)),
+                     (70, overlapping.as_strided((1, 70, 2, Dh), (0, 8, Dh, 1)))):
+            keys = torch.tensor([n], device=dev)
+            got = K.packed_attention(q, k[:, :n], v, cu, keys, Dh ** -0.5, causal=causal).view(m, 2, Dh)
+            p = torch.ones(m, n, dtype=torch.bool, device=dev)
+            if causal:
+                p = torch.arange(n, device=dev) <= torch.arange(m, device=dev)[:, None] + n - m
+            met = (p.double() @ (~torch.isfinite(v[0])).double().reshape(n, -1)).view(m, 2, Dh) > 0
+            assert met.any()
+            assert (got[met].isnan() if math.isnan(bad) else got[met] == bad).all()
+            assert torch.isfinite(got[~met]).all()
