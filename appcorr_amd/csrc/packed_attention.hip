@@ -1,6 +1,7 @@
 // Grouped-head attention of packed query rows over the keys of their own sequences, causal or not.
 //
-// A sequence of m rows and n keys: its row i sees the keys j < n (causal: j <= n - m + i),
+// A sequence of m rows and n keys: its row i sees the keys j < n (causal: j <= n - m + i), as far as the buffers hold
+// them,
 //   out = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c (q . k_j) - c mu),  c = scale log2 e,
 // with an online softmax: mu is a reference that follows the running maximum, and sum and output are rescaled when it
 // moves. Scores, statistics and outputs are fp32; the p_j are rounded to the element type for the second product, and
@@ -130,10 +131,12 @@ __device__ __forceinline__ int clamp_idx(int v, int lo, int hi) { return max(lo,
 // A sequence's rows and keys, and the item that a workgroup takes of it. Uniform over the wave.
 struct Item {
   int seq, q0, m, n, k0;  // first row, rows, keys, first key row (packed keys)
+  int before;             // causal: row i sees the first before + i + 1 of the keys
   int tile, part, parts;
 };
 
-// Sequence s: rows and keys, cut to the buffers.
+// Sequence s: rows and keys, cut to the buffers. Rows and keys that are cut off still count for what the others see: the
+// last row of the uncut sequence sees the last of its uncut keys.
 __device__ __forceinline__ void load_seq(const PackedAttn& a, int s, Item& t) {
   const int c0 = load_idx(a.cu_q, s, a.cu_wide), c1 = load_idx(a.cu_q, s + 1, a.cu_wide);
   const int k0 = load_idx(a.keys, s, a.keys_wide), k1 = load_idx(a.keys, s + (a.batched ? 0 : 1), a.keys_wide);
@@ -141,6 +144,9 @@ __device__ __forceinline__ void load_seq(const PackedAttn& a, int s, Item& t) {
   t.m = clamp_idx(c1, t.q0, a.rows) - t.q0;
   t.k0 = a.batched ? 0 : clamp_idx(k0, 0, a.key_cap);
   t.n = clamp_idx(k1, t.k0, a.key_cap) - t.k0;
+  // (m, n < 2^30: what passes them either way sees all or nothing)
+  const int64_t before = (int64_t)k1 - t.k0 - ((int64_t)c1 - t.q0);
+  t.before = (int)max(-(int64_t)(1 << 30), min((int64_t)(1 << 30), before));
 }
 
 // Wave-wide sums and maxima by data-parallel moves (no LDS round trips): value of every lane combined with those of
@@ -208,7 +214,7 @@ __device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w
   auto tiles = [&]() { return (t.m * a.G + R - 1) / R; };
   auto key_tiles = [&]() { return (t.n + KT - 1) / KT; };
   auto load = [&](int s0) {
-    t.q0 = t.m = t.n = t.k0 = 0;
+    t.q0 = t.m = t.n = t.k0 = t.before = 0;
     if (s0 + lane < a.S) load_seq(a, s0 + lane, t);
   };
   load(0);
@@ -241,6 +247,7 @@ __device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w
         w.m = __builtin_amdgcn_readlane(t.m, l);
         w.n = __builtin_amdgcn_readlane(t.n, l);
         w.k0 = __builtin_amdgcn_readlane(t.k0, l);
+        w.before = __builtin_amdgcn_readlane(t.before, l);
         w.parts = __builtin_amdgcn_readlane(parts, l);
         const int from_last = w.parts == 1 ? within : within / w.parts;
         w.part = within - from_last * w.parts;
@@ -259,7 +266,7 @@ __device__ __forceinline__ bool scan_item(const PackedAttn& a, int item, Item& w
 // grid says, those without an item too.
 template <int R, int KT>
 __device__ __forceinline__ bool take_item(const PackedAttn& a, int item, int h, Item& w) {
-  __shared__ int shared[9];
+  __shared__ int shared[10];
   if (threadIdx.x < 64) {
     w = Item{};
     bool found = a.search ? search_item<R, KT>(a, item, w) : scan_item<R, KT>(a, item, w);
@@ -281,18 +288,19 @@ __device__ __forceinline__ bool take_item(const PackedAttn& a, int item, int h, 
       shared[5] = w.tile;
       shared[6] = w.part;
       shared[7] = w.parts;
-      shared[8] = found;
+      shared[8] = w.before;
+      shared[9] = found;
     }
   }
   __syncthreads();
   auto get = [&](int i) { return __builtin_amdgcn_readfirstlane(shared[i]); };
-  w = Item{get(0), get(1), get(2), get(3), get(4), get(5), get(6), get(7)};
-  return get(8) != 0;
+  w = Item{get(0), get(1), get(2), get(3), get(4), get(8), get(5), get(6), get(7)};
+  return get(9) != 0;
 }
 
 // Keys that token i of the sequence sees.
 __device__ __forceinline__ int seen_keys(const PackedAttn& a, const Item& w, int i) {
-  return a.causal ? min(w.n, max(0, w.n - w.m + i + 1)) : w.n;
+  return a.causal ? min(w.n, max(0, w.before + i + 1)) : w.n;
 }
 
 // Floats of one part: reference and sum of R rows, then R rows of DH.

@@ -1523,7 +1523,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     k, v either packed [Mk, Hk, Dh] with keys = cu_k [S + 1] (rows cu_k[s] .. cu_k[s + 1] - 1), or a cache
     [B, N, Hk, Dh] (kv_cache[:, :, 0] and [:, :, 1]) with keys = the key counts [S]: sequence s reads the first
     keys[s] of batch s. Query head h reads key head h // (Hq / Hk). causal: row i of a sequence's m sees the keys
-    0 .. n - m + i of its n, so the last row sees all; else every row sees all n.
+    0 .. n - m + i of its n, so the last row sees all; else every row sees all n. Rows and keys outside the buffers are
+    left out, but counted in m and n: with keys[s] past N, every row sees what the cache holds of its own past.
     A row without keys gives 0; hidden keys have no influence, NaN or infinite ones neither. Rows of `out` behind
     the last sequence stay as they were (undefined in a new tensor). scale must be positive. bf16 or fp16; Dh 64
     or 128. With few query rows the keys of a sequence are split over workgroups and merged, in a fixed order. `out`

@@ -787,12 +787,13 @@ int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t rows, int6
                            int64_t qo_rs, oudjat_stream_t stream);
 
 /* Grouped-head attention of packed query rows over the keys of their own sequences. Query head h reads key head
- * h / (Hq / Hk). Sequence s has query rows cu_q[s] .. cu_q[s + 1] - 1 (int32, or int64 if cu_wide; cut to 0 .. rows)
- * of q [rows, Hq, Dh] and n_s keys:
- *   batched: keys (s, 0 .. n_s - 1) of k, v [>= S, key_cap, Hk, Dh] (strides k_bs, k_rs, k_hs and the same for v),
- *            n_s = keys[s] cut to 0 .. key_cap;
- *   packed:  rows keys[s] .. keys[s + 1] - 1 of k, v [key_cap, Hk, Dh] (k_bs, v_bs unused), cut to 0 .. key_cap.
- *   (keys: int32, or int64 if keys_wide.)
+ * h / (Hq / Hk). Sequence s has query rows cu_q[s] .. cu_q[s + 1] - 1 (int32, or int64 if cu_wide) of q [rows, Hq, Dh]
+ * and n_s keys:
+ *   batched: n_s = keys[s], keys (s, 0 .. n_s - 1) of k, v [>= S, key_cap, Hk, Dh] (strides k_bs, k_rs, k_hs and the
+ *            same for v);
+ *   packed:  rows keys[s] .. keys[s + 1] - 1 of k, v [key_cap, Hk, Dh] (k_bs, v_bs unused).
+ *   (keys: int32, or int64 if keys_wide.) Rows outside 0 .. rows - 1 and keys outside 0 .. key_cap - 1 do not exist, but
+ *   count in m and n_s below: a sequence longer than its cache keeps the causal edge of its rows.
  * out[r, h*Dh..] = softmax(q . K^T * scale) . V in fp32 with the probabilities rounded to the type; causal: row i of
  * a sequence's m sees keys 0 .. n_s - m + i (the last row sees all). A row that sees no key is 0; hidden keys and
  * values have no influence whatever they hold; rows past the last sequence are not written.

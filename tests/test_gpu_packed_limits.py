@@ -84,3 +84,54 @@ def test_values_closer_than_a_row(dev, m, Dh, causal, bad):
             assert met.any()
             assert (got[met].isnan() if math.isnan(bad) else got[met] == bad).all()
             assert torch.isfinite(got[~met]).all()
+
+
+def edge_reference(q, k, v, first, end, k0, k1, scale):
+    """(out, slack) of the rows `first` .. `end` of a buffer, a sequence whose last row is end - 1 and whose keys are rows
+    k0 .. k1 - 1 of a key buffer, causal: row r sees the key rows up to k1 - end + r. What lies outside a buffer is
+    not there."""
+    rows = range(max(0, first), min(end, q.shape[0]))
+    outs = []
+    for r in rows:
+        lo, hi = max(0, k0), min(k.shape[0], k1 - end + r + 1)
+        outs.append(attention64(q[r:r + 1], k[lo:max(lo, hi)], v[lo:max(lo, hi)], 1, max(0, hi - lo), scale, True))
+    return rows, torch.cat([o for o, _ in outs]), torch.cat([s for _, s in outs])
+
+
+@pytest.mark.parametrize("m,n,N,Hq,Hk,Dh", [
+    ([4], [54], 50, 2, 2, 64), ([10, 1, 3], [54, 51, 40], 50, 4, 1, 128), ([70], [130], 100, 8, 2, 64),
+    ([300, 2], [500, 90], 299, 4, 1, 128), ([5, 1], [2601, 1 << 40], 2500, 8, 1, 64), ([200], [4000], 3900, 2, 1, 128),
+    ([90], [70], 64, 2, 1, 64), ([1] * 70, [40 + i for i in range(70)], 60, 2, 2, 64), ([9], [1 << 40], 33, 2, 2, 64)])
+def test_causal_edge_of_sequences_longer_than_their_cache(dev, m, n, N, Hq, Hk, Dh):
+    """Row i of m sees the keys up to its own token n - m + i, as far as the cache holds them."""
+    for dtype in (BF, HF):
+        q, k, v, cu, _ = packed_case(dev, m, [N] * len(m), Hq, Hk, Dh, dtype, True, 63)
+        k, v = k[:, :N], v[:, :N]
+        got = K.packed_attention(q, k, v, cu, torch.tensor(n, device=dev), Dh ** -0.5, causal=True).view(-1, Hq, Dh)
+        at = 0
+        for s, (a, b) in enumerate(zip(m, n)):
+            rows, ref, slack = edge_reference(q, k[s], v[s], at, at + a, 0, b, Dh ** -0.5)
+            near(got[rows.start:rows.stop], ref, slack, f"{dtype} sequence {s}")
+            at += a
+
+
+@pytest.mark.parametrize("cu,cu_k,M,Mk,Hq,Hk,Dh", [
+    ([0, 3, 7, 12], [0, 10, 20, 30], 8, 30, 2, 2, 64), ([0, 60, 500], [0, 100, 2300], 200, 1500, 4, 2, 64),
+    ([-5, 20, 45], [-4, 30, 70], 40, 60, 4, 1, 128), ([0, 2, 3], [0, 3000, 1 << 40], 3, 3500, 8, 1, 128),
+    ([-(1 << 40), 5], [0, 20], 10, 20, 2, 1, 64), ([0, 700], [-300, 500], 400, 450, 2, 1, 128),
+    (list(range(0, 140, 2)), list(range(0, 1400, 20)), 101, 1111, 2, 2, 64)])
+def test_causal_edge_of_offsets_outside_the_buffers(dev, cu, cu_k, M, Mk, Hq, Hk, Dh):
+    g = gen(dev, 64)
+    for dtype in (BF, HF):
+        q = torch.randn(M, Hq, Dh, generator=g, device=dev).to(dtype)
+        kv = torch.randn(Mk, 2, Hk, Dh, generator=g, device=dev).to(dtype)
+        k, v = kv[:, 0], kv[:, 1]
+        out = torch.full((M, Hq * Dh), 5.0, device=dev, dtype=dtype)
+        K.packed_attention(q, k, v, torch.tensor(cu, device=dev), torch.tensor(cu_k, device=dev), Dh ** -0.5, causal=True,
+                           out=out)
+        for s in range(len(cu) - 1):
+            if max(cu[s], 0) >= min(cu[s + 1], M):
+                continue
+            rows, ref, slack = edge_reference(q, k, v, cu[s], cu[s + 1], cu_k[s], cu_k[s + 1], Dh ** -0.5)
+            near(out.view(M, Hq, Dh)[rows.start:rows.stop], ref, slack, f"{dtype} sequence {s}")
+        assert (out[min(cu[-1], M):] == 5.0).all()
