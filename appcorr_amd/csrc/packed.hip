@@ -9,13 +9,16 @@
 namespace oudjat {
 
 // ------------------------------------------------------------------------------------------------
-// packed_plan. With nq_s = max(q_lens[s], 0) and the offsets c_s = min(sum of nq before s, rows), sequence s has
-// rows c_s .. c_{s+1} - 1; its key count is k_lens[s] cut to 0 .. cache_len (or, packed keys, what is left of
-// key_rows), and row r of it is token k_s - c_{s+1} + r of sequence s: its new rows are its last tokens.
+// packed_plan. With nq_s = max(q_lens[s], 0), nk_s = max(k_lens[s], 0) and the offsets c_s = min(sum of nq before s,
+// rows), sequence s has rows c_s .. c_{s+1} - 1, the first of its new rows where the buffer ends inside them. A
+// sequence's new rows are its last tokens, so row r is token first_s + r - c_s, first_s = nk_s - nq_s, and the keys that
+// go with the rows that are there are n_s = max(0, first_s + c_{s+1} - c_s). A token has a slot where it is not negative
+// and below cache_len. Packed keys: sequence s has key rows from the sum of n before it on, if all n_s fit into
+// key_rows, else none, and its rows no slots.
 // Every workgroup scans all lengths for itself (at most kPlanMaxSeqs of them, read from L2, offsets in LDS) and
 // then looks its own rows up by bisection, so that the plan is one launch and no workgroup waits for another.
-// Bound by that scan's latency: a thread reads its lengths eight at a time, scans within its wave by lane
-// shuffles and across waves through LDS.
+// Bound by that scan's latency: a thread reads its lengths eight at a time (once, up to 2048 sequences), scans within
+// its wave by lane shuffles and across waves through LDS.
 // ------------------------------------------------------------------------------------------------
 static constexpr int kPlanThreads = 256;
 static constexpr int kPlanMaxSeqs = 4096;     // 2 x 16 KB of LDS
@@ -59,49 +62,77 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(
     int64_t* __restrict__ cu_k, int64_t* __restrict__ batch_idx, int64_t* __restrict__ token_idx) {
   extern __shared__ int32_t plan_lds[];
   int32_t* ends = plan_lds;         // c_{s+1}
-  int32_t* toks = plan_lds + S;     // k_s - c_{s+1}: token of row r is toks[s] + r
+  int32_t* toks = plan_lds + S;     // first_s - c_s: token of row r is toks[s] + r; INT32_MIN: no row has a slot
   __shared__ int64_t wave_sums[kPlanThreads / 64];
+  __shared__ int32_t last_fit;      // packed keys: the key rows up to the last sequence that fits
   const int tid = threadIdx.x;
   const int per = (S + kPlanThreads - 1) / kPlanThreads;
   const int s0 = min(tid * per, S), s1 = min(s0 + per, S);
-  int64_t nq = 0, nk = 0, total;
-  for (int s = s0; s < s1; s += 8) {
-    int64_t a[8], b[8];
+  int64_t ql[8], kl[8];  // lengths of sequences s .. s + 7
+  auto load = [&](int s) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = min(s + e, S - 1);
-      a[e] = load_len(q_lens, i, q_wide);
-      b[e] = load_len(k_lens, i, k_wide);
+      ql[e] = load_len(q_lens, i, q_wide);
+      kl[e] = load_len(k_lens, i, k_wide);
     }
+  };
+  int64_t cq = 0, ck = 0, total;
+  // This thread's sequences in turn: f(sequence, its rows' begin and end, token of its first
+  // row, its keys n).
+  auto each = [&](int64_t q0, auto&& f) {
+    for (int s = s0; s < s1; s += 8) {
+      if (per > 8) load(s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (s + e < s1) {
+          const int64_t begin = min(q0, rows);
+          q0 += clamp_len(ql[e], rows);
+          const int64_t end = min(q0, rows), first = max(kl[e], (int64_t)0) - max(ql[e], (int64_t)0);
+          f(s + e, (int32_t)begin, (int32_t)end, first, max(first + end - begin, (int64_t)0));
+        }
+    }
+  };
+  if (s0 < s1 && per <= 8) load(s0);
+  int64_t nq = 0, nk = 0;
+  for (int s = s0; s < s1; s += 8) {
+    if (per > 8) load(s);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (s + e < s1) {
-        nq += clamp_len(a[e], rows);
-        nk += clamp_len(b[e], key_cap);
-      }
+      if (s + e < s1) nq += clamp_len(ql[e], rows);
   }
-  int64_t cq = block_scan(nq, wave_sums, &total);
-  int64_t ck = block_scan(nk, wave_sums, &total);
+  cq = block_scan(nq, wave_sums, &total);
+  // Keys of a sequence in the running sum: what the cache holds of them, or all (one that does not fit is past the end).
+  auto held = [&](int64_t n) { return packed_keys ? min(n, key_cap + 1) : min(n, key_cap); };
+  each(cq, [&](int, int32_t, int32_t, int64_t, int64_t n) { nk += held(n); });
+  if (tid == 0) last_fit = 0;
+  ck = block_scan(nk, wave_sums, &total);
   const bool writer = blockIdx.x == 0;  // the per-sequence results are written once
-  for (int s = s0; s < s1; ++s) {
-    const int64_t kb = packed_keys ? min(ck, key_cap) : ck;
-    cq += clamp_len(load_len(q_lens, s, q_wide), rows);
-    ck += clamp_len(load_len(k_lens, s, k_wide), key_cap);
-    const int64_t ke = packed_keys ? min(ck, key_cap) : ck;
-    const int32_t end = (int32_t)min(cq, rows), klen = (int32_t)(ke - kb);
+  int64_t ke = ck;
+  each(cq, [&](int s, int32_t begin, int32_t end, int64_t first, int64_t n) {
+    ke += held(n);
+    const bool fits = !packed_keys || ke <= key_cap;
     ends[s] = end;
-    toks[s] = klen - end;
+    toks[s] = n > 0 && first < key_cap && fits ? (int32_t)(first - begin) : INT32_MIN;  // (n > 0: first > -end)
     if (writer) {
       cu_q[s + 1] = end;
-      k_out[s] = klen;
-      cu_k[s + 1] = ke;
+      k_out[s] = fits ? (int32_t)min(n, (int64_t)INT32_MAX) : 0;
+      if (fits) cu_k[s + 1] = ke;
+      if (packed_keys && fits) atomicMax(&last_fit, (int32_t)ke);
     }
-  }
+  });
   if (writer && tid == 0) {
     cu_q[0] = 0;
     cu_k[0] = 0;
   }
   __syncthreads();
+  if (writer && packed_keys) {
+    ke = ck;
+    each(cq, [&](int s, int32_t, int32_t, int64_t, int64_t n) {
+      ke += held(n);
+      if (ke > key_cap) cu_k[s + 1] = last_fit;
+    });
+  }
   const int64_t r0 = ((int64_t)blockIdx.x * kPlanThreads + tid) * kPlanRowsPerThread;
   if (r0 >= rows) return;
   int64_t bi[kPlanRowsPerThread], ti[kPlanRowsPerThread];
@@ -114,9 +145,10 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(
       if (ends[mid] > r) hi = mid;
       else lo = mid + 1;
     }
-    const int t = lo < S ? toks[lo] + r : -1;
-    bi[e] = t >= 0 ? lo : -1;
-    ti[e] = t >= 0 ? t : -1;
+    const int64_t t = lo < S ? (int64_t)toks[lo] + r : -1;
+    const bool slot = t >= 0 && t < key_cap;
+    bi[e] = slot ? lo : -1;
+    ti[e] = slot ? t : -1;
   }
   if (r0 + 1 < rows) {
     typedef int64_t i64x2_t __attribute__((ext_vector_type(2)));

@@ -1379,8 +1379,9 @@ def _rows_packed(t: torch.Tensor, inner: int) -> bool:
 
 @dataclass
 class PackedPlan:
-    """Offsets and cache slots of packed rows (packed_plan): cu_q int32 [S + 1], k_lens int32 [S], cu_k int64
-    [S + 1], batch_idx and token_idx int64 [rows] (-1 where a row has no slot)."""
+    """Offsets and cache slots of packed rows (packed_plan): cu_q int32 [S + 1], k_lens int32 [S] (past cache_len where a
+    sequence is longer than its cache), cu_k int64 [S + 1] (the running sum of the keys that a buffer holds), batch_idx
+    and token_idx int64 [rows] (-1 where a row has no slot)."""
     cu_q: torch.Tensor
     k_lens: torch.Tensor
     cu_k: torch.Tensor
@@ -1393,10 +1394,12 @@ def packed_plan(q_lens: torch.Tensor, k_lens: torch.Tensor, rows: int, *, cache_
     """Where the rows of S sequences lie, from their lengths on the device (nothing is read back).
 
     Sequence s has q_lens[s] new rows in a buffer of `rows` and k_lens[s] keys, its new rows the last of them.
-    Exactly one of cache_len (every sequence has its own cache of that many tokens; k_lens are cut to it) and
-    key_rows (keys packed like the queries in that many rows) is given. Row r of sequence s is token_idx[r] of
-    batch_idx[r] = s, which is also its position there; rows behind the last sequence and rows that come before
-    token 0 have -1, -1. Lengths below 0 count as 0; rows past `rows` are cut off. At most 4096 sequences."""
+    Exactly one of cache_len (every sequence has its own cache of that many tokens) and key_rows (keys packed like the
+    queries in that many rows) is given. Row i of sequence s is its token k_lens[s] - q_lens[s] + i: token_idx of
+    batch_idx = s, which is also its position. Rows past `rows` are cut off, and their tokens do not count in the plan's
+    k_lens. Rows behind the last sequence, before token 0 and past the cache have -1, -1; the plan's k_lens count the
+    latter, so that packed_attention places the causal edge. Packed keys: a sequence whose keys do not all fit
+    into key_rows has none, its rows -1, -1. Lengths below 0 count as 0. At most 4096 sequences."""
     dev = _gpu_of(q_lens, k_lens)
     S = q_lens.numel()
     _require(_is_lengths(q_lens, S) and _is_lengths(k_lens, S),

@@ -746,13 +746,17 @@ enum oudjat_dtype { OUDJAT_BF16 = 0, OUDJAT_FP16 = 1 };
 enum oudjat_pos { OUDJAT_POS_I32 = 0, OUDJAT_POS_I64 = 1, OUDJAT_POS_F32 = 2 };
 
 /* Row offsets, key lengths and cache slots of S sequences from their lengths (device arrays; *_wide: int64, else
- * int32). q_lens[s] new rows, k_lens[s] keys with these among them. Negative lengths count as 0.
- *   cu_q [S + 1] int32: cu_q[s + 1] = min(q_lens[0] + .. + q_lens[s], rows);
- *   k_out [S] int32: the key lengths, each cut to key_cap (a cache of key_cap tokens per sequence), or, with
- *     packed_keys, their running sum cut to key_cap (key rows packed like the queries); cu_k [S + 1] int64 the
- *     running sum;
- *   batch_idx, token_idx [rows] int64: row r of sequence s is token k_out[s] - cu_q[s + 1] + r of it (a sequence's
- *     new rows are its last tokens); -1, -1 for rows past the last sequence and where that token is negative.
+ * int32). q_lens[s] new rows, k_lens[s] keys with these among them, the new rows the last tokens: row i of sequence s is
+ * its token t = k_lens[s] - q_lens[s] + i. Negative lengths count as 0.
+ *   cu_q [S + 1] int32: cu_q[s + 1] = min(q_lens[0] + .. + q_lens[s], rows): what passes the row buffer is left out,
+ *     the last rows of a sequence first;
+ *   k_out [S] int32: the keys up to the sequence's last row in the buffer, max(0, k_lens[s] less its rows left out). It
+ *     may pass key_cap, the tokens that a sequence's cache holds: oudjat_packed_attention reads those, and places the
+ *     causal edge by k_out. packed_keys (key_cap key rows for all, packed like the queries): 0 where they do not all
+ *     fit behind the keys of the sequences before;
+ *   cu_k [S + 1] int64: the running sum of k_out, each cut to key_cap;
+ *   batch_idx, token_idx [rows] int64: s and t of every row; -1, -1 for rows past the last sequence, where t is negative
+ *     or not below key_cap, and (packed_keys) where the sequence's keys do not fit.
  * At most 4096 sequences; row maps 16-byte aligned. */
 int oudjat_packed_plan(const void* q_lens, int q_wide, const void* k_lens, int k_wide, int64_t S, int64_t rows,
                        int64_t key_cap, int packed_keys, int32_t* cu_q, int32_t* k_out, int64_t* cu_k,

@@ -2,6 +2,7 @@
 rows, groups as large as a tile, value rows that overlap, heads at the ends of the type's range."""
 
 import math
+import random
 
 import pytest
 import torch
@@ -135,3 +136,124 @@ def test_causal_edge_of_offsets_outside_the_buffers(dev, cu, cu_k, M, Mk, Hq, Hk
             rows, ref, slack = edge_reference(q, k, v, cu[s], cu[s + 1], cu_k[s], cu_k[s + 1], Dh ** -0.5)
             near(out.view(M, Hq, Dh)[rows.start:rows.stop], ref, slack, f"{dtype} sequence {s}")
         assert (out[min(cu[-1], M):] == 5.0).all()
+
+
+def plan_reference(q_lens, k_lens, rows, cache_len, key_rows):
+    """Token by token: row i of a sequence is token k - q + i; rows past the buffer are not there, nor are their tokens."""
+    cu_q, nk, cu_k, batch, token = [0], [], [0], [], []
+    for s, (a, b) in enumerate(zip(q_lens, k_lens)):
+        a, b = max(a, 0), max(b, 0)
+        kept = min(a, rows - len(batch))
+        n = max(0, b - (a - kept))
+        fits = cache_len is not None or cu_k[-1] + n <= key_rows and (not nk or nk[-1] is not None)
+        cap = key_rows if cache_len is None else cache_len
+        for t in range(b - a, b - a + kept):
+            there = fits and 0 <= t < cap
+            batch.append(s if there else -1)
+            token.append(t if there else -1)
+        cu_q.append(len(batch))
+        nk.append(min(n, (1 << 31) - 1) if fits else None)
+        cu_k.append(cu_k[-1] + (min(n, cap) if fits else 0))
+    pad = [-1] * (rows - len(batch))
+    return cu_q, [n or 0 for n in nk], cu_k, batch + pad, token + pad
+
+
+def check_plan(dev, q_lens, k_lens, rows, want=None, dtype=torch.int64, **cap):
+    p = K.packed_plan(torch.tensor(q_lens, dtype=dtype, device=dev), torch.tensor(k_lens, dtype=dtype, device=dev), rows,
+                      **cap)
+    ref = plan_reference(q_lens, k_lens, rows, cap.get("cache_len"), cap.get("key_rows"))
+    for i, name in enumerate(("cu_q", "k_lens", "cu_k", "batch_idx", "token_idx")):
+        got = getattr(p, name).tolist()
+        assert got == ref[i], name
+        assert want is None or got == want[i], name
+
+
+@pytest.mark.parametrize("q_lens,k_lens,rows,cap,want", [
+    # The row buffer ends inside the third sequence: its first row is its token 5, and 5 earlier tokens are its keys.
+    ([3, 4, 5], [10, 10, 10], 8, dict(cache_len=50),
+     ([0, 3, 7, 8], [10, 10, 6], [0, 10, 20, 26], [0, 0, 0, 1, 1, 1, 1, 2], [7, 8, 9, 6, 7, 8, 9, 5])),
+    # The second one's rows are all left out: what was cached of it stays.
+    ([4, 3, 0], [4, 9, 2], 4, dict(cache_len=50), ([0, 4, 4, 4], [4, 6, 2], [0, 4, 10, 12], [0] * 4, [0, 1, 2, 3])),
+    # Tokens 50 .. 53 of a cache of 50, and 48 .. 51: only the first two have a slot.
+    ([4, 4], [54, 52], 8, dict(cache_len=50), ([0, 4, 8], [54, 52], [0, 50, 100], [-1] * 4 + [1, 1, -1, -1],
+                                               [-1] * 4 + [48, 49, -1, -1])),
+    # Both: of 9 new rows, tokens 45 .. 53, the buffer has 7.
+    ([9], [54], 7, dict(cache_len=50), ([0, 7], [52], [0, 50], [0] * 5 + [-1] * 2, [45, 46, 47, 48, 49, -1, -1])),
+    # Packed keys, rows cut: prompts of 3, 4 and 5 rows in buffers of 8.
+    ([3, 4, 5], [3, 4, 5], 8, dict(key_rows=8), ([0, 3, 7, 8], [3, 4, 1], [0, 3, 7, 8], [0] * 3 + [1] * 4 + [2],
+                                                 [0, 1, 2, 0, 1, 2, 3, 0])),
+    # Packed keys, too few key rows for the second sequence and so for all behind it.
+    ([2, 2, 1], [4, 7, 1], 5, dict(key_rows=10), ([0, 2, 4, 5], [4, 0, 0], [0, 4, 4, 4], [0, 0, -1, -1, -1],
+                                                  [2, 3, -1, -1, -1])),
+    # Lengths past 31 and 32 bits.
+    ([1 << 40, 5], [1 << 40, 9], 3, dict(cache_len=20), ([0, 3, 3], [3, 4], [0, 3, 7], [0] * 3, [0, 1, 2])),
+    ([2, 2], [(1 << 40) + 1, 2], 4, dict(cache_len=20), ([0, 2, 4], [(1 << 31) - 1, 2], [0, 20, 22], [-1, -1, 1, 1],
+                                                       [-1, -1, 0, 1])),
+    ([3, 1], [(1 << 31) - 1, 1], 4, dict(cache_len=(1 << 31) - 2),
+     ([0, 3, 4], [(1 << 31) - 1, 1], [0, (1 << 31) - 2, (1 << 31) - 1], [0, 0, -1, 1],
+      [(1 << 31) - 4, (1 << 31) - 3, -1, 0])),
+    ([1 << 62], [1], 2, dict(cache_len=20), ([0, 2], [0], [0, 0], [-1, -1], [-1, -1])),
+])
+def test_plan_of_lengths_past_the_buffers(dev, q_lens, k_lens, rows, cap, want):
+    check_plan(dev, q_lens, k_lens, rows, want, **cap)
+    if max(q_lens + k_lens) < 1 << 31:
+        check_plan(dev, q_lens, k_lens, rows, want, dtype=torch.int32, **cap)
+
+
+@pytest.mark.parametrize("S", [1, 2, 7, 64, 65, 256, 257, 1000, 2048, 2049, 4096])
+def test_plan_of_many_sequences_past_the_buffers(dev, S):
+    rng = random.Random(S)
+    q = [rng.choice([-1, 0, 1, rng.randrange(40)]) for _ in range(S)]
+    k = [max(a, 0) + rng.randrange(-3, 100) for a in q]
+    for rows in (sum(max(a, 0) for a in q) + 5, sum(max(a, 0) for a in q) // 3):
+        check_plan(dev, q, k, rows, cache_len=90)
+        check_plan(dev, q, k, rows, cache_len=1000)
+        check_plan(dev, q, k, rows, key_rows=sum(max(b, 0) for b in k) // 2)
+        check_plan(dev, q, k, rows, key_rows=sum(max(b, 0) for b in k))
+        check_plan(dev, q, k, rows, key_rows=0)
+
+
+@pytest.mark.parametrize("rows,N,key_rows", [(9, 50, None), (40, 50, None), (23, 30, None), (26, None, 90), (12, None, 60)])
+def test_layer_of_sequences_past_the_buffers(dev, rows, N, key_rows):
+    """Plan, rotation with the K/V write and attention of sequences that do not fit: every row meets the keys of its own
+    past that are there, at their own tokens, and what was cached before stays."""
+    Hq, Hk, Dh, g = 4, 2, 64, gen(dev, 65)
+    new, total = [6, 1, 11, 8], [25, 31, 34, 20]
+    plan = K.packed_plan(torch.tensor(new, device=dev), torch.tensor(total, device=dev), rows, cache_len=N,
+                         key_rows=key_rows)
+    qkv = torch.randn(rows, Hq + 2 * Hk, Dh, generator=g, device=dev).to(BF)
+    q = torch.zeros(rows, Hq, Dh, device=dev, dtype=BF)
+    pos = torch.zeros(rows, 1, device=dev, dtype=torch.int64)  # no rotation: keys are only normed
+    freq = torch.ones(32, device=dev)
+    n = N or max(total)
+    old = torch.randn(4, n, 2, Hk, Dh, generator=g, device=dev).to(BF)
+    kv = old.clone()
+    K.qk_norm_rope_kv(qkv, Hq, Hk, (None, None), (None, None), 1e-6, pos, freq, (32,), plan.batch_idx, plan.token_idx,
+                      kv, q)
+    if N:
+        got = K.packed_attention(q, kv[:, :, 0], kv[:, :, 1], plan.cu_q, plan.k_lens, Dh ** -0.5, causal=True)
+    else:
+        ck = plan.cu_k.tolist()
+        flat = torch.cat([kv[s, :ck[s + 1] - ck[s]] for s in range(4)] + [torch.full_like(kv[0, :1], math.nan)])
+        got = K.packed_attention(q, flat[:, 0], flat[:, 1], plan.cu_q, plan.cu_k, Dh ** -0.5, causal=True)
+    normed = qkv[:, Hq:Hq + Hk].double()
+    normed = normed / (normed.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt()
+    r, room = 0, key_rows
+    for s, (a, b) in enumerate(zip(new, total)):
+        kept = min(a, rows - r)
+        if room is not None:
+            room -= b - a + kept
+        fits = room is None or room >= 0
+        for i in range(kept):
+            t = b - a + i
+            if fits and t < n:  # the row's own key and value lie at its token
+                assert (kv[s, t, 0].double() - normed[r]).abs().max() <= 2.0 ** -7 * normed[r].abs().max()
+                assert torch.equal(kv[s, t, 1], qkv[r, Hq + Hk:])
+            seen = min(t + 1, n) if fits else 0
+            ref, slack = attention64(q[r:r + 1], kv[s, :seen, 0], kv[s, :seen, 1], 1, seen, Dh ** -0.5, True)
+            if fits and t < n:
+                near(got[r:r + 1].view(1, Hq, Dh), ref, slack, f"sequence {s} row {i}")
+            elif not fits:
+                assert not got[r].any()
+            r += 1
+        assert torch.equal(kv[s, :min(n, b - a)], old[s, :min(n, b - a)]), "tokens cached before were written"
