@@ -353,22 +353,43 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kv_kernel(
       float x[16], y[16];
       E::to8(x0, x);
       E::to8(x1, x + 8);
-      if constexpr (LAYER) {
-        float s = 0.0f;
+      // mean(x^2) + eps of the head's values (LayerNorm: less their mean, which is taken off x).
+      auto variance = [&](float eps_) {
+        if constexpr (LAYER) {
+          float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += x[e];
+          for (int e = 0; e < 16; ++e) s += x[e];
 #pragma unroll
-        for (int d = L / 2; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
-        s *= 1.0f / DH;
+          for (int d = L / 2; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
+          s *= 1.0f / DH;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] -= s;
+          for (int e = 0; e < 16; ++e) x[e] -= s;
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+        for (int d = L / 2; d > 0; d >>= 1) ss += __shfl_xor(ss, d, 64);
+        return fmaf(ss, 1.0f / DH, eps_);
+      };
+      float var = variance(eps);
+      if (!(var > 0x1p-100f && var < 0x1p126f)) {
+        // Sums or squares that leave fp32's range (bf16 values from 1e19 on; below 1e-15 where eps is as small): the head
+        // again, scaled by a power of two that takes its largest value to 1 .. 4, or from far below towards it.
+        E::to8(x0, x);
+        E::to8(x1, x + 8);
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+        for (int d = L / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        const int exponent = (int)(__float_as_uint(top) >> 23) - 127;
+        const float scale = ldexpf(1.0f, -max(var < 1.0f ? -100 : 0, min(126, exponent)));  // (eps scale^2 is finite)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] *= scale;
+        var = variance(eps * scale * scale);
       }
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int d = L / 2; d > 0; d >>= 1) ss += __shfl_xor(ss, d, 64);
-      const float inv = 1.0f / sqrtf(fmaf(ss, 1.0f / DH, eps));
+      const float inv = 1.0f / sqrtf(var);
       const int which = h < Hq ? 0 : 1;
       E::to8(which ? w[1][0] : w[0][0], y);
       E::to8(which ? w[1][1] : w[0][1], y + 8);

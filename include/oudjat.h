@@ -780,7 +780,7 @@ int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, const uint16
  * Dh values or NULL), rotated as in oudjat_rope_axes, rounded once; queries to q_out [rows, Hq, Dh] (row stride
  * qo_rs), keys and (unchanged) values to kv + batch * kv_bs + token * kv_ns (+ kv_cs for values), Hk x Dh packed.
  * Rows whose (batch, token) lies outside B x N are skipped: neither q_out nor the cache is written for them. The
- * slots of the other rows must be unique. Dh 64 or 128; 16-byte aligned rows, those of q_out and of the cache apart
+ * slots of the other rows must be unique. Heads whose squares leave fp32's range are scaled first. Dh 64 or 128; 16-byte aligned rows, those of q_out and of the cache apart
  * (any order of its strides). Neither output may overlap qkv. */
 int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t rows, int64_t Hq, int64_t Hk, int64_t Dh,
                            int dtype, int layer_norm, const uint16_t* q_weight, const uint16_t* q_bias,

@@ -9,7 +9,8 @@ import torch
 
 from appcorr_amd import _lib
 from appcorr_amd import kernels as K
-from tests.test_gpu_packed import BF, HF, attention64, gen, near, packed_case
+from tests.test_gpu_packed import (BF, HF, angles64, attention64, gen, near, norm64, norm_case, packed_case,
+                                   rotate64)
 
 pytestmark = pytest.mark.gpu
 
@@ -257,3 +258,50 @@ def test_layer_of_sequences_past_the_buffers(dev, rows, N, key_rows):
                 assert not got[r].any()
             r += 1
         assert torch.equal(kv[s, :min(n, b - a)], old[s, :min(n, b - a)]), "tokens cached before were written"
+
+
+@pytest.mark.parametrize("Hq,Hk,Dh", [(2, 1, 64), (3, 2, 128)])
+@pytest.mark.parametrize("layer", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -120, 1e-6, 2.0 ** 127])
+def test_norm_of_heads_at_the_ends_of_the_range(dev, Hq, Hk, Dh, layer, eps):
+    """Heads whose sums or squares pass fp32's largest value, or whose squares are below its smallest: bf16's largest
+    values, its subnormals, both in one head. The bound is the norm's own (1e-6 + 30 * 2^-24 of the value's size, then
+    half a step of 2^-8), and 2^-134 more: below 2^-126 bf16 values are 2^-133 apart, so that rounding one is off by up
+    to 2^-134 whatever its size, and eps = 1e-6 leaves the smallest heads there."""
+    qkv, qn, kn, pos, freq, sections, bi, ti, kv, q_out = norm_case(dev, 24, Hq, Hk, Dh, BF, layer, True, seed=66)
+    x = qkv.float()
+    sizes = [1e18, 1e19, 3e19, 1e25, 1e30, 5e37, 1e38] + [2.0 ** -e for e in (40, 50, 62, 70, 100, 126)]
+    for i, size in enumerate(sizes):
+        x[i] *= size
+    top = torch.finfo(BF).max
+    x[13] = torch.where(x[13] > 0, top, -top)
+    x[14] = torch.where(x[14] > 0, top, top / 2)     # (a sum past the range)
+    x[15, :, ::2] *= 1e30                            # half of the head negligible
+    x[16, :, 1] = 2.0 ** 120
+    x[17, :, 1:] *= 2.0 ** -110
+    x[18] = torch.where(x[18] > 0, 1.0, -1.0) * 2.0 ** -133
+    x = x.clamp(-top, top).to(BF)
+    K.qk_norm_rope_kv(x, Hq, Hk, qn, kn, eps, pos, freq, sections, bi, ti, kv, q_out, layer_norm=layer)
+    angle = angles64(pos, freq, sections)
+    half = angle.shape[1]
+    for got, heads, weights in ((q_out, x[:, :Hq], qn), (kv[bi, ti, 0], x[:, Hq:Hq + Hk], kn)):
+        y, size = norm64(heads, *weights, eps, layer)
+        ref, _ = rotate64(y, angle)
+        pair = size[..., :half] + size[..., half:2 * half]
+        slack = (1e-6 + 30 * 2.0 ** -24) * torch.cat([pair, pair, size[..., 2 * half:]], -1)
+        assert torch.isfinite(got).all()
+        assert ((got.double() - ref).abs() <= slack + 2.0 ** -8 * (ref.abs() + slack) + 2.0 ** -134).all()
+
+
+def test_norm_of_heads_that_are_not_finite(dev):
+    """As the formula has it: an infinite value makes its own quotient NaN and the others 0, a NaN all of them."""
+    qkv, qn, kn, _, freq, sections, bi, ti, kv, q_out = norm_case(dev, 4, 1, 1, 64, BF, False, False, seed=67)
+    pos = torch.zeros(4, len(sections), device=dev, dtype=torch.int64)
+    qkv[0, 0, 3] = math.inf
+    qkv[1, 0, 9] = -math.inf
+    qkv[2, 0, 11] = math.nan
+    qkv[3] = 0
+    K.qk_norm_rope_kv(qkv, 1, 1, qn, kn, 0.0, pos, freq, sections, bi, ti, kv, q_out)
+    y = q_out[:, 0].float()
+    assert y[0].isnan().sum() == 2 and y[0, 3].isnan() and y[1].isnan().sum() == 2 and y[1, 9].isnan()
+    assert (y[:2].nan_to_num() == 0).all() and y[2:].isnan().all()
