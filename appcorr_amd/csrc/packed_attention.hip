@@ -646,9 +646,9 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 // S^T per 16-key block on v_mfma_f32_16x16x32 (lane l, G = l / 16: keys 4 G + v of row l % 16), O^T per 16 dims
 // (keys 4 G + {0..3} and 16 + 4 G + {0..3} per lane, V^T by the transposing LDS read).
 // ------------------------------------------------------------------------------------------------
-template <class E, int DH, int NS, int WAVES>
+template <class E, int DH, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedAttn a) {
-  constexpr int R = 16, KEYS = 32, QK_STEPS = DH / 32, DB = DH / 16;
+  constexpr int R = 16, KEYS = 32, NS = 2, QK_STEPS = DH / 32, DB = DH / 16;
   constexpr int ROWB = 2 * DH, CPR = DH / 8, TILEB = KEYS * ROWB, RPI = 1024 / ROWB, L = KEYS / RPI;
   typedef typename E::v8 v8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -696,12 +696,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
   };
   // At most n of this wave's K or V tiles may stay in flight.
   auto wait_loads = [&](int n) __attribute__((always_inline)) {
-    static_assert((2 * NS - 1) * L < 64, "vmcnt range");
-    if (n >= 2 * NS - 1) wait_vmcnt<(2 * NS - 1) * L>();
-    else if (NS > 3 && n == 6) wait_vmcnt<6 * L>();
-    else if (NS > 3 && n == 5) wait_vmcnt<5 * L>();
-    else if (NS > 2 && n == 4) wait_vmcnt<4 * L>();
-    else if (NS > 2 && n == 3) wait_vmcnt<3 * L>();
+    static_assert(NS == 2 && 3 * L < 64, "vmcnt range");
+    if (n >= 3) wait_vmcnt<3 * L>();
     else if (n == 2) wait_vmcnt<2 * L>();
     else if (n == 1) wait_vmcnt<L>();
     else wait_vmcnt<0>();
@@ -1045,26 +1041,27 @@ static int launch_rows(const PackedAttn& a, hipStream_t st, const char* what) {
 template <class E, int DH, int WAVES>
 static int launch_keys(const PackedAttn& a, hipStream_t st, const char* what) {
   static std::atomic<uint64_t> done{0};
-  constexpr int NS = 2, lds = WAVES * 2 * NS * 32 * 2 * DH;
-  const int rc = allow_lds((const void*)packed_attn_keys_kernel<E, DH, NS, WAVES>, lds, done, what);
+  constexpr int lds = WAVES * 2 * 2 * 32 * 2 * DH;  // a wave's rings: two tiles each of K and V
+  const int rc = allow_lds((const void*)packed_attn_keys_kernel<E, DH, WAVES>, lds, done, what);
   if (rc != OUDJAT_OK) return rc;
-  packed_attn_keys_kernel<E, DH, NS, WAVES><<<(unsigned)a.items * a.Hk, WAVES * 64, lds, st>>>(a);
+  packed_attn_keys_kernel<E, DH, WAVES><<<(unsigned)a.items * a.Hk, WAVES * 64, lds, st>>>(a);
   return check_launch(what);
 }
 
 template <class E, int DH>
 static int launch_packed(const PackedAttn& a, int R, int waves, hipStream_t st, const char* what) {
+  constexpr int kHigh = DH == 128 ? 256 : 128;  // rows of the highest tile
   int rc;
   if (R == 16) {
     if constexpr (DH == 64) rc = waves == 8 ? launch_keys<E, DH, 8>(a, st, what) : launch_keys<E, DH, 4>(a, st, what);
     else rc = launch_keys<E, DH, 4>(a, st, what);
   }
-  else rc = R == 256 ? launch_rows<E, DH, 8>(a, st, what) : launch_rows<E, DH, 4>(a, st, what);
+  else rc = R == 128 ? launch_rows<E, DH, 4>(a, st, what) : launch_rows<E, DH, kHigh / 32>(a, st, what);
   if (rc != OUDJAT_OK || !a.target) return rc;
   const dim3 grid((unsigned)a.items * a.Hk, (unsigned)(R / merge_rows(R, DH)));
   if (R == 16) packed_attn_merge_kernel<E, DH, 16><<<grid, 256, 0, st>>>(a);
   else if (R == 128) packed_attn_merge_kernel<E, DH, 128><<<grid, 256, 0, st>>>(a);
-  else packed_attn_merge_kernel<E, DH, 256><<<grid, 256, 0, st>>>(a);
+  else packed_attn_merge_kernel<E, DH, kHigh><<<grid, 256, 0, st>>>(a);
   return check_launch("packed_attention (merge)");
 }
 

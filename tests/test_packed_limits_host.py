@@ -1,0 +1,22 @@
+"""CPU checks of the packed-sequence operators: the kernels that the library holds, and calls that are decided on the host."""
+
+import re
+
+from appcorr_amd import _lib
+
+
+def test_every_attention_kernel_of_the_library_is_one_that_a_call_takes():
+    """Rows kernels of 4 waves (128 rows), 8 only at Dh = 128; keys kernels of 4 waves, 8 only at Dh = 64; a merge for
+    each height of a tile."""
+    blob = _lib.LIB_PATH.read_bytes()
+
+    def instances(kernel):
+        found = re.findall(kernel.encode() + rb"INS_8Attn(Bf16|Fp16)E((?:Li\d+E)+)E", blob)
+        return {(e.decode(), *map(int, re.findall(rb"\d+", n))) for e, n in found}
+
+    def both(*shapes):
+        return {(e, *s) for e in ("Bf16", "Fp16") for s in shapes}
+
+    assert instances("packed_attn_rows_kernel") == both((64, 4), (128, 4), (128, 8))
+    assert instances("packed_attn_keys_kernel") == both((64, 4), (64, 8), (128, 4))
+    assert instances("packed_attn_merge_kernel") == both((64, 16), (64, 128), (128, 16), (128, 128), (128, 256))
