@@ -523,7 +523,9 @@ extern "C" int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t
   OUDJAT_REQUIRE(eps >= 0.0f, OUDJAT_ERR_INVALID_ARGUMENT, "%s: eps must not be negative or NaN", what);
   OUDJAT_REQUIRE(layer_norm || (!qb && !kb), OUDJAT_ERR_INVALID_ARGUMENT, "%s: a bias without layer_norm", what);
   if (rows == 0) return OUDJAT_OK;
-  OUDJAT_REQUIRE(qkv && batch_idx && token_idx && kv && q_out, OUDJAT_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  const bool empty = B == 0 || N == 0;  // a cache without slots: every row is skipped
+  OUDJAT_REQUIRE(qkv && batch_idx && token_idx && (kv || empty) && q_out, OUDJAT_ERR_INVALID_ARGUMENT,
+                 "%s: null pointer", what);
   OUDJAT_REQUIRE(Dh == 64 || Dh == 128, OUDJAT_ERR_UNSUPPORTED_SHAPE, "%s: Dh=%lld (64 or 128)", what, (long long)Dh);
   OUDJAT_REQUIRE(((x_rs | kv_bs | kv_ns | kv_cs | qo_rs) % 8) == 0 && aligned(qkv, 16) && aligned(kv, 16) &&
                      aligned(q_out, 16) && aligned(qw, 16) && aligned(qb, 16) && aligned(kw, 16) && aligned(kb, 16) &&
@@ -537,6 +539,7 @@ extern "C" int oudjat_qk_norm_rope_kv(const uint16_t* qkv, int64_t x_rs, int64_t
   const int per = rope_rows_per_wg(rows, a.half);
   OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24) && (Hq + 2 * Hk) * Dh * per < INT32_MAX, OUDJAT_ERR_TOO_LARGE,
                  "%s: too large", what);
+  if (empty) return OUDJAT_OK;
   auto go = [&](auto e, auto dh, auto layer) {
     qk_norm_rope_kv_kernel<decltype(e), decltype(dh)::value, decltype(layer)::value>
         <<<(unsigned)cdiv(rows, per), kRopeThreads, (size_t)per * 2 * a.half * 4, as_stream(stream)>>>(

@@ -2,7 +2,10 @@
 
 import re
 
+import pytest
+
 from appcorr_amd import _lib
+from tests.test_packed_refusals import NULL, norm_args, refused
 
 
 def test_every_attention_kernel_of_the_library_is_one_that_a_call_takes():
@@ -20,3 +23,14 @@ def test_every_attention_kernel_of_the_library_is_one_that_a_call_takes():
     assert instances("packed_attn_rows_kernel") == both((64, 4), (128, 4), (128, 8))
     assert instances("packed_attn_keys_kernel") == both((64, 4), (64, 8), (128, 4))
     assert instances("packed_attn_merge_kernel") == both((64, 16), (64, 128), (128, 16), (128, 128), (128, 256))
+
+
+@pytest.mark.parametrize("kw", [dict(B=0), dict(N=0), dict(B=0, N=0, kv_bs=0)])
+def test_a_cache_without_slots_skips_every_row(kw):
+    """Nothing is launched, and torch gives an empty cache no address; other arguments are checked all the same."""
+    host, args = norm_args(kv=NULL, **kw)
+    _lib.call("oudjat_qk_norm_rope_kv", *args)
+    host, args = norm_args(kv=NULL, qo_rs=0, **kw)
+    refused("OUDJAT_ERR_UNSUPPORTED_LAYOUT", "oudjat_qk_norm_rope_kv", *args)
+    host, args = norm_args(kv=NULL)
+    refused("OUDJAT_ERR_INVALID_ARGUMENT", "oudjat_qk_norm_rope_kv", *args)
