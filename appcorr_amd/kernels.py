@@ -1422,7 +1422,9 @@ def packed_plan(q_lens: torch.Tensor, k_lens: torch.Tensor, rows: int, *, cache_
 @functools.lru_cache(maxsize=64)
 def _sections(sections: tuple):
     """(host array of the sections that a call reads, their sum)."""
-    return (ctypes.c_int64 * max(1, len(sections)))(*map(int, sections)), int(sum(sections))
+    counts = [int(n) for n in sections]
+    _require(counts == list(sections), "sections must be whole numbers")
+    return (ctypes.c_int64 * max(1, len(counts)))(*counts), sum(counts)
 
 
 def _axis_rope(positions: torch.Tensor, inv_freq: torch.Tensor, sections, rows: int, what: str) -> tuple:

@@ -3,8 +3,10 @@
 import re
 
 import pytest
+import torch
 
 from appcorr_amd import _lib
+from appcorr_amd import kernels as K
 from tests.test_packed_refusals import NULL, norm_args, refused
 
 
@@ -34,3 +36,13 @@ def test_a_cache_without_slots_skips_every_row(kw):
     refused("OUDJAT_ERR_UNSUPPORTED_LAYOUT", "oudjat_qk_norm_rope_kv", *args)
     host, args = norm_args(kv=NULL)
     refused("OUDJAT_ERR_INVALID_ARGUMENT", "oudjat_qk_norm_rope_kv", *args)
+
+
+def test_sections_are_whole_numbers():
+    """Fractions were cut one by one, and inv_freq checked against their sum: (4.5, 4.5) took 9 frequencies and read 8."""
+    pos = torch.zeros(3, 2)
+    for sections, count in (((4.5, 4.5), 9), ((7.5, 8.5), 16)):
+        with pytest.raises(ValueError, match="whole numbers"):
+            K._axis_rope(pos, torch.zeros(count), sections, 3, "rope")
+    for sections in ((16, 16), [16, 16], (16.0, 16.0), torch.tensor([16, 16])):
+        assert K._axis_rope(pos, torch.zeros(32), sections, 3, "rope")[4] == 2
