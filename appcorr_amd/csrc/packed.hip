@@ -491,6 +491,8 @@ extern "C" int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, c
   AxisRope a;
   const int rc = make_axis_rope(&a, pos, pos_kind, pos_rs, pos_as, axes, inv_freq, sections, Dh, what);
   if (rc != OUDJAT_OK) return rc;
+  OUDJAT_REQUIRE(Hq == 0 || Hk == 0 || q_out != k_out, OUDJAT_ERR_INVALID_ARGUMENT,
+                 "%s: q_out and k_out are the same buffer", what);
   const int per = rope_rows_per_wg(rows, a.half);
   OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24) && (Hq + Hk) * Dh * per < INT32_MAX, OUDJAT_ERR_TOO_LARGE, "%s: too large",
                  what);

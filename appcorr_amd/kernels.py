@@ -1447,7 +1447,8 @@ def apply_rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, i
     inv_freq fp32 [sum(sections)]: dims (i, i + R/2) with R = 2 sum(sections) turn by positions[m, axis of i] *
     inv_freq[i] radians, formed in 64 bits; dims from R on stay. Position 0 leaves a row as it is (cls and
     register tokens). bf16 or fp16; q and k may be views of a qkv row with packed heads' last dim. `out` =
-    (q_out, k_out) receives the result and may be (q, k): in place; it must not overlap itself or them otherwise."""
+    (q_out, k_out) receives the result and may be (q, k): in place; it must not overlap itself (so q in place of both is
+    refused) or them otherwise."""
     qs, ks, dtype = q.shape, k.shape, q.dtype
     kind = _DTYPES.get(dtype)
     _require(len(qs) == len(ks) == 3 and qs[0] == ks[0] and qs[2] == ks[2],

@@ -766,8 +766,8 @@ int oudjat_packed_plan(const void* q_lens, int q_wide, const void* k_lens, int k
  * axes: with R / 2 the sum of `sections` (host array, one entry per axis: how many consecutive frequencies it
  * has), dims (i, i + R/2), i < R/2, of row m turn by pos[m, axis of i] * inv_freq[i] radians (formed in 64 bits);
  * dims from R on are copied. fp32 arithmetic, one rounding. pos [rows, axes] with strides pos_rs, pos_as of type
- * oudjat_pos, 1 to 4 axes. The outputs may be the inputs (in place) but not overlap them otherwise. Hq or Hk may
- * be 0. Dh % 16 == 0, Dh <= 512; R / 2 a multiple of 8; 16-byte aligned rows and heads, an output's rows and heads
+ * oudjat_pos, 1 to 4 axes. The outputs may be the inputs (in place) but not overlap them otherwise, nor one
+ * another. Hq or Hk may be 0. Dh % 16 == 0, Dh <= 512; R / 2 a multiple of 8; 16-byte aligned rows and heads, an output's rows and heads
  * apart (any order of the two strides). */
 int oudjat_rope_axes(const uint16_t* q, int64_t q_rs, int64_t q_hs, const uint16_t* k, int64_t k_rs, int64_t k_hs,
                      int64_t rows, int64_t Hq, int64_t Hk, int64_t Dh, int dtype, const void* pos, int pos_kind,

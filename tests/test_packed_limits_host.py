@@ -7,7 +7,7 @@ import torch
 
 from appcorr_amd import _lib
 from appcorr_amd import kernels as K
-from tests.test_packed_refusals import NULL, norm_args, refused
+from tests.test_packed_refusals import NULL, P16, norm_args, refused, rope_args
 
 
 def test_every_attention_kernel_of_the_library_is_one_that_a_call_takes():
@@ -46,3 +46,11 @@ def test_sections_are_whole_numbers():
             K._axis_rope(pos, torch.zeros(count), sections, 3, "rope")
     for sections in ((16, 16), [16, 16], (16.0, 16.0), torch.tensor([16, 16])):
         assert K._axis_rope(pos, torch.zeros(32), sections, 3, "rope")[4] == 2
+
+
+def test_rope_refuses_one_output_for_q_and_k():
+    """In place with q for both, say: each head would be turned by two threads, once or twice."""
+    host, args = rope_args(qo=P16, ko=P16)
+    refused("OUDJAT_ERR_INVALID_ARGUMENT", "oudjat_rope_axes", *args)
+    host, args = rope_args(rows=0, qo=P16, ko=P16)
+    _lib.call("oudjat_rope_axes", *args)
