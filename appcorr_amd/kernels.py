@@ -25,7 +25,8 @@ P = ctypes.c_void_p
 
 # Optional live timing of launch sites: every launch at a site named in `_probe["tags"]` is bracketed
 # by a pair of timing events on the launch stream (used by bench.py for the roofline). Sites are the
-# kernels' roles in the pass: "qkv", "proj", "fc1", "fc2", "w1", "w2", "w3", "attention", ...
+# kernels' roles in the pass: "qkv", "proj", "fc1", "fc2", "w1", "w2", "w3", "attention", ...; those of packed
+# sequences go by their entry points ("packed_plan", "rope_axes", "qk_norm_rope_kv", "packed_attention").
 _probe: dict = {"tags": frozenset(), "events": {}}
 
 
@@ -1508,8 +1509,8 @@ def qk_norm_rope_kv(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm, k_norm
     bi, ti = _index(batch_idx, "batch_idx"), _index(token_idx, "token_idx")
     _require(bi.shape == (M,) and ti.shape == (M,), "qk_norm_rope_kv: one slot per row")
     pos = _axis_rope(positions, inv_freq, sections, M, "qk_norm_rope_kv")
-    _launch_on("qkv_post", dev, qkv, "oudjat_qk_norm_rope_kv", qkv.data_ptr(), *_strides(qkv, 1), M, heads, kv_heads, Dh,
-               kind, layer_norm, qw.data_ptr() if qw is not None else 0,
+    _launch_on("qk_norm_rope_kv", dev, qkv, "oudjat_qk_norm_rope_kv", qkv.data_ptr(), *_strides(qkv, 1), M, heads,
+               kv_heads, Dh, kind, layer_norm, qw.data_ptr() if qw is not None else 0,
                qb.data_ptr() if qb is not None else 0, kw.data_ptr() if kw is not None else 0,
                kb.data_ptr() if kb is not None else 0, eps, *pos, bi.data_ptr(), ti.data_ptr(), kv_cache.data_ptr(),
                *_strides(kv_cache, 3), cache[0], cache[1], q_out.data_ptr(), *_strides(q_out, 1),
@@ -1564,7 +1565,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         sk, sv = _strides(k, 3), _strides(v, 3)
     else:
         sk, sv = (0, *_strides(k, 2)), (0, *_strides(v, 2))
-    _launch_on("attention", dev, q, "oudjat_packed_attention", q.data_ptr(), *_strides(q, 2), M, Hq, Dh, k.data_ptr(),
+    _launch_on("packed_attention", dev, q, "oudjat_packed_attention", q.data_ptr(), *_strides(q, 2), M, Hq, Dh, k.data_ptr(),
                *sk, v.data_ptr(), *sv, Hk, cap, batched, cu_q.data_ptr(), cu_q.dtype == torch.int64, keys.data_ptr(),
                keys.dtype == torch.int64, S, scale, causal, kind, out.data_ptr(), *_strides(out, 1),
                0 if ws is None else ws.data_ptr(), elems, _lib.stream_of(q))

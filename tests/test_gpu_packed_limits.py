@@ -305,3 +305,24 @@ def test_norm_of_heads_that_are_not_finite(dev):
     y = q_out[:, 0].float()
     assert y[0].isnan().sum() == 2 and y[0, 3].isnan() and y[1].isnan().sum() == 2 and y[1, 9].isnan()
     assert (y[:2].nan_to_num() == 0).all() and y[2:].isnan().all()
+
+
+def test_probed_sites_of_packed_sequences_are_their_own(dev):
+    """The sites of the rectangular pass ("attention", "qkv_post") do not time the packed operators."""
+    qkv, qn, kn, pos, freq, sections, bi, ti, kv, q_out = norm_case(dev, 6, 2, 1, 64, BF, False, True)
+    cu = torch.tensor([0, 6], device=dev)
+
+    def layer():
+        K.packed_plan(cu[1:], cu[1:], 6, cache_len=9)
+        K.apply_rope_axes(qkv[:, :2], qkv[:, 2:3], pos, freq, sections)
+        K.qk_norm_rope_kv(qkv, 2, 1, qn, kn, 1e-6, pos, freq, sections, bi, ti, kv, q_out)
+        K.packed_attention(q_out, kv[:1, :, 0], kv[:1, :, 1], cu, cu[1:], 0.1, causal=True)
+
+    own = ("packed_plan", "rope_axes", "qk_norm_rope_kv", "packed_attention")
+    try:
+        for tags, want in ((("attention", "qkv_post"), {}), (own, {t: 1 for t in own})):
+            K.set_probe(tags)
+            layer()
+            assert {t: len(e) for t, e in K.probe_events().items()} == want
+    finally:
+        K.set_probe(None)
