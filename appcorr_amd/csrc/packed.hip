@@ -17,8 +17,8 @@ namespace oudjat {
 // key_rows, else none, and its rows no slots.
 // Every workgroup scans all lengths for itself (at most kPlanMaxSeqs of them, read from L2, offsets in LDS) and
 // then looks its own rows up by bisection, so that the plan is one launch and no workgroup waits for another.
-// Bound by that scan's latency: a thread reads its lengths eight at a time (once, up to 2048 sequences), scans within
-// its wave by lane shuffles and across waves through LDS.
+// Bound by that scan's latency: a thread reads its lengths eight at a time, scans within its wave by lane
+// shuffles and across waves through LDS.
 // ------------------------------------------------------------------------------------------------
 static constexpr int kPlanThreads = 256;
 static constexpr int kPlanMaxSeqs = 4096;     // 2 x 16 KB of LDS
@@ -64,75 +64,82 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(
   int32_t* ends = plan_lds;         // c_{s+1}
   int32_t* toks = plan_lds + S;     // first_s - c_s: token of row r is toks[s] + r; INT32_MIN: no row has a slot
   __shared__ int64_t wave_sums[kPlanThreads / 64];
-  __shared__ int32_t last_fit;      // packed keys: the key rows up to the last sequence that fits
+  __shared__ int32_t last_fit;      // packed keys: the key rows before the first sequence that does not fit
   const int tid = threadIdx.x;
   const int per = (S + kPlanThreads - 1) / kPlanThreads;
   const int s0 = min(tid * per, S), s1 = min(s0 + per, S);
-  int64_t ql[8], kl[8];  // lengths of sequences s .. s + 7
-  auto load = [&](int s) {
+  int64_t nq = 0, nk = 0, total, a[8], b[8];
+  auto load = [&](int s) {  // lengths of sequences s .. s + 7
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = min(s + e, S - 1);
-      ql[e] = load_len(q_lens, i, q_wide);
-      kl[e] = load_len(k_lens, i, k_wide);
+      a[e] = load_len(q_lens, i, q_wide);
+      b[e] = load_len(k_lens, i, k_wide);
     }
   };
-  int64_t cq = 0, ck = 0, total;
-  // This thread's sequences in turn: f(sequence, its rows' begin and end, token of its first
-  // row, its keys n).
-  auto each = [&](int64_t q0, auto&& f) {
-    for (int s = s0; s < s1; s += 8) {
-      if (per > 8) load(s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (s + e < s1) {
-          const int64_t begin = min(q0, rows);
-          q0 += clamp_len(ql[e], rows);
-          const int64_t end = min(q0, rows), first = max(kl[e], (int64_t)0) - max(ql[e], (int64_t)0);
-          f(s + e, (int32_t)begin, (int32_t)end, first, max(first + end - begin, (int64_t)0));
-        }
-    }
-  };
-  if (s0 < s1 && per <= 8) load(s0);
-  int64_t nq = 0, nk = 0;
   for (int s = s0; s < s1; s += 8) {
-    if (per > 8) load(s);
+    load(s);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (s + e < s1) nq += clamp_len(ql[e], rows);
+      if (s + e < s1) nq += clamp_len(a[e], rows);
   }
-  cq = block_scan(nq, wave_sums, &total);
-  // Keys of a sequence in the running sum: what the cache holds of them, or all (one that does not fit is past the end).
-  auto held = [&](int64_t n) { return packed_keys ? min(n, key_cap + 1) : min(n, key_cap); };
-  each(cq, [&](int, int32_t, int32_t, int64_t, int64_t n) { nk += held(n); });
-  if (tid == 0) last_fit = 0;
-  ck = block_scan(nk, wave_sums, &total);
-  const bool writer = blockIdx.x == 0;  // the per-sequence results are written once
-  int64_t ke = ck;
-  each(cq, [&](int s, int32_t begin, int32_t end, int64_t first, int64_t n) {
-    ke += held(n);
-    const bool fits = !packed_keys || ke <= key_cap;
-    ends[s] = end;
-    toks[s] = n > 0 && first < key_cap && fits ? (int32_t)(first - begin) : INT32_MIN;  // (n > 0: first > -end)
-    if (writer) {
-      cu_q[s + 1] = end;
-      k_out[s] = fits ? (int32_t)min(n, (int64_t)INT32_MAX) : 0;
-      if (fits) cu_k[s + 1] = ke;
-      if (packed_keys && fits) atomicMax(&last_fit, (int32_t)ke);
+  int64_t cq = block_scan(nq, wave_sums, &total);
+  const int begin0 = (int)min(cq, rows);
+  auto keys = [&](int64_t q, int64_t k, int64_t kept) {  // n_s
+    return max(max(k, (int64_t)0) - max(q, (int64_t)0) + kept, (int64_t)0);
+  };
+  // n_s in the running sum: what a cache holds of them, or (packed) all, as far as it matters that they do not fit.
+  const int64_t most = packed_keys ? key_cap + 1 : key_cap;
+  auto take = [&](int s, int64_t q, int64_t k) {
+    const int64_t begin = min(cq, rows);
+    cq += clamp_len(q, rows);
+    const int64_t end = min(cq, rows), n = keys(q, k, end - begin), first = n - (end - begin);
+    nk += min(n, most);
+    ends[s] = (int32_t)end;
+    toks[s] = n > 0 && first < key_cap ? (int32_t)(first - begin) : INT32_MIN;  // (n > 0: first > -end)
+  };
+  if (per == 1) {  // up to 256 sequences
+    if (s0 < s1) take(s0, a[0], b[0]);
+  } else {
+    for (int s = s0; s < s1; s += 8) {
+      load(s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (s + e < s1) take(s + e, a[e], b[e]);
     }
-  });
-  if (writer && tid == 0) {
-    cu_q[0] = 0;
-    cu_k[0] = 0;
+  }
+  int64_t ck = block_scan(nk, wave_sums, &total);
+  const bool writer = blockIdx.x == 0;  // the per-sequence results are written once
+  int past = s1;                        // packed keys: this thread's first sequence that does not fit
+  if (packed_keys || writer) {
+    int begin = begin0;
+    for (int s = s0; s < s1; ++s) {
+      const int end = ends[s], t = toks[s];
+      const int64_t n = t != INT32_MIN ? (int64_t)t + end
+                                       : keys(load_len(q_lens, s, q_wide), load_len(k_lens, s, k_wide), end - begin);
+      const int64_t before = ck;
+      begin = end;
+      ck += min(n, most);
+      const bool fits = !packed_keys || ck <= key_cap;
+      if (!fits) {
+        toks[s] = INT32_MIN;
+        past = min(past, s);
+        if (before <= key_cap) last_fit = (int32_t)before;  // (one sequence of all)
+      }
+      if (writer) {
+        cu_q[s + 1] = end;
+        k_out[s] = fits ? (int32_t)min(n, (int64_t)INT32_MAX) : 0;
+        if (fits) cu_k[s + 1] = ck;
+      }
+    }
+    if (writer && tid == 0) {
+      cu_q[0] = 0;
+      cu_k[0] = 0;
+    }
   }
   __syncthreads();
-  if (writer && packed_keys) {
-    ke = ck;
-    each(cq, [&](int s, int32_t, int32_t, int64_t, int64_t n) {
-      ke += held(n);
-      if (ke > key_cap) cu_k[s + 1] = last_fit;
-    });
-  }
+  if (writer)
+    for (int s = past; s < s1; ++s) cu_k[s + 1] = last_fit;
   const int64_t r0 = ((int64_t)blockIdx.x * kPlanThreads + tid) * kPlanRowsPerThread;
   if (r0 >= rows) return;
   int64_t bi[kPlanRowsPerThread], ti[kPlanRowsPerThread];
