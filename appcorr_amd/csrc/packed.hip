@@ -299,8 +299,9 @@ __global__ __launch_bounds__(kRopeThreads) void rope_axes_kernel(
 // RMS: y = x / sqrt(mean(x^2) + eps) * w;  LayerNorm: the same of x - mean(x), plus b. Then the rotation, then one
 // rounding to the type; values are copied. Dh / 16 lanes hold a head, 16 dims each (as above), so that its sums
 // are two to three lane exchanges, and a thread keeps the weights of its dims for all heads it takes. A row whose
-// slot lies outside the cache is skipped. Bound by HBM: 16404 rows, 32 + 2 x 8 heads of 128, 398 MB, 83.7 us
-// (4.75 TB/s); one token of 32 streams 4.8 us, a launch and two dependent rounds of loads.
+// slot lies outside the cache is skipped. Bound by HBM: 16404 rows, 32 + 2 x 8 heads of 128, 398 MB, 81.8 us
+// (4.87 TB/s); one token of 32 streams 4.7 us, a launch and two dependent rounds of loads; the branch for heads out of
+// fp32's range costs 0.1 us of it.
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, bool LAYER>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kv_kernel(

@@ -5,7 +5,9 @@
 //   out = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c (q . k_j) - c mu),  c = scale log2 e,
 // with an online softmax: mu is a reference that follows the running maximum, and sum and output are rescaled when it
 // moves. Scores, statistics and outputs are fp32; the p_j are rounded to the element type for the second product, and
-// the sum is of the rounded values, so that numerator and normaliser use the same weights.
+// the sum is of the rounded values, so that numerator and normaliser use the same weights. The matrix cores take 16-bit
+// operands; a second product for the remainders would add half of a tile's matrix work for an error against 64 bits of
+// 0.0016 instead of 0.0020 to 0.0023 (bf16, of the outputs' size; 0.0016 is the rounding of the output).
 //
 // The G query heads of a key head are packed into the query rows: packed row r of a sequence is token r / G, head
 // r % G of the group, so that one pass over a key head's K and V serves the whole group, a single token fills G rows
@@ -22,8 +24,10 @@
 //
 // Two kernels. packed_attn_rows: R = 32 W rows, a wave owns 32, all waves of the workgroup share K/V tiles of 64 keys.
 // packed_attn_keys, for few rows: R = 16, the waves share the rows and take 32 keys each in turn. Measured:
-// prompts of up to 16384 tokens, 32 over 8 heads of 128, 3.36 ms (1020 TF/s; a 16384^3 product of the library 1360);
-// 32 tokens over caches of up to 16385 keys 155 us (5.0 TB/s); 24 crops of up to 1029 tokens, 16 heads of 64, 44 us.
+// prompts of up to 16384 tokens, 32 over 8 heads of 128, 3.32 to 3.52 ms by the card (977 to 1040 TF/s; a 16384^3 product
+// of the library 1360); 32 tokens over caches of up to 16385 keys 155 us (5.0 TB/s); 24 crops of up to 1029 tokens, 16
+// heads of 64, 43 us on a GPU that is busy, 47 on one that was idle. The steps' figures below were taken one against the
+// other on one card.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -984,6 +988,8 @@ struct PackedShape {
 //   keys, 8 key heads: 19.2, two per CU 24.7.
 // search (above): 256 tokens over 200 keys 17 by search, 26 by scan; 128 over up to 4 k keys 139 by search, 126 by scan.
 // min_tiles: 6 x 100 rows over 3 k keys: 15.5 from 6, 20.8 from 12; 2 x 16 rows over 2 k keys: 9.8 from 2, 11.3 from 4.
+// All go by the row buffer and the number of sequences, the host's upper bounds: single tokens in a buffer much longer
+// than their number run on the rows kernel unsplit (32 tokens over up to 16 k keys 135 us, in 2048 rows 266).
 static PackedShape packed_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh, int64_t key_cap) {
   PackedShape s{};
   const int64_t G = Hq / Hk, seqs = std::max<int64_t>(1, std::min(S, rows));
