@@ -223,7 +223,10 @@ def call(name: str, *args) -> None:
 def stream_of(t: torch.Tensor) -> int:
     """Raw hipStream_t of torch's current stream on the tensor's device (without the Stream object that
     torch.cuda.current_stream builds, 2 us of a call)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    dev = t.get_device()
+    if dev < 0:  # (which torch would take for the current device)
+        raise ValueError(f"expected a GPU tensor, got one on {t.device}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def verify_runtime(device: torch.device | int | None = None) -> bool:

@@ -54,3 +54,9 @@ def test_rope_refuses_one_output_for_q_and_k():
     refused("OUDJAT_ERR_INVALID_ARGUMENT", "oudjat_rope_axes", *args)
     host, args = rope_args(rows=0, qo=P16, ko=P16)
     _lib.call("oudjat_rope_axes", *args)
+
+
+def test_a_cpu_tensor_has_no_stream():
+    """Its device index, -1, is the current device to torch: a launch with the tensor's address would follow."""
+    with pytest.raises(ValueError, match="GPU tensor"):
+        _lib.stream_of(torch.zeros(1))
