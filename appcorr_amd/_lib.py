@@ -17,7 +17,7 @@ from pathlib import Path
 import torch  # noqa: F401  -- must be loaded before the HIP library, see module docstring
 
 LIB_PATH = Path(__file__).resolve().parent / "liboudjat_hip.so"
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 OK = 0
 STATUS_NAMES = {
@@ -169,6 +169,16 @@ SIGNATURES: dict[str, list] = {
     "oudjat_packed_attention": [_p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64,
                                 _i64, _i32, _p, _i32, _p, _i32, _i64, _f32, _i32, _i32, _p, _i64, _p, _i64, _p],
     "oudjat_packed_attention_workspace_elems": [_i64, _i64, _i64, _i64, _i64, _i64],
+    "oudjat_quantize_int8": [_p, _i64, _i64, _i64, _i32, _p, _i64, _p, _p],
+    "oudjat_linear_int8": [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i32, _p],
+    "oudjat_kv_nvfp4_write": [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _i64, _i64, _i64,
+                              _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p],
+    "oudjat_kv_nvfp4_read": [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p,
+                             _i64, _i32, _p, _p, _p],
+    "oudjat_packed_attention_nvfp4": [_p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                                      _i64, _p, _i64, _i64, _p, _i32, _p, _i32, _i64, _f32, _i32, _i32, _p, _i64, _p,
+                                      _i64, _p],
+    "oudjat_packed_attention_nvfp4_workspace_elems": [_i64, _i64, _i64, _i64, _i64, _i64],
     "oudjat_query_attention_prob_noalloc": [_p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _p,
                                             _i64, _i32, _p],
 }
@@ -176,6 +186,7 @@ _RESTYPES = {"oudjat_status_string": ctypes.c_char_p, "oudjat_last_error": ctype
              "oudjat_linear_workspace_elems": ctypes.c_int64, "oudjat_linear_warm_slots": ctypes.c_int64,
              "oudjat_sparse_query_attention_workspace_elems": ctypes.c_int64,
              "oudjat_packed_attention_workspace_elems": ctypes.c_int64,
+             "oudjat_packed_attention_nvfp4_workspace_elems": ctypes.c_int64,
              "oudjat_patch_attention_prob_workspace_elems": ctypes.c_int64}
 
 _lock = threading.Lock()

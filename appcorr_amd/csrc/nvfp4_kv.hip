@@ -1,0 +1,186 @@
+// K/V caches in NVFP4: rows of keys and values written into one, and rows of it read back in 16 bits.
+//
+// A block is 16 consecutive dims of one head of one token. With h the head's tensor scale (fp32, one each for keys and
+// values), a = max |x| over the block:
+//   s8 = e4m3(clamp((a / 6) / h, 2^-16, 448)),   code_i = e2m1(x_i / (h s8)),   value_i = e2m1(code_i) e4m3(s8) h,
+// the element arithmetic of nvfp4.hpp (IEEE quotients, nearest even, saturating). A block whose scale rounds to 0 holds
+// zeros; a NaN counts as 0 and an infinity as the largest value, for which the format has nothing else: what a cache
+// holds is finite. Element 2i lies in the low nibble of byte i. The scale bytes are read without their sign bit, and
+// 0x7f (never written) as 480, so that memory that nobody has written cannot give a NaN either.
+#include <algorithm>
+
+#include "elem.hpp"
+#include "nvfp4_kv.hpp"
+
+namespace oudjat {
+
+static constexpr int kKvThreads = 256;
+
+// Write. An item is half a block, 8 dims (16 bytes in, 4 out): the wave reads and writes consecutive pieces of a row, the
+// two lanes of a block exchange their maxima, and one lane in eight stores four scales. A workgroup takes `per_wg`
+// rows.
+template <class E>
+__global__ __launch_bounds__(kKvThreads) void kv_nvfp4_write_kernel(
+    const uint16_t* __restrict__ k, int64_t k_rs, int64_t k_hs, const uint16_t* __restrict__ v, int64_t v_rs,
+    int64_t v_hs, int64_t rows, int dims8, Divisor by_row, Divisor by_head, const int64_t* __restrict__ batch_idx,
+    const int64_t* __restrict__ token_idx, KvNvfp4 c, int per_wg) {
+  const int64_t row0 = (int64_t)blockIdx.x * per_wg;
+  const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * dims8;
+  for (int i = threadIdx.x; i < n * per_row; i += kKvThreads) {
+    const int r = by_row(i), j = i - r * per_row;
+    const int kh = by_head(j), d8 = j - kh * dims8;  // key heads, then value heads; 8 dims
+    const bool val = kh >= c.Hk;
+    const int h = val ? kh - c.Hk : kh;
+    const int64_t row = row0 + r;
+    float f[8];
+    E::to8(load16((val ? v + row * v_rs + h * v_hs : k + row * k_rs + h * k_hs) + 8 * d8), f);
+    const int64_t b = batch_idx[row], t = token_idx[row];
+    const float ts = c.ts[kh];
+    float am = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[e] = f[e] == f[e] ? f[e] : 0.0f;
+      am = fmaxf(am, fabsf(f[e]));
+    }
+    am = fmaxf(am, __shfl_xor(am, 1, 64));
+    uint32_t s8;
+    float unit;
+    nvfp4_block_scale(am, ts, s8, unit);
+    // (values past 8 units saturate all the same, and their quotients stay finite)
+    const float most = 8.0f * unit;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fminf(fmaxf(f[e], -most), most);
+    const uint32_t word = s8 ? nvfp4_codes8(f, unit, 1.0f / unit) : 0u;
+    // Four blocks' scales into one word: lanes 8 apart hold those of the next four.
+    uint32_t four = s8 << (8 * ((d8 >> 1) & 3));
+    four |= __shfl_xor(four, 2, 64);
+    four |= __shfl_xor(four, 4, 64);
+    if (b < 0 || b >= c.B || t < 0 || t >= c.N) continue;
+    *reinterpret_cast<uint32_t*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 4 * d8) = word;
+    if ((d8 & 7) == 0)
+      *reinterpret_cast<uint32_t*>(c.scales + b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d8 / 2) = four;
+  }
+}
+
+// Read. An item is 8 dims: 4 bytes of codes and a scale byte in, 16 bytes out.
+template <class E>
+__global__ __launch_bounds__(kKvThreads) void kv_nvfp4_read_kernel(KvNvfp4 c, int dims8, Divisor by_row, Divisor by_head,
+                                                                   const int64_t* __restrict__ batch_idx,
+                                                                   const int64_t* __restrict__ token_idx, int64_t rows,
+                                                                   uint16_t* __restrict__ k_out,
+                                                                   uint16_t* __restrict__ v_out, int per_wg) {
+  const int64_t row0 = (int64_t)blockIdx.x * per_wg;
+  const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * dims8;
+  for (int i = threadIdx.x; i < n * per_row; i += kKvThreads) {
+    const int r = by_row(i), j = i - r * per_row;
+    const int kh = by_head(j), d8 = j - kh * dims8;
+    const bool val = kh >= c.Hk;
+    const int h = val ? kh - c.Hk : kh;
+    const int64_t row = row0 + r, b = batch_idx[row], t = token_idx[row];
+    float f[8] = {};
+    if (b >= 0 && b < c.B && t >= 0 && t < c.N) {
+      const uint32_t w =
+          *reinterpret_cast<const uint32_t*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 4 * d8);
+      const uint32_t s8 = c.scales[b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d8 / 2];
+      const float s = e4m3_decode(s8 & 0x7f), ts = c.ts[kh];
+      const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
+      const auto v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+      const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2);
+      const auto v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+      const float e2[8] = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = (e2[e] * s) * ts;  // (the first product is exact)
+    }
+    store16((val ? v_out : k_out) + (row * c.Hk + h) * (8 * dims8) + 8 * d8, E::from8(f));
+  }
+}
+
+// Rows of a workgroup: about 1024 items, four a thread.
+static int kv_rows_per_wg(int64_t per_row) { return (int)std::max<int64_t>(1, 1024 / per_row); }
+
+int check_kv_nvfp4(const KvNvfp4& c, int64_t Dh, const char* what) {
+  OUDJAT_REQUIRE(c.bs >= 0 && c.ns >= 0 && c.cs >= 0 && c.hs >= 0 && c.sbs >= 0 && c.sns >= 0 && c.scs >= 0 && c.shs >= 0,
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: negative stride", what);
+  OUDJAT_REQUIRE(((c.bs | c.ns | c.cs | c.hs) % 16) == 0 && ((c.sbs | c.sns | c.scs | c.shs) % (Dh / 16)) == 0 &&
+                     aligned(c.codes, 16) && aligned(c.scales, Dh / 16) && aligned(c.ts, 4),
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: a head's codes must be 16-byte aligned, its scales by their own size",
+                 what);
+  return OUDJAT_OK;
+}
+
+}  // namespace oudjat
+
+using namespace oudjat;
+
+extern "C" int oudjat_kv_nvfp4_write(const uint16_t* k, int64_t k_rs, int64_t k_hs, const uint16_t* v, int64_t v_rs,
+                                     int64_t v_hs, int64_t rows, int64_t Hk, int64_t Dh, int dtype,
+                                     const int64_t* batch_idx, const int64_t* token_idx, uint8_t* codes, int64_t c_bs,
+                                     int64_t c_ns, int64_t c_cs, int64_t c_hs, uint8_t* scales, int64_t s_bs,
+                                     int64_t s_ns, int64_t s_cs, int64_t s_hs, const float* tensor_scale, int64_t B,
+                                     int64_t N, oudjat_stream_t stream) {
+  const char* what = "kv_nvfp4_write";
+  OUDJAT_REQUIRE(rows >= 0 && Hk > 0 && Dh > 0 && B >= 0 && N >= 0, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad size", what);
+  OUDJAT_REQUIRE(dtype == OUDJAT_BF16 || dtype == OUDJAT_FP16, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad element type %d",
+                 what, dtype);
+  OUDJAT_REQUIRE(Dh == 64 || Dh == 128, OUDJAT_ERR_UNSUPPORTED_SHAPE, "%s: Dh=%lld (64 or 128)", what, (long long)Dh);
+  OUDJAT_REQUIRE(Hk <= 65535, OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
+  if (rows == 0) return OUDJAT_OK;
+  const bool empty = B == 0 || N == 0;  // a cache without slots: every row is skipped
+  OUDJAT_REQUIRE(k && v && batch_idx && token_idx && ((codes && scales) || empty) && tensor_scale,
+                 OUDJAT_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  OUDJAT_REQUIRE(k_rs >= 0 && k_hs >= 0 && v_rs >= 0 && v_hs >= 0 && ((k_rs | k_hs | v_rs | v_hs) % 8) == 0 &&
+                     aligned(k, 16) && aligned(v, 16) && aligned(batch_idx, 8) && aligned(token_idx, 8),
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned rows and heads of k and v required", what);
+  const KvNvfp4 c{codes, c_bs, c_ns, c_cs, c_hs, scales, s_bs, s_ns, s_cs, s_hs, tensor_scale, B, N, (int)Hk};
+  const int rc = check_kv_nvfp4(c, Dh, what);
+  if (rc != OUDJAT_OK) return rc;
+  OUDJAT_REQUIRE(entries_apart({{B, c_bs}, {N, c_ns}, {2, c_cs}, {Hk, c_hs}}, Dh / 2) &&
+                     entries_apart({{B, s_bs}, {N, s_ns}, {2, s_cs}, {Hk, s_hs}}, Dh / 16),
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: the rows of the cache must not overlap", what);
+  const int64_t per_row = 2 * Hk * Dh / 8;
+  const int per = kv_rows_per_wg(per_row);
+  OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
+  if (empty) return OUDJAT_OK;
+  auto go = [&](auto e) {
+    kv_nvfp4_write_kernel<decltype(e)><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
+        k, k_rs, k_hs, v, v_rs, v_hs, rows, (int)(Dh / 8), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 8)),
+        batch_idx, token_idx, c, per);
+  };
+  if (dtype == OUDJAT_BF16) go(ElemBf16{});
+  else go(ElemFp16{});
+  return check_launch(what);
+}
+
+extern "C" int oudjat_kv_nvfp4_read(const uint8_t* codes, int64_t c_bs, int64_t c_ns, int64_t c_cs, int64_t c_hs,
+                                    const uint8_t* scales, int64_t s_bs, int64_t s_ns, int64_t s_cs, int64_t s_hs,
+                                    const float* tensor_scale, int64_t B, int64_t N, int64_t Hk, int64_t Dh,
+                                    const int64_t* batch_idx, const int64_t* token_idx, int64_t rows, int dtype,
+                                    uint16_t* k_out, uint16_t* v_out, oudjat_stream_t stream) {
+  const char* what = "kv_nvfp4_read";
+  OUDJAT_REQUIRE(rows >= 0 && Hk > 0 && Dh > 0 && B >= 0 && N >= 0, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad size", what);
+  OUDJAT_REQUIRE(dtype == OUDJAT_BF16 || dtype == OUDJAT_FP16, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad element type %d",
+                 what, dtype);
+  OUDJAT_REQUIRE(Dh == 64 || Dh == 128, OUDJAT_ERR_UNSUPPORTED_SHAPE, "%s: Dh=%lld (64 or 128)", what, (long long)Dh);
+  OUDJAT_REQUIRE(Hk <= 65535, OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
+  if (rows == 0) return OUDJAT_OK;
+  OUDJAT_REQUIRE(batch_idx && token_idx && ((codes && scales) || B == 0 || N == 0) && tensor_scale && k_out && v_out,
+                 OUDJAT_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  OUDJAT_REQUIRE(k_out != v_out, OUDJAT_ERR_INVALID_ARGUMENT, "%s: k_out and v_out are the same buffer", what);
+  const KvNvfp4 c{const_cast<uint8_t*>(codes), c_bs, c_ns, c_cs, c_hs, const_cast<uint8_t*>(scales), s_bs, s_ns, s_cs,
+                  s_hs, tensor_scale, B, N, (int)Hk};
+  const int rc = check_kv_nvfp4(c, Dh, what);
+  if (rc != OUDJAT_OK) return rc;
+  OUDJAT_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16) && aligned(batch_idx, 8) && aligned(token_idx, 8),
+                 OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned outputs required", what);
+  const int64_t per_row = 2 * Hk * Dh / 8;
+  const int per = kv_rows_per_wg(per_row);
+  OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
+  auto go = [&](auto e) {
+    kv_nvfp4_read_kernel<decltype(e)><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
+        c, (int)(Dh / 8), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 8)), batch_idx, token_idx, rows, k_out,
+        v_out, per);
+  };
+  if (dtype == OUDJAT_BF16) go(ElemBf16{});
+  else go(ElemFp16{});
+  return check_launch(what);
+}

@@ -1570,3 +1570,183 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
                keys.dtype == torch.int64, S, scale, causal, kind, out.data_ptr(), *_strides(out, 1),
                0 if ws is None else ws.data_ptr(), elems, _lib.stream_of(q))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# A layer of packed sequences in 8 and 4 bits: INT8 products with token and channel scales, NVFP4 K/V caches
+# (no counterpart in the reference)
+# ------------------------------------------------------------------------------------------------
+
+
+def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of x [.., K] (bf16 or fp16) as (int8 codes [.., K], fp32 scales [..]): scale = max |x| / 127 of the row, code =
+    x / scale to the nearest whole number (ties to even; 0 where the scale is 0). A row with a NaN or an infinity gets
+    scale NaN and codes 0, so that its products are NaN. The activations of linear_int8, or its weight [N, K] (a scale for
+    each output channel). K a multiple of 16, rows contiguous and 16-byte aligned."""
+    dev = _gpu_of(x)
+    kind = _DTYPES.get(x.dtype)
+    _require(kind is not None and x.dim() >= 1, "quantize_int8: [.., K] bf16 or fp16")
+    K = x.shape[-1]
+    _require(x.stride(-1) == 1 or K <= 1, "quantize_int8: rows must be contiguous")
+    codes = torch.empty(x.shape, device=x.device, dtype=torch.int8)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    rows = scale.numel()
+    if rows:
+        x2 = x.reshape(rows, K)
+        _launch_on("quantize_int8", dev, x, "oudjat_quantize_int8", x2.data_ptr(), rows, K, *_strides(x2, 1), kind,
+                   codes.data_ptr(), K, scale.data_ptr(), _lib.stream_of(x))
+    return codes, scale
+
+
+def linear_int8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor,
+                bias: torch.Tensor | None = None, *, epilogue: int = _lib.EPI_BIAS, gamma: torch.Tensor | None = None,
+                resid: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                dtype: torch.dtype = torch.bfloat16, site: str = "linear_int8") -> torch.Tensor:
+    """y = (x8 . w8^T) * x_scale[row] * w_scale[column] + bias of int8 codes x8 [.., K] and w8 [N, K] (quantize_int8's), the
+    sums exact, then the epilogue in fp32 and one rounding to `dtype` (bf16 or fp16): EPI_BIAS, EPI_BIAS_LS (y * gamma),
+    EPI_BIAS_LS_RESID (resid + y * gamma), EPI_BIAS_SILU_MUL (silu(y) * resid). bias, gamma [N] and resid [.., N] of that
+    type; `out` may be resid but not overlap itself. K a multiple of 64 below 131072, N of 8."""
+    dev = _gpu_of(x8, x_scale, w8, w_scale, bias, gamma, resid, out)
+    kind = _DTYPES.get(dtype)
+    _require(kind is not None, "linear_int8: dtype must be bf16 or fp16")
+    _require(x8.dtype == w8.dtype == torch.int8 and x8.dim() >= 1 and w8.dim() == 2 and w8.shape[1] == x8.shape[-1],
+             "linear_int8: int8 codes x8 [.., K] and w8 [N, K]")
+    N, Kd = w8.shape
+    _require(x_scale.shape == x8.shape[:-1] and w_scale.shape == (N,) and x_scale.dtype == w_scale.dtype == torch.float32,
+             "linear_int8: fp32 scales x_scale [..] and w_scale [N]")
+    M = x_scale.numel()
+    x2 = x8.reshape(M, Kd)
+    _require((x2.stride(1) == 1 and w8.stride(1) == 1) or Kd <= 1, "linear_int8: rows must be contiguous")
+    for t, name in ((bias, "bias"), (gamma, "gamma")):
+        _require(t is None or (t.shape == (N,) and t.dtype == dtype), f"linear_int8: {name} must be [N] of the output's type")
+    shape = (*x8.shape[:-1], N)
+    for t, name in ((resid, "resid"), (out, "out")):
+        _require(t is None or (t.shape == shape and t.dtype == dtype and (t.stride(-1) == 1 or N <= 1)),
+                 f"linear_int8: {name} must be [.., N] of the output's type with contiguous rows")
+    if out is None:
+        out = torch.empty(shape, device=x8.device, dtype=dtype)
+    o2 = out.view(M, N)
+    r2 = None if resid is None else resid.reshape(M, N)
+    sx, sw = x_scale.contiguous(), w_scale.contiguous()
+    b = None if bias is None else bias.contiguous()
+    g = None if gamma is None else gamma.contiguous()
+    _launch_on(site, dev, x8, "oudjat_linear_int8", x2.data_ptr(), M, Kd, *_strides(x2, 1), sx.data_ptr(), w8.data_ptr(), N,
+               *_strides(w8, 1), sw.data_ptr(), 0 if b is None else b.data_ptr(), int(epilogue),
+               0 if g is None else g.data_ptr(), 0 if r2 is None else r2.data_ptr(),
+               0 if r2 is None else _strides(r2, 1)[0], o2.data_ptr(), *_strides(o2, 1), kind, _lib.stream_of(x8))
+    return out
+
+
+@dataclass
+class KvNvfp4:
+    """A K/V cache in NVFP4: codes uint8 [B, N, 2, Hk, Dh / 2] (keys, then values; two e2m1 codes a byte, the even dim in
+    the low nibble), scales float8_e4m3fn [B, N, 2, Hk, Dh / 16] (one for 16 dims), tensor_scale fp32 [2, Hk] (positive):
+    value = e2m1 * scale * tensor_scale. Any strides, the last dim contiguous and a head's codes 16-byte aligned (its scales
+    by their own size); kv_nvfp4_cache lays a head's tokens side by side, which the attention reads fastest."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    tensor_scale: torch.Tensor
+
+
+def kv_nvfp4_cache(batches: int, cache_len: int, kv_heads: int, head_dim: int, device, *,
+                   tensor_scale: torch.Tensor | float = 1.0 / 448) -> KvNvfp4:
+    """An empty cache. tensor_scale: fp32 [2, kv_heads] or a number for all: max |x| / (448 * 6) of calibrated keys and
+    values uses all of the format; values past 2688 tensor scales saturate. The default takes values up to 6."""
+    codes = torch.zeros((batches, 2, kv_heads, cache_len, head_dim // 2), device=device, dtype=torch.uint8)
+    scales = torch.zeros((batches, 2, kv_heads, cache_len, head_dim // 16), device=device, dtype=torch.uint8)
+    if not isinstance(tensor_scale, torch.Tensor):
+        tensor_scale = torch.full((2, kv_heads), tensor_scale, device=device, dtype=torch.float32)
+    return KvNvfp4(codes.permute(0, 3, 1, 2, 4), scales.view(torch.float8_e4m3fn).permute(0, 3, 1, 2, 4), tensor_scale)
+
+
+def _kv_nvfp4_args(cache: KvNvfp4, Hk: int, Dh: int, what: str) -> tuple:
+    """(addresses and strides as the C entries take them) of a cache of Hk heads of Dh."""
+    codes, scales, ts = cache.codes, cache.scales, cache.tensor_scale
+    cs, ss = codes.shape, scales.shape
+    _require(len(cs) == 5 and cs == (cs[0], cs[1], 2, Hk, Dh // 2) and ss == (cs[0], cs[1], 2, Hk, Dh // 16)
+             and codes.dtype == torch.uint8 and scales.dtype in (torch.float8_e4m3fn, torch.uint8)
+             and codes.stride(4) == 1 and scales.stride(4) == 1,
+             f"{what}: the cache must be codes uint8 [B, N, 2, Hk, Dh / 2] and scales e4m3 [B, N, 2, Hk, Dh / 16]")
+    _require(ts.shape == (2, Hk) and ts.dtype == torch.float32 and ts.is_contiguous(),
+             f"{what}: tensor_scale must be contiguous fp32 [2, Hk]")
+    return (codes.data_ptr(), *_strides(codes, 4), scales.data_ptr(), *_strides(scales, 4), ts.data_ptr())
+
+
+def kv_nvfp4_write(k: torch.Tensor, v: torch.Tensor, batch_idx: torch.Tensor, token_idx: torch.Tensor,
+                   cache: KvNvfp4) -> None:
+    """k, v [M, Hk, Dh] (bf16 or fp16, views of a qkv row for instance) into the cache at (batch_idx, token_idx).
+
+    A block of 16 dims has the scale e4m3(max |x| / 6 / tensor_scale) and the nearest e2m1 values of x / (tensor_scale *
+    scale), ties to even, saturating. NaN is stored as 0, an infinity as the largest value. Rows with a slot outside the cache (packed_plan's
+    -1) are skipped; the other rows' slots must be unique. The cache must not overlap itself (expanded) or k and v. Dh
+    64 or 128."""
+    shape, kind = k.shape, _DTYPES.get(k.dtype)
+    _require(len(shape) == 3 and v.shape == shape and kind is not None and v.dtype == k.dtype and k.stride(2) == 1
+             and v.stride(2) == 1, "kv_nvfp4_write: k and v [M, Hk, Dh] bf16 or fp16 with contiguous heads")
+    dev = _gpu_of(k, v, batch_idx, token_idx, cache.codes, cache.scales, cache.tensor_scale)
+    M, Hk, Dh = shape
+    bi, ti = _index(batch_idx, "batch_idx"), _index(token_idx, "token_idx")
+    _require(bi.shape == (M,) and ti.shape == (M,), "kv_nvfp4_write: one slot per row")
+    c = _kv_nvfp4_args(cache, Hk, Dh, "kv_nvfp4_write")
+    _launch_on("kv_nvfp4_write", dev, k, "oudjat_kv_nvfp4_write", k.data_ptr(), *_strides(k, 2), v.data_ptr(),
+               *_strides(v, 2), M, Hk, Dh, kind, bi.data_ptr(), ti.data_ptr(), *c, *cache.codes.shape[:2],
+               _lib.stream_of(k))
+
+
+def kv_nvfp4_read(cache: KvNvfp4, batch_idx: torch.Tensor, token_idx: torch.Tensor, *,
+                  dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [M, Hk, Dh] in bf16 or fp16 of the cache's slots (batch_idx, token_idx), in any order and as often as named;
+    zeros for a slot outside the cache."""
+    kind = _DTYPES.get(dtype)
+    _require(kind is not None and cache.codes.dim() == 5, "kv_nvfp4_read: a cache, and dtype bf16 or fp16")
+    dev = _gpu_of(cache.codes, cache.scales, cache.tensor_scale, batch_idx, token_idx)
+    B, N, _, Hk, half = cache.codes.shape
+    bi, ti = _index(batch_idx, "batch_idx"), _index(token_idx, "token_idx")
+    M = bi.shape[0]
+    _require(ti.shape == (M,), "kv_nvfp4_read: batch_idx and token_idx of one length")
+    c = _kv_nvfp4_args(cache, Hk, 2 * half, "kv_nvfp4_read")
+    k = torch.empty((M, Hk, 2 * half), device=bi.device, dtype=dtype)
+    v = torch.empty((M, Hk, 2 * half), device=bi.device, dtype=dtype)
+    _launch_on("kv_nvfp4_read", dev, bi, "oudjat_kv_nvfp4_read", *c, B, N, Hk, 2 * half, bi.data_ptr(), ti.data_ptr(), M,
+               kind, k.data_ptr(), v.data_ptr(), _lib.stream_of(bi))
+    return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _packed_attention_nvfp4_workspace(rows: int, S: int, Hq: int, Hk: int, Dh: int, cap: int) -> int:
+    return int(_lib.load().oudjat_packed_attention_nvfp4_workspace_elems(rows, S, Hq, Hk, Dh, cap))
+
+
+def packed_attention_nvfp4(q: torch.Tensor, cache: KvNvfp4, cu_q: torch.Tensor, k_lens: torch.Tensor, scale: float, *,
+                           causal: bool, out: torch.Tensor | None = None) -> torch.Tensor:
+    """packed_attention over an NVFP4 cache -> [M, Hq * Dh].
+
+    q [M, Hq, Dh], cu_q, causal, out and the rows without keys as there; k_lens [S] the key counts: sequence s reads the
+    first k_lens[s] tokens of batch s. Keys and values are the cache's, exactly; scores, statistics and sums in fp32, the
+    probabilities rounded to fp16 for either type of q. Unwritten or hidden tokens have no influence. A query row with a
+    NaN or an infinity gives NaN. scale must be positive. bf16 or fp16; Dh 64 or 128."""
+    qs, dtype = q.shape, q.dtype
+    kind = _DTYPES.get(dtype)
+    _require(len(qs) == 3 and kind is not None and q.stride(2) == 1 and cache.codes.dim() == 5,
+             "packed_attention_nvfp4: q [M, Hq, Dh] bf16 or fp16 with contiguous heads, and a cache")
+    M, Hq, Dh = qs
+    B, cap, _, Hk, _ = cache.codes.shape
+    c = _kv_nvfp4_args(cache, Hk, Dh, "packed_attention_nvfp4")
+    if out is None:
+        dev = _gpu_of(q, cache.codes, cache.scales, cache.tensor_scale, cu_q, k_lens)
+        out = torch.empty((M, Hq * Dh), device=q.device, dtype=dtype)
+    else:
+        dev = _gpu_of(q, cache.codes, cache.scales, cache.tensor_scale, cu_q, k_lens, out)
+        _require(out.shape == (M, Hq * Dh) and out.dtype == dtype and out.stride(1) == 1,
+                 "packed_attention_nvfp4: out must be [M, Hq * Dh] of q's type with contiguous rows")
+    S = cu_q.numel() - 1
+    _require(S >= 0 and _is_lengths(cu_q, S + 1) and _is_lengths(k_lens, S),
+             "packed_attention_nvfp4: cu_q [S + 1] and k_lens [S] must be contiguous int32 or int64")
+    _require(B >= S, "packed_attention_nvfp4: the cache has fewer batches than sequences")
+    elems = _packed_attention_nvfp4_workspace(M, S, Hq, Hk, Dh, cap)
+    ws = q.new_empty(elems, dtype=torch.float32) if elems > 0 else None  # (from the allocator: see packed_attention)
+    _launch_on("packed_attention_nvfp4", dev, q, "oudjat_packed_attention_nvfp4", q.data_ptr(), *_strides(q, 2), M, Hq, Dh,
+               *c, Hk, cap, cu_q.data_ptr(), cu_q.dtype == torch.int64, k_lens.data_ptr(), k_lens.dtype == torch.int64, S,
+               scale, causal, kind, out.data_ptr(), *_strides(out, 1), 0 if ws is None else ws.data_ptr(), elems,
+               _lib.stream_of(q))
+    return out

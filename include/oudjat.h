@@ -815,6 +815,64 @@ int oudjat_packed_attention(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64
 int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh,
                                                 int64_t key_cap);
 
+/* ---- INT8 products and NVFP4 K/V caches ------------------------------------------------------------------
+ * A layer of packed sequences in 8 and 4 bits (no counterpart in the reference, whose low-precision linears take
+ * per-tensor FP8 or NVFP4 and whose caches are 16-bit). */
+
+/* Rows of x [rows, K] (row stride x_rs) in 8 bits: scale[r] = max |x[r]| / 127 (fp32), codes[r, i] = x[r, i] / scale[r] to the
+ * nearest whole number, ties to even (IEEE quotient; 0 where the scale is 0). A row with a NaN or an infinity gets the
+ * scale NaN and codes 0. The same for a weight [N, K]: a scale for each output channel. K % 16 == 0; 16-byte aligned
+ * rows, those of codes (stride c_rs) apart from one another and from x. */
+int oudjat_quantize_int8(const uint16_t* x, int64_t rows, int64_t K, int64_t x_rs, int dtype, int8_t* codes, int64_t c_rs,
+                         float* scale, oudjat_stream_t stream);
+
+/* C[m, n] = epilogue((sum_k A[m, k] W[n, k]) (a_scale[m] w_scale[n]) + bias[n]) of int8 codes A [M, K], W [N, K], the sum
+ * exact in int32. Epilogues OUDJAT_EPI_BIAS, _LS (times gamma[n]), _LS_RESID (resid[m, n] + that) and _SILU_MUL (y / (1 +
+ * e^-y) resid[m, n]), in fp32 with one rounding at the end. bias (may be NULL), gamma, resid and C of type `dtype`. K % 64
+ * == 0, K < 2^17, N % 8 == 0; 16-byte aligned operands and rows (a_scale: 4). The rows of C apart; C may be resid. */
+int oudjat_linear_int8(const int8_t* A, int64_t M, int64_t K, int64_t lda, const float* a_scale, const int8_t* W,
+                       int64_t N, int64_t ldw, const float* w_scale, const uint16_t* bias, int epi,
+                       const uint16_t* gamma, const uint16_t* resid, int64_t ldr, uint16_t* C, int64_t ldc, int dtype,
+                       oudjat_stream_t stream);
+
+/* An NVFP4 K/V cache: codes [B, N, 2, Hk, Dh / 2] (two values a byte, the even one in the low nibble; strides c_bs, c_ns,
+ * c_cs, c_hs) and scales [B, N, 2, Hk, Dh / 16] (e4m3, one for 16 dims; s_bs .. s_hs), strides in bytes, and tensor_scale
+ * [2, Hk] fp32 (keys, then values): value = e2m1(code) * e4m3(scale) * tensor_scale. A head's codes 16-byte aligned, its
+ * scales by Dh / 16 bytes. Dh 64 or 128. Scale bytes are read without their sign; 0x7f counts as 480.
+ *
+ * Keys and values k, v [rows, Hk, Dh] (row and head strides) into the cache at (batch_idx, token_idx): per block of 16 dims
+ * scale = e4m3(clamp(max |x| / 6 / tensor_scale, 2^-16, 448)), code = e2m1(x / (tensor_scale * scale)) in fp32 with IEEE
+ * quotients, nearest even, saturating; a block whose scale rounds to 0 holds zeros. NaN counts as 0, infinities as the
+ * largest value. Rows whose slot lies outside B x N are skipped; the slots of the others must be unique. The cache may
+ * not overlap itself or k and v. tensor_scale > 0 and finite. */
+int oudjat_kv_nvfp4_write(const uint16_t* k, int64_t k_rs, int64_t k_hs, const uint16_t* v, int64_t v_rs, int64_t v_hs,
+                          int64_t rows, int64_t Hk, int64_t Dh, int dtype, const int64_t* batch_idx,
+                          const int64_t* token_idx, uint8_t* codes, int64_t c_bs, int64_t c_ns, int64_t c_cs,
+                          int64_t c_hs, uint8_t* scales, int64_t s_bs, int64_t s_ns, int64_t s_cs, int64_t s_hs,
+                          const float* tensor_scale, int64_t B, int64_t N, oudjat_stream_t stream);
+
+/* Rows of the cache in 16 bits: k_out, v_out [rows, Hk, Dh] contiguous, the values rounded once; zeros for a slot outside
+ * B x N. */
+int oudjat_kv_nvfp4_read(const uint8_t* codes, int64_t c_bs, int64_t c_ns, int64_t c_cs, int64_t c_hs,
+                         const uint8_t* scales, int64_t s_bs, int64_t s_ns, int64_t s_cs, int64_t s_hs,
+                         const float* tensor_scale, int64_t B, int64_t N, int64_t Hk, int64_t Dh,
+                         const int64_t* batch_idx, const int64_t* token_idx, int64_t rows, int dtype, uint16_t* k_out,
+                         uint16_t* v_out, oudjat_stream_t stream);
+
+/* oudjat_packed_attention over an NVFP4 cache (sequence s in batch s, key_cap tokens each, keys[s] of them), with the
+ * cached values as k and v. The probabilities are rounded to fp16 whatever the type of q and out. A query row with a NaN
+ * or an infinity gives NaN where it sees a key. c_ns, s_ns < 2^24. Workspace of
+ * oudjat_packed_attention_nvfp4_workspace_elems fp32 elements as there. */
+int oudjat_packed_attention_nvfp4(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64_t rows, int64_t Hq, int64_t Dh,
+                                  const uint8_t* codes, int64_t c_bs, int64_t c_ns, int64_t c_cs, int64_t c_hs,
+                                  const uint8_t* scales, int64_t s_bs, int64_t s_ns, int64_t s_cs, int64_t s_hs,
+                                  const float* tensor_scale, int64_t Hk, int64_t key_cap, const void* cu_q, int cu_wide,
+                                  const void* keys, int keys_wide, int64_t S, float scale, int causal, int dtype,
+                                  uint16_t* out, int64_t out_rs, float* workspace, int64_t workspace_elems,
+                                  oudjat_stream_t stream);
+int64_t oudjat_packed_attention_nvfp4_workspace_elems(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh,
+                                                      int64_t key_cap);
+
 #ifdef __cplusplus
 }
 #endif
