@@ -5,6 +5,7 @@
 // then the epilogue in fp32 and one rounding to the output's type.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "elem.hpp"
 #include "packed_attn.hpp"
@@ -129,21 +130,18 @@ struct Int8Gemm {
 template <class E, int EPI>
 __device__ __forceinline__ void int8_store4(const Int8Gemm& g, int m, int n, const i32x4v_t& acc) {
   typedef uint16_t u16x4_t __attribute__((ext_vector_type(4)));
-  const float sa = g.sa[m];
-  const float4 sw = *reinterpret_cast<const float4*>(g.sw + n);
-  float y[4] = {(float)acc[0] * (sa * sw.x), (float)acc[1] * (sa * sw.y), (float)acc[2] * (sa * sw.z),
-                (float)acc[3] * (sa * sw.w)};
   auto four = [&](const uint16_t* p, float* f) {
-    const u16x4_t b = *reinterpret_cast<const u16x4_t*>(p);
+    const u16x4_t v = *reinterpret_cast<const u16x4_t*>(p);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = E::value(b[e]);
+    for (int e = 0; e < 4; ++e) f[e] = E::value(v[e]);
   };
-  float t[4];
-  if (g.bias) {
-    four(g.bias + n, t);
+  const float sa = g.sa[m];
+  const float4 sw4 = *reinterpret_cast<const float4*>(g.sw + n);
+  const float sw[4] = {sw4.x, sw4.y, sw4.z, sw4.w};
+  float y[8] = {}, bias[4] = {}, t[4];
+  if (g.bias) four(g.bias + n, bias);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] += t[e];
-  }
+  for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf((float)acc[e], sa * sw[e], bias[e]);
   if constexpr (EPI == OUDJAT_EPI_BIAS_LS || EPI == OUDJAT_EPI_BIAS_LS_RESID) {
     four(g.gamma + n, t);
 #pragma unroll
@@ -155,21 +153,85 @@ __device__ __forceinline__ void int8_store4(const Int8Gemm& g, int m, int n, con
     for (int e = 0; e < 4; ++e)
       y[e] = EPI == OUDJAT_EPI_BIAS_LS_RESID ? y[e] + t[e] : y[e] / (1.0f + expf(-y[e])) * t[e];
   }
-  const float out[8] = {y[0], y[1], y[2], y[3], 0, 0, 0, 0};
-  const uint4 o = E::from8(out);
+  const uint4 o = E::from8(y);
   *reinterpret_cast<uint2*>(g.c + (int64_t)m * g.ldc + n) = make_uint2(o.x, o.y);
 }
 
-// Tile kernel: BM x BN outputs, WGM x WGN waves, K in steps of 128 bytes through NST stages of LDS, filled by buffer
-// loads (descriptors of the tile's rows that exist: others load as zeros). LDS row r keeps its 16-byte chunk c in slot
-// c ^ (r / 2) % 8, so that 16 rows at one chunk cover all banks. v_mfma_i32_16x16x64_i8 with the weight as its first
-// operand: lane l holds row l % 16, columns 4 (l / 16) .. + 3 of a 16 x 16 block.
+// Direct kernel, for few rows: 16 x 16 outputs a workgroup, whose eight waves take 128 bytes of K each in turn, straight
+// from memory to registers (a weight is used by one workgroup, or by few), four such chunks in flight, and add their
+// sums up in LDS. Bound by the latency of a launch and two rounds of loads, then by reading the weight: 1 x 4096 x 4096
+// 5.9 us (2.8 TB/s; one chunk more or fewer in flight, 16 waves, 16 x 32 outputs: 5.8 to 7.3).
+static constexpr int kDirectWaves = 8;
+template <class E, int EPI>
+__global__ __launch_bounds__(kDirectWaves * 64) void int8_direct_kernel(Int8Gemm g) {
+  constexpr int WAVES = kDirectWaves, U = 4;  // chunks in flight
+  __shared__ i32x4v_t park[WAVES * 64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, G = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tm = blockIdx.x % g.tiles_m, tn = blockIdx.x / g.tiles_m;
+  const int m0 = tm * 16, n0 = tn * 16;
+  const int8_t *A = g.a + (int64_t)m0 * g.lda, *W = g.w + (int64_t)n0 * g.ldw;
+  // (rows past the last repeat it and are not stored)
+  const uint32_t oa = (uint32_t)min(l16, g.M - 1 - m0) * (uint32_t)g.lda + 16u * G;
+  const uint32_t ow = (uint32_t)min(l16, g.N - 1 - n0) * (uint32_t)g.ldw + 16u * G;
+  struct Unit {
+    i32x4v_t a[2], w[2];
+  };
+  const int chunks = (g.K + 127) / 128;
+  auto both = [&](int c) { return c * 128 + 64 < g.K; };  // K = 64 mod 128: the last chunk is half a one
+  auto load = [&](Unit& u, int c) __attribute__((always_inline)) {
+    const int8_t *a = A + (int64_t)c * 128, *w = W + (int64_t)c * 128;
+    const uint32_t second = both(c) ? 64u : 0u;
+    u.w[0] = *reinterpret_cast<const i32x4v_t*>(w + ow);
+    u.w[1] = *reinterpret_cast<const i32x4v_t*>(w + (ow + second));
+    u.a[0] = *reinterpret_cast<const i32x4v_t*>(a + oa);
+    u.a[1] = *reinterpret_cast<const i32x4v_t*>(a + (oa + second));
+  };
+  i32x4v_t acc = {0, 0, 0, 0};
+  auto products = [&](const Unit& u, int c) __attribute__((always_inline)) {
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.w[0], u.a[0], acc, 0, 0, 0);
+    if (both(c)) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.w[1], u.a[1], acc, 0, 0, 0);
+  };
+  Unit u[U];
+  int c = wave;
+#pragma unroll
+  for (int i = 0; i < U - 1; ++i)
+    if (c + i * WAVES < chunks) load(u[i], c + i * WAVES);
+  while (c < chunks) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (c >= chunks) break;
+      if (c + (U - 1) * WAVES < chunks) load(u[(i + U - 1) % U], c + (U - 1) * WAVES);
+      products(u[i], c);
+      c += WAVES;
+    }
+  }
+  park[wave * 64 + lane] = acc;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) acc += park[w * 64 + lane];
+  if (m0 + l16 < g.M && n0 + 4 * G < g.N) int8_store4<E, EPI>(g, m0 + l16, n0 + 4 * G, acc);
+}
+
+// Tile kernel: BM x BN outputs, WGM x WGN waves of WM x WN each, K in tiles of 128 bytes through NST stages of LDS that
+// buffer loads fill (descriptors of the tile's rows that exist: others load as zeros). LDS row r keeps its 16-byte chunk
+// c in slot c ^ (r / 2) % 8, so that 16 rows at one chunk cover all banks. v_mfma_i32_16x16x64_i8 with the weight as its
+// first operand: lane l holds row l % 16, columns 4 (l / 16) .. + 3 of a 16 x 16 block.
+// A tile of K is two steps. While the matrix cores work on the fragments of one step, those of the next are read; a
+// barrier in the middle of the tile says that all waves have read it, so that the loads of the K tile NST further on may
+// go to its stage, and that the next tile has landed.
+// 256 x 256: eight waves of 128 x 64, two on a SIMD (four of 128 x 128 with twice the accumulators need both register files,
+// and moves between them: 571 us against 433 at 8192^3). 8192^3: 433 us, 2540 TOP/s at 1.9 GHz, matrix cores busy 65 %
+// (the library's product 1897 TOP/s there, 2335 at 16384^3). Small tiles are bound by their fragments' way through
+// LDS and by the two rounds of its latency in each K tile, which deeper stages do not shorten.
 template <class E, int EPI, int BM, int BN, int WGM, int WGN, int NST>
 __global__ __launch_bounds__(WGM * WGN * 64) void int8_tile_kernel(Int8Gemm g) {
   constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
-  constexpr int STAGE = (BM + BN) * 128, LA = BM / (8 * NW), LW = BN / (8 * NW), L = LA + LW;
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads");
-  static_assert((NST - 1) * L < 64, "vmcnt range");
+  constexpr int STAGE = (BM + BN) * 128, L = (BM + BN + 8 * NW - 1) / (8 * NW);
+  constexpr int LEAST = (BM + BN) / (8 * NW);  // loads of a tile that every wave has
+  static_assert(BM % 16 == 0 && BN % 16 == 0 && WM % 16 == 0 && WN % 16 == 0, "whole blocks");
+  static_assert(NST >= 2 && (NST - 1) * L < 64, "vmcnt range");
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 63, l16 = lane & 15, G = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -181,67 +243,165 @@ __global__ __launch_bounds__(WGM * WGN * 64) void int8_tile_kernel(Int8Gemm g) {
   const int high = min(8, g.tiles_m - first), tm = first + in % high, tn = in / high;
   const int m0 = tm * BM, n0 = tn * BN;
 
-  const int8_t* A = g.a + (int64_t)m0 * g.lda;
-  const int8_t* W = g.w + (int64_t)n0 * g.ldw;
-  const i32x4_t ra = make_buffer_rsrc(A, (uint32_t)(min(BM, g.M - m0) - 1) * (uint32_t)g.lda + (uint32_t)g.K);
-  const i32x4_t rw = make_buffer_rsrc(W, (uint32_t)(min(BN, g.N - n0) - 1) * (uint32_t)g.ldw + (uint32_t)g.K);
-  const int lrow = lane >> 3;  // of the 8 rows that one load fills
-  const uint32_t chunk = (uint32_t)(((lane & 7) ^ ((8 * wave + lrow) >> 1)) & 7) << 4;
-  const uint32_t va = (uint32_t)(8 * wave + lrow) * (uint32_t)g.lda + chunk;
-  const uint32_t vw = (uint32_t)(8 * wave + lrow) * (uint32_t)g.ldw + chunk;
-  auto issue = [&](int kt) __attribute__((always_inline)) {
-    unsigned char* st = smem + (kt % NST) * STAGE + wave * 1024;
+  const i32x4_t ra = make_buffer_rsrc(g.a + (int64_t)m0 * g.lda,
+                                      (uint32_t)(min(BM, g.M - m0) - 1) * (uint32_t)g.lda + (uint32_t)g.K);
+  const i32x4_t rw = make_buffer_rsrc(g.w + (int64_t)n0 * g.ldw,
+                                      (uint32_t)(min(BN, g.N - n0) - 1) * (uint32_t)g.ldw + (uint32_t)g.K);
+  const int lrow = 8 * wave + (lane >> 3);  // of the 8 rows that one load fills
+  const uint32_t chunk = (uint32_t)((lane & 7) ^ ((lrow >> 1) & 7)) << 4;
+  const uint32_t va = (uint32_t)lrow * (uint32_t)g.lda + chunk, vw = (uint32_t)lrow * (uint32_t)g.ldw + chunk;
+  auto load = [&](int kt, int i) __attribute__((always_inline)) {  // load i of L: rows of A, then of W
+    unsigned char* st = smem + (kt % NST) * STAGE + (i * NW + wave) * 1024;
     const uint32_t k0 = (uint32_t)kt * 128u;
-#pragma unroll
-    for (int i = 0; i < LA; ++i)
-      buffer_load_lds16(ra, st + i * NW * 1024, va + (uint32_t)(i * 8 * NW) * (uint32_t)g.lda + k0);
-#pragma unroll
-    for (int i = 0; i < LW; ++i)
-      buffer_load_lds16(rw, st + BM * 128 + i * NW * 1024, vw + (uint32_t)(i * 8 * NW) * (uint32_t)g.ldw + k0);
+    const uint32_t oa = va + (uint32_t)(i * 8 * NW) * (uint32_t)g.lda + k0;
+    if ((i + 1) * 8 * NW > BM + BN && i * 8 * NW + 8 * wave >= BM + BN) return;
+    const uint32_t ow = vw + (uint32_t)(i * 8 * NW - BM) * (uint32_t)g.ldw + k0;
+    if ((i + 1) * 8 * NW <= BM) buffer_load_lds16(ra, st, oa);
+    else if (i * 8 * NW >= BM) buffer_load_lds16(rw, st, ow);
+    else if (i * 8 * NW + 8 * wave < BM) buffer_load_lds16(ra, st, oa);
+    else buffer_load_lds16(rw, st, ow);
   };
-  auto at = [&](int row, int c) { return row * 128 + ((c ^ ((row >> 1) & 7)) << 4); };
 
+  struct Frags {
+    i32x4v_t a[FM], w[FN];
+  };
+  const int swz = (l16 >> 1) & 7;
+  const int aoff = (wm * WM + l16) * 128, woff = (BM + wn * WN + l16) * 128;
+  const int slot[2] = {(G ^ swz) << 4, ((4 + G) ^ swz) << 4};
+  // Fragment f of a step: the weight's first, which the step's first products all need.
+  auto read = [&](Frags& x, const unsigned char* st, int s, int f) __attribute__((always_inline)) {
+    if (f < FN) x.w[f] = *reinterpret_cast<const i32x4v_t*>(st + woff + slot[s] + f * 2048);
+    else x.a[f - FN] = *reinterpret_cast<const i32x4v_t*>(st + aoff + slot[s] + (f - FN) * 2048);
+  };
   i32x4v_t acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = i32x4v_t{0, 0, 0, 0};
-  const int KT = (g.K + 127) / 128;
+  // One step: the products of `cur`, one row of blocks at a time, with the reads of `nxt` (step s of stage `st`) and the
+  // loads of K tile kt spread over them. PART: a wave whose last rows are past M leaves those blocks out.
+  constexpr int RPR = (FM + FN + FM - 1) / FM, LPR = (L + FM - 1) / FM;  // reads and loads for each row of blocks
+  const int blocks = min(FM, (g.M - m0 - wm * WM + 15) / 16);
+  auto step = [&](const Frags& cur, Frags& nxt, const unsigned char* st, int s, int kt, auto reads, auto loads, auto part)
+      __attribute__((always_inline)) {
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s)
-    if (s < KT) issue(s);
-  for (int kt = 0; kt < KT; ++kt) {
-    // Tile kt has landed when only the loads of the tiles after it are in flight.
-    if (NST == 2 || kt + 1 >= KT) wait_vmcnt<0>();
-    else if (NST == 3 || kt + 2 >= KT) wait_vmcnt<L>();
-    else wait_vmcnt<2 * L>();
-    block_barrier();
-    if (kt + NST - 1 < KT) issue(kt + NST - 1);
-    const unsigned char* st = smem + (kt % NST) * STAGE;
+    for (int i = 0; i < FM; ++i) {
+      if constexpr (decltype(reads)::value)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (s == 1 && kt * 128 + 64 >= g.K) break;  // K = 64 mod 128: the last half tile holds other rows' bytes
-      i32x4v_t fa[FM], fw[FN];
+        for (int f = i * RPR; f < (i + 1) * RPR; ++f)
+          if (f < FM + FN) read(nxt, st, s, f);
+      if constexpr (decltype(loads)::value)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-        fa[i] = *reinterpret_cast<const i32x4v_t*>(st + at(wm * WM + 16 * i + l16, 4 * s + G));
+        for (int f = i * LPR; f < (i + 1) * LPR; ++f)
+          if (f < L) load(kt, f);
+      if (!decltype(part)::value || i < blocks) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-        fw[j] = *reinterpret_cast<const i32x4v_t*>(st + BM * 128 + at(wn * WN + 16 * j + l16, 4 * s + G));
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[j], cur.a[i], acc[i][j], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-  }
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  const int KT = (g.K + 127) / 128;
+  auto wait_tiles = [&](int n) __attribute__((always_inline)) {  // the loads of n tiles may stay in flight
+    if constexpr (NST > 3) {
+      if (n >= 3) return wait_vmcnt<(NST > 4 ? 3 : 2) * LEAST>();
+    }
+    if constexpr (NST > 2) {
+      if (n == 2) return wait_vmcnt<(NST > 3 ? 2 : 1) * LEAST>();
+      if (n == 1) return wait_vmcnt<LEAST>();
+    }
+    wait_vmcnt<0>();
+  };
+  Frags x, y;
+  auto run = [&](auto part) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = m0 + wm * WM + 16 * i + l16;
-    if (m >= g.M) continue;
+    for (int f = 0; f < FM + FN; ++f) read(x, smem, 0, f);
+    int kt = 0, st = 0;
+    auto middle = [&](int n) __attribute__((always_inline)) {
+      wait_tiles(n);
+      block_barrier();
+    };
+    auto next = [&]() { return st + 1 == NST ? 0 : st + 1; };
+    for (; kt + NST < KT; ++kt) {
+      step(x, y, smem + st * STAGE, 1, 0, Yes{}, No{}, part);
+      middle(NST - 2);
+      st = next();
+      step(y, x, smem + st * STAGE, 0, kt + NST, Yes{}, Yes{}, part);
+    }
+    for (; kt + 1 < KT; ++kt) {
+      step(x, y, smem + st * STAGE, 1, 0, Yes{}, No{}, part);
+      middle(KT - 2 - kt);
+      st = next();
+      step(y, x, smem + st * STAGE, 0, 0, Yes{}, No{}, part);
+    }
+    step(x, y, smem + st * STAGE, 1, 0, Yes{}, No{}, part);
+    if (g.K % 128 == 0) step(y, x, smem, 0, 0, No{}, No{}, part);  // K = 64 mod 128: that half holds other rows' bytes
+  };
+#pragma unroll
+  for (int t = 0; t < NST; ++t)
+    if (t < KT)
+#pragma unroll
+      for (int f = 0; f < L; ++f) load(t, f);
+  wait_tiles(min(NST, KT) - 1);
+  block_barrier();
+  run(std::integral_constant<bool, (BM >= 128)>{});
+
+  // Epilogue. A wave writes its outputs in fp32, bias and gamma applied, to LDS, RB rows at a time, and takes them up again
+  // in rows, 8 columns a lane, for the residual and the stores.
+  constexpr int RB = WM % 32 ? 16 : 32, LD = WN + 4, CL = WN / 8, RPP = 64 / CL;  // rows of a pass over the lanes
+  static_assert(WM % RB == 0 && 64 % CL == 0 && RB % RPP == 0, "rows of the epilogue");
+  block_barrier();  // (every wave is done with the stages)
+  float* park = reinterpret_cast<float*>(smem) + wave * RB * LD;
+  typedef uint16_t u16x4_t __attribute__((ext_vector_type(4)));
+  auto four = [&](const uint16_t* p, float* f) __attribute__((always_inline)) {
+    const u16x4_t v = *reinterpret_cast<const u16x4_t*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = E::value(v[e]);
+  };
+#pragma unroll
+  for (int h = 0; h < WM / RB; ++h) {
+    if (m0 + wm * WM + h * RB >= g.M) break;  // uniform over the wave
+    float sa[RB / 16];
+#pragma unroll
+    for (int i = 0; i < RB / 16; ++i) sa[i] = g.sa[min(m0 + wm * WM + h * RB + 16 * i + l16, g.M - 1)];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      const int n = n0 + wn * WN + 16 * j + 4 * G;
-      if (n < g.N) int8_store4<E, EPI>(g, m, n, acc[i][j]);
+      const int n = min(n0 + wn * WN + 16 * j + 4 * G, g.N - 4);  // (columns past the last are not stored)
+      const float4 sw4 = *reinterpret_cast<const float4*>(g.sw + n);
+      const float sw[4] = {sw4.x, sw4.y, sw4.z, sw4.w};
+      float bias[4] = {}, gamma[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+      if (g.bias) four(g.bias + n, bias);
+      if constexpr (EPI == OUDJAT_EPI_BIAS_LS || EPI == OUDJAT_EPI_BIAS_LS_RESID) four(g.gamma + n, gamma);
+#pragma unroll
+      for (int i = 0; i < RB / 16; ++i) {
+        f32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = __builtin_fmaf((float)acc[h * (RB / 16) + i][j][e], sa[i] * sw[e], bias[e]);
+          if constexpr (EPI == OUDJAT_EPI_BIAS_LS || EPI == OUDJAT_EPI_BIAS_LS_RESID) v[e] *= gamma[e];
+        }
+        *reinterpret_cast<f32x4_t*>(park + (16 * i + l16) * LD + 16 * j + 4 * G) = v;
+      }
+    }
+    const int c = lane % CL, n = n0 + wn * WN + 8 * c;
+#pragma unroll
+    for (int r0 = 0; r0 < RB; r0 += RPP) {
+      const int r = r0 + lane / CL, m = m0 + wm * WM + h * RB + r;
+      if (m >= g.M || n >= g.N) continue;
+      const float* src = park + r * LD + 8 * c;
+      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(src), hi = *reinterpret_cast<const f32x4_t*>(src + 4);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if constexpr (EPI == OUDJAT_EPI_BIAS_LS_RESID || EPI == OUDJAT_EPI_BIAS_SILU_MUL) {
+        float t[8];
+        E::to8(load16(g.resid + (int64_t)m * g.ldr + n), t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[e] = EPI == OUDJAT_EPI_BIAS_LS_RESID ? v[e] + t[e] : v[e] / (1.0f + expf(-v[e])) * t[e];
+      }
+      store16(g.c + (int64_t)m * g.ldc + n, E::from8(v));
     }
   }
 }
@@ -285,7 +445,8 @@ extern "C" int oudjat_quantize_int8(const uint16_t* x, int64_t rows, int64_t K, 
 template <class E, int EPI, int BM, int BN, int WGM, int WGN, int NST>
 static int launch_tile(Int8Gemm g, hipStream_t st, const char* what) {
   static std::atomic<uint64_t> done{0};
-  constexpr int lds = NST * (BM + BN) * 128;
+  constexpr int RB = BM / WGM % 32 ? 16 : 32;  // rows of a wave that the epilogue stages
+  constexpr int lds = std::max(NST * (BM + BN) * 128, WGM * WGN * RB * (BN / WGN + 4) * 4);
   const auto fn = int8_tile_kernel<E, EPI, BM, BN, WGM, WGN, NST>;
   const int rc = allow_lds((const void*)fn, lds, done, what);
   if (rc != OUDJAT_OK) return rc;
@@ -296,8 +457,59 @@ static int launch_tile(Int8Gemm g, hipStream_t st, const char* what) {
 }
 
 template <class E, int EPI>
+static int launch_direct(Int8Gemm g, hipStream_t st, const char* what) {
+  g.tiles_m = (int)cdiv(g.M, 16);
+  g.tiles_n = (int)cdiv(g.N, 16);
+  int8_direct_kernel<E, EPI><<<(unsigned)g.tiles_m * g.tiles_n, kDirectWaves * 64, 0, st>>>(g);
+  return check_launch(what);
+}
+
+// The kernels, and the time of a call in us: start + rounds of tiles over the CUs x (K tiles x per_k + per_tile), fitted to
+// 74 shapes (1 .. 16404 rows, N 64 .. 12288, K 64 .. 8192) that ran with each of them on one card; the kernel that this
+// chooses is 1 % slower than the fastest on the mean, 16 % at most (668 x 256 x 1088: 5.2 us by 64 x 64 tiles, 4.5 directly).
+// Where the others lie, us by 16 x 16 directly / 64 x 64 / 64 x 128 / 128 x 128 / 192 x 256 / 256 x 256:
+//   1 x 4096 x 4096: 5.9 / 9.4 / 12 / 21 / 28 / 30;  32 x 8192 x 4096: 17 / 9.8 / 13 / 22 / 28 / 30;
+//   512 x 4096 x 4096: 114 / 16 / 14 / 25 / 40 / 47;  1656 x 4096 x 8192: 727 / 90 / 78 / 60 / 76 / 87;
+//   1656 x 12288 x 4096: 1090 / 134 / 110 / 97 / 91 / 101;  16404 x 4096 x 8192: - / 833 / 671 / 547 / 504 / 499.
+struct Int8Tile {
+  int bm, bn;
+  float start, per_k, per_tile;
+};
+static const Int8Tile kInt8Tiles[] = {
+    {16, 16, 2.29f, 0.088f, 0.2f},   {64, 64, 2.27f, 0.189f, 0.91f}, {64, 128, 1.97f, 0.292f, 1.39f},
+    {128, 128, 2.5f, 0.479f, 2.39f}, {192, 256, 1.0f, 1.18f, 6.87f}, {256, 256, 1.0f, 1.346f, 9.13f},
+};
+static int choose_int8(int64_t M, int64_t N, int64_t K) {
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < (int)(sizeof(kInt8Tiles) / sizeof(kInt8Tiles[0])); ++i) {
+    const Int8Tile& t = kInt8Tiles[i];
+    const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
+    const float us = t.start + (float)cdiv(tiles, 256) * ((float)K / 128.0f * t.per_k + t.per_tile);
+    if (i == 0 || us < least) best = i, least = us;
+  }
+  return best;
+}
+
+template <class E, int EPI>
 static int launch_int8(const Int8Gemm& g, hipStream_t st, const char* what) {
-  return launch_tile<E, EPI, 128, 128, 2, 2, 2>(g, st, what);
+  switch (choose_int8(g.M, g.N, g.K)) {
+    case 0: return launch_direct<E, EPI>(g, st, what);
+    case 1: return launch_tile<E, EPI, 64, 64, 2, 2, 4>(g, st, what);
+    case 2: return launch_tile<E, EPI, 64, 128, 2, 4, 3>(g, st, what);
+    case 3: return launch_tile<E, EPI, 128, 128, 2, 2, 2>(g, st, what);
+    case 4: return launch_tile<E, EPI, 192, 256, 2, 4, 2>(g, st, what);
+    default: return launch_tile<E, EPI, 256, 256, 2, 4, 2>(g, st, what);
+  }
+}
+
+extern "C" int oudjat_linear_int8_tile(int64_t M, int64_t N, int64_t K, int* rows, int* columns) {
+  const char* what = "linear_int8_tile";
+  OUDJAT_REQUIRE(M > 0 && N > 0 && K > 0 && rows && columns, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad argument", what);
+  const Int8Tile& t = kInt8Tiles[choose_int8(M, N, K)];
+  *rows = t.bm;
+  *columns = t.bn;
+  return OUDJAT_OK;
 }
 
 extern "C" int oudjat_linear_int8(const int8_t* A, int64_t M, int64_t K, int64_t lda, const float* a_scale,

@@ -1637,6 +1637,13 @@ def linear_int8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_sca
     return out
 
 
+def linear_int8_tile(M: int, N: int, K: int) -> tuple[int, int]:
+    """(rows, columns) of the output tile that linear_int8 takes for an M x N x K product."""
+    rows, columns = ctypes.c_int(0), ctypes.c_int(0)
+    call("oudjat_linear_int8_tile", M, N, K, ctypes.addressof(rows), ctypes.addressof(columns))
+    return rows.value, columns.value
+
+
 @dataclass
 class KvNvfp4:
     """A K/V cache in NVFP4: codes uint8 [B, N, 2, Hk, Dh / 2] (keys, then values; two e2m1 codes a byte, the even dim in

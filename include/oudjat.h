@@ -835,6 +835,10 @@ int oudjat_linear_int8(const int8_t* A, int64_t M, int64_t K, int64_t lda, const
                        const uint16_t* gamma, const uint16_t* resid, int64_t ldr, uint16_t* C, int64_t ldc, int dtype,
                        oudjat_stream_t stream);
 
+/* Rows and columns of the output tile that oudjat_linear_int8 takes for an M x N x K product (16 x 16: the kernel without LDS
+ * tiles, for few rows). */
+int oudjat_linear_int8_tile(int64_t M, int64_t N, int64_t K, int* rows, int* columns);
+
 /* An NVFP4 K/V cache: codes [B, N, 2, Hk, Dh / 2] (two values a byte, the even one in the low nibble; strides c_bs, c_ns,
  * c_cs, c_hs) and scales [B, N, 2, Hk, Dh / 16] (e4m3, one for 16 dims; s_bs .. s_hs), strides in bytes, and tensor_scale
  * [2, Hk] fp32 (keys, then values): value = e2m1(code) * e4m3(scale) * tensor_scale. A head's codes 16-byte aligned, its

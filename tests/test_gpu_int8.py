@@ -132,6 +132,12 @@ SHAPES = [(1, 8, 64), (1, 4096, 4096), (2, 384, 384), (15, 200, 128), (16, 1024,
           (1656, 4096, 512), (2049, 776, 192), (4176, 1024, 1024)]
 
 
+# Every tile at least twice, with ragged edges, one and several K tiles, whole ones and half ones at the end
+# (test_int8_nvfp4_host.py says so); the widths of this package's blocks.
+SHAPES += [(3531, 2184, 64), (2305, 5000, 192), (4117, 3896, 832), (2289, 4680, 192), (922, 11272, 320), (3000, 4104, 64),
+           (3000, 4104, 192), (5243, 5448, 704), (1656, 8200, 576), (300, 1032, 2112)]
+
+
 @pytest.mark.parametrize("epi", ["bias", "ls", "ls_resid", "silu"])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("M,N,Kd", SHAPES)
