@@ -257,27 +257,257 @@ __global__ __launch_bounds__(WAVES * 64) void nvfp4_attn_keys_kernel(Nvfp4Attn n
   store16(a.out + (int64_t)orow * a.o_rs + (int64_t)ohead * DH + 8 * ch, E::from8(z));
 }
 
+// ------------------------------------------------------------------------------------------------
+// Rows kernel: R = 32 W packed rows, a wave owns 32, all waves of the workgroup share tiles of 64 keys in fp16 in LDS. S^T =
+// K . Q^T and O^T += V^T . P^T on v_mfma_f32_32x32x16 as in packed_attention.hip: a row is one lane pair (l, l ^ 32), whose
+// registers hold its scores. A thread turns pieces of 32 dims (16 bytes of codes, two scales) into fp16 once for the
+// workgroup; a piece is loaded two tiles ahead and written one tile ahead, between the first product and the softmax of
+// the tile before. 16 lanes write the same dims of 16 keys, which covers all banks.
+// ------------------------------------------------------------------------------------------------
+template <class E, int DH, int W>
+__global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na) {
+  constexpr int R = 32 * W, QK_STEPS = DH / 16, OB = DH / 32, ROWB = 2 * DH;
+  constexpr int TILEB = kKeyTile * ROWB, STAGE = 2 * TILEB;
+  constexpr int PIECES = 2 * kKeyTile * (DH / 32) / (64 * W), PPW = 64 / (DH / 32);  // a thread's; keys of a wave's pieces
+  static_assert(PIECES == 1 || PIECES == 2, "whole pieces");
+  const PackedAttn& a = na.p;
+  extern __shared__ __align__(16) unsigned char smem[];
+
+  const int item = a.by_hk(blockIdx.x), h = blockIdx.x - item * a.Hk;
+  Item w;
+  if (!take_item<R, kKeyTile>(a, item, h, w)) return;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int total = w.m * a.G;                       // packed rows of the sequence
+  const int r0 = w.tile * R, rw = r0 + wave * 32;    // first row of the tile and of this wave
+  const int row = rw + l32;
+  const bool active = rw < total, mine = row < total;
+  const int at = min(row, total - 1);  // rows past the last repeat it and are not stored
+  const int tok = a.by_g(at), head = at - tok * a.G;
+  const int lim = seen_keys(a, w, tok);
+  // Keys: the tile's last row sees kend, its first lim_tile (all full tiles below need no mask); the same per wave.
+  const int kend = seen_keys(a, w, a.by_g(min(r0 + R, total) - 1));
+  const int lim_tile = seen_keys(a, w, a.by_g(r0));
+  const int kend_wave = active ? seen_keys(a, w, a.by_g(min(rw + 32, total) - 1)) : 0;
+  const int lim_wave = active ? seen_keys(a, w, a.by_g(rw)) : w.n;
+  const int all_tiles = (kend + kKeyTile - 1) / kKeyTile;
+  const int per = w.parts == 1 ? all_tiles : (all_tiles + w.parts - 1) / w.parts;
+  const int tb = w.part * per;                       // first key tile of this part; tiles are numbered from it below
+  const int ntiles = max(0, min(per, all_tiles - tb));
+  const int nfull = lim_tile / kKeyTile - tb;
+
+  h8_t qf[QK_STEPS];  // lane: row l32, dims 16 ks + 8 g ..
+  bool bad;
+  const float down = load_query<E, QK_STEPS>(
+      a.q + (int64_t)(w.q0 + tok) * a.q_rs + (int64_t)(h * a.G + head) * a.q_hs + 8 * g, 16, qf, bad,
+      [](float x) { return xor32_max(x); }, [](float x) { return xor32_sum(x); });
+  const float c = fmaxf(na.scale_log2 * na.c.ts[h] * down, 1.17549435e-38f);
+
+  // This thread's pieces: with one a thread the waves' first half takes keys, the second values.
+  const int pw = PIECES == 1 ? wave % (W / 2) : wave, pkey = pw * PPW + (lane & 15) + 16 * (lane / (16 * (DH / 32)));
+  const int pc = (lane >> 4) % (DH / 32);
+  const uint8_t *kc = na.c.codes + (int64_t)w.seq * na.c.bs + (int64_t)h * na.c.hs + 16 * pc;
+  const uint8_t *ksc = na.c.scales + (int64_t)w.seq * na.c.sbs + (int64_t)h * na.c.shs + 2 * pc;
+  const bool second = PIECES == 1 && wave >= W / 2;
+  if (second) {
+    kc += na.c.cs;
+    ksc += na.c.scs;
+  }
+  struct Pieces {
+    uint4 codes[PIECES];
+    uint32_t scales[PIECES];
+  };
+  auto load = [&](Pieces& x, int t) __attribute__((always_inline)) {
+    const int key0 = (tb + t) * kKeyTile;
+    const uint32_t r = (uint32_t)min(pkey, w.n - 1 - key0);  // keys past the last repeat it, their weight is 0
+    const uint8_t *kp = kc + (int64_t)key0 * na.c.ns, *ksp = ksc + (int64_t)key0 * na.c.sns;
+    const uint32_t off = r * (uint32_t)na.c.ns, soff = r * (uint32_t)na.c.sns;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      x.codes[i] = *reinterpret_cast<const uint4*>(kp + (i ? na.c.cs : 0) + off);
+      x.scales[i] = *reinterpret_cast<const uint16_t*>(ksp + (i ? na.c.scs : 0) + soff);
+    }
+  };
+  int slot[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) slot[j] = tile_slot<DH>(pkey, 4 * pc + j) + (second ? TILEB : 0);
+  auto expand = [&](const Pieces& x, unsigned char* st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint32_t word[4] = {x.codes[i].x, x.codes[i].y, x.codes[i].z, x.codes[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<h8_t*>(st + slot[j] + i * TILEB) = xhat8(word[j], scale_pair(x.scales[i], j / 2));
+    }
+  };
+
+  f32x16_t o[OB];
+  float m_i = -INFINITY, l_i = 0.0f;
+#pragma unroll
+  for (int d = 0; d < OB; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+  int koff[QK_STEPS], voff[OB][2];
+#pragma unroll
+  for (int ks = 0; ks < QK_STEPS; ++ks) koff[ks] = tile_slot<DH>(l32, ks * 2 + g);
+  {
+    const int sl = lane & 15, hh = (lane >> 4) & 1, key = 4 * g + (sl >> 2);
+#pragma unroll
+    for (int db = 0; db < OB; ++db) {
+      const int dcol = 32 * db + 16 * hh + 4 * (sl & 3);  // first of the 4 dims this lane addresses
+      voff[db][0] = TILEB + tile_slot<DH>(key, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+      voff[db][1] = TILEB + tile_slot<DH>(key + 8, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+    }
+  }
+  f32x16_t s[2];  // s[kb][v]: key 32 kb + 8 (v / 4) + 4 g + v % 4, row l32
+  auto scores = [&](const unsigned char* st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      h8_t kf[QK_STEPS];
+#pragma unroll
+      for (int ks = 0; ks < QK_STEPS; ++ks) kf[ks] = *reinterpret_cast<const h8_t*>(st + koff[ks] + kb * 32 * ROWB);
+      const f32x16_t zero = {};
+      s[kb] = AttnFp16::mfma32(kf[0], qf[0], zero);
+#pragma unroll
+      for (int ks = 1; ks < QK_STEPS; ++ks) s[kb] = AttnFp16::mfma32(kf[ks], qf[ks], s[kb]);
+    }
+  };
+  auto finish = [&](const unsigned char* st, int t, auto masked) __attribute__((always_inline)) {
+    const int key0 = (tb + t) * kKeyTile;
+    if (decltype(masked)::value && key0 + kKeyTile > lim_wave) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (key0 + kb * 32 + 8 * (v >> 2) + 4 * g + (v & 3) >= lim) s[kb][v] = -INFINITY;
+    }
+    float mq[4];
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      mq[q4] = s[q4 >> 1][8 * (q4 & 1)];
+#pragma unroll
+      for (int v = 1; v < 8; ++v) mq[q4] = fmaxf(mq[q4], s[q4 >> 1][8 * (q4 & 1) + v]);
+    }
+    const float mx = xor32_max(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]))) * c;
+    const float m_new = softmax_ref_max(m_i, mx, 1.0f);
+    const float mc = ref_shift(m_new, 1.0f);
+    const float alpha = __builtin_amdgcn_exp2f(m_i - mc);
+    const float shift = kProbShift - mc;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_amdgcn_exp2f(fmaf(s[kb][v], c, shift));
+    h8_t pf[4];
+    float rs[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float tmp[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tmp[e] = s[j >> 1][8 * (j & 1) + e];
+      pf[j] = round8<AttnFp16>(tmp);
+      rs[j] = AttnFp16::sum8(pf[j], 0.0f);
+    }
+    l_i = l_i * alpha + xor32_sum((rs[0] + rs[1]) + (rs[2] + rs[3]));
+    m_i = m_new;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < OB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+    }
+#pragma unroll
+    for (int db = 0; db < OB; ++db)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const i16x8_t vt = join8(read_tr(st + voff[db][0] + j * 16 * ROWB), read_tr(st + voff[db][1] + j * 16 * ROWB));
+        o[db] = AttnFp16::mfma32(__builtin_bit_cast(h8_t, vt), pf[j], o[db]);
+      }
+  };
+
+  // Iteration t: barrier (tile t is in its stage, and every wave is done with tile t - 1's), first product of tile t, tile
+  // t + 1 into the other stage, loads of tile t + 2, softmax and second product of tile t. All waves of the workgroup
+  // pass the same barriers; waves without rows only load and expand.
+  if (ntiles > 0) {
+    Pieces x;
+    load(x, 0);
+    expand(x, smem);
+    if (ntiles > 1) load(x, 1);
+    auto pipeline = [&](auto work_c) __attribute__((always_inline)) {
+      constexpr bool WORK = decltype(work_c)::value;
+      auto step = [&](int t, auto masked) __attribute__((always_inline)) {
+        unsigned char* st = smem + (t & 1) * STAGE;
+        const bool sees = WORK && (!decltype(masked)::value || (tb + t) * kKeyTile < kend_wave);
+        block_barrier();
+        if (sees) scores(st);
+        if (t + 1 < ntiles) {
+          expand(x, smem + (~t & 1) * STAGE);
+          if (t + 2 < ntiles) load(x, t + 2);
+        }
+        if (sees) finish(st, t, masked);
+      };
+      int t = 0;
+      for (; t < min(nfull, ntiles); ++t) step(t, std::false_type{});
+      for (; t < ntiles; ++t) step(t, std::true_type{});
+    };
+    if (active) pipeline(std::true_type{});
+    else pipeline(std::false_type{});
+  }
+  if (bad && lim > 0) l_i = NAN;  // (its scores may all be -inf: 0 otherwise)
+
+  // O^T: lane l, register v of block db -> dim 32 db + 8 (v / 4) + 4 g + v % 4 of row l32.
+  if (!mine) return;
+  const float vts = na.c.ts[a.Hk + h];
+  const int orow = w.q0 + tok, ohead = h * a.G + head;
+  if (w.parts > 1) {
+    float* ws = a.ws + ((int64_t)item * a.Hk + h) * part_floats(R, DH);
+    const int r = row - r0;
+    if (g == 0) {
+      ws[r] = m_i;
+      ws[R + r] = l_i;
+    }
+    float* wo = ws + 2 * R + (int64_t)r * DH + 4 * g;
+#pragma unroll
+    for (int d = 0; d < OB; ++d)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4)
+        *reinterpret_cast<f32x4_t*>(wo + 32 * d + 8 * r4) =
+            f32x4_t{o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]} * vts;
+    return;
+  }
+  const float inv = l_i == 0.0f ? 0.0f : vts / l_i;
+  uint16_t* op = a.out + (int64_t)orow * a.o_rs + (int64_t)ohead * DH + 4 * g;
+#pragma unroll
+  for (int d = 0; d < OB; ++d)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const float y[8] = {o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv};
+      const uint4 b = E::from8(y);
+      *reinterpret_cast<uint2*>(op + 32 * d + 8 * r4) = make_uint2(b.x, b.y);
+    }
+}
+
 }  // namespace oudjat
 
 using namespace oudjat;
 
-static constexpr int kNvfp4Cus = 256;
+static constexpr int kNvfp4Cus = 256, kNvfp4KeysWaves = 4;
 
 // How a call is dealt, as packed_attention.hip's packed_shape.
 struct Nvfp4Shape {
-  int R, waves, target, min_tiles;
+  int R, target, min_tiles;
   bool search;
   int64_t items;
 };
 static Nvfp4Shape nvfp4_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, int64_t Dh, int64_t key_cap) {
   Nvfp4Shape s{};
   const int64_t G = Hq / Hk, seqs = std::max<int64_t>(1, std::min(S, rows));
-  s.R = 16;
-  s.min_tiles = 2;
+  const int64_t mean = cdiv(rows * G, seqs);  // packed rows of a sequence
+  s.R = mean <= 32 ? 16 : Dh == 128 && mean > 192 ? 256 : 128;
+  s.min_tiles = s.R == 16 ? 2 : 6;
   const int64_t tiles = std::max(rows * G / s.R, seqs);  // about as many as there are
-  s.waves = 4;
-  const int keys = 32 * s.waves;
-  if (tiles * Hk < 4 * kNvfp4Cus && key_cap > 2048) s.target = (int)cdiv(kNvfp4Cus, Hk);
+  const int keys = s.R == 16 ? 32 * kNvfp4KeysWaves : kKeyTile;  // of a key tile
+  const int64_t fill = s.R == 16 ? 4 * kNvfp4Cus : kNvfp4Cus;
+  if (tiles * Hk < fill && key_cap > 2048) s.target = (int)cdiv(kNvfp4Cus, Hk);
   s.search = S > 64 && !s.target && (S > kSortedSeqs || key_cap <= 2048);
   const int64_t most = rows * G / s.R + (s.search ? S : seqs), most_parts = cdiv(cdiv(key_cap, keys), s.min_tiles);
   s.items = s.target ? std::min(most + s.target + s.target / 16 + 1, most * most_parts) : most;
@@ -306,12 +536,27 @@ static int launch_nvfp4_keys(const Nvfp4Attn& a, hipStream_t st, const char* wha
   return check_launch(what);
 }
 
+template <class E, int DH, int W>
+static int launch_nvfp4_rows(const Nvfp4Attn& a, hipStream_t st, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int lds = 2 * 2 * kKeyTile * 2 * DH;
+  const int rc = allow_lds((const void*)nvfp4_attn_rows_kernel<E, DH, W>, lds, done, what);
+  if (rc != OUDJAT_OK) return rc;
+  nvfp4_attn_rows_kernel<E, DH, W><<<(unsigned)a.p.items * a.p.Hk, W * 64, lds, st>>>(a);
+  return check_launch(what);
+}
+
 template <class E, class A, int DH>
-static int launch_nvfp4(const Nvfp4Attn& a, const Nvfp4Shape& s, hipStream_t st, const char* what) {
-  const int rc = launch_nvfp4_keys<E, DH, 4>(a, st, what);
+static int launch_nvfp4(const Nvfp4Attn& a, int R, hipStream_t st, const char* what) {
+  constexpr int kHigh = DH == 128 ? 256 : 128;  // rows of the highest tile
+  const int rc = R == 16 ? launch_nvfp4_keys<E, DH, kNvfp4KeysWaves>(a, st, what)
+                 : R == 128 ? launch_nvfp4_rows<E, DH, 4>(a, st, what)
+                            : launch_nvfp4_rows<E, DH, kHigh / 32>(a, st, what);
   if (rc != OUDJAT_OK || !a.p.target) return rc;
-  const dim3 grid((unsigned)a.p.items * a.p.Hk, (unsigned)(s.R / merge_rows(s.R, DH)));
-  packed_attn_merge_kernel<A, DH, 16><<<grid, 256, 0, st>>>(a.p);
+  const dim3 grid((unsigned)a.p.items * a.p.Hk, (unsigned)(R / merge_rows(R, DH)));
+  if (R == 16) packed_attn_merge_kernel<A, DH, 16><<<grid, 256, 0, st>>>(a.p);
+  else if (R == 128) packed_attn_merge_kernel<A, DH, 128><<<grid, 256, 0, st>>>(a.p);
+  else packed_attn_merge_kernel<A, DH, kHigh><<<grid, 256, 0, st>>>(a.p);
   return check_launch("packed_attention_nvfp4 (merge)");
 }
 
@@ -364,8 +609,8 @@ extern "C" int oudjat_packed_attention_nvfp4(const uint16_t* q, int64_t q_rs, in
                     c, scale * 1.4426950408889634f};
   hipStream_t st = as_stream(stream);
   if (dtype == OUDJAT_BF16)
-    return Dh == 64 ? launch_nvfp4<ElemBf16, AttnBf16, 64>(a, s, st, what)
-                    : launch_nvfp4<ElemBf16, AttnBf16, 128>(a, s, st, what);
-  return Dh == 64 ? launch_nvfp4<ElemFp16, AttnFp16, 64>(a, s, st, what)
-                  : launch_nvfp4<ElemFp16, AttnFp16, 128>(a, s, st, what);
+    return Dh == 64 ? launch_nvfp4<ElemBf16, AttnBf16, 64>(a, s.R, st, what)
+                    : launch_nvfp4<ElemBf16, AttnBf16, 128>(a, s.R, st, what);
+  return Dh == 64 ? launch_nvfp4<ElemFp16, AttnFp16, 64>(a, s.R, st, what)
+                  : launch_nvfp4<ElemFp16, AttnFp16, 128>(a, s.R, st, what);
 }
