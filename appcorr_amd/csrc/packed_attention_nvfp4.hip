@@ -25,6 +25,20 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 
 static constexpr float kProbShift = 7.0f;
 
+// Byte of 16-byte chunk `chunk` of key row `row` in a tile. Dh = 128: the chunks of row r lie at chunk ^ swz(r), swz a
+// permutation of 0 .. 15 that puts four consecutive rows into four quarters of a row and the next four into the other
+// halves of these, so that 16 rows at one chunk (fragment reads of keys, writes), four rows at four chunks and eight rows at
+// two chunks (transposing reads of values for 32 and 16 dims) cover all banks.
+template <int DH>
+__device__ __forceinline__ int nv_slot(int row, int chunk) {
+  if constexpr (DH == 128) {
+    const int swz = ((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1);
+    return row * 2 * DH + ((chunk ^ swz) << 4);
+  } else {
+    return tile_slot<DH>(row, chunk);
+  }
+}
+
 // fp16 pair of 2^-8 e4m3(byte i of s), twice.
 __device__ __forceinline__ h2_t scale_pair(uint32_t s, int i) {
   return __builtin_bit_cast(h2_t, ((s >> (8 * i)) & 0x7fu) * 0x00800080u);
@@ -69,10 +83,13 @@ __device__ __forceinline__ float load_query(const uint16_t* p, int step, h8_t* q
 // turn; the waves' results meet in LDS at the end. A lane loads its piece of a key row (four lanes a row) and its
 // scales into registers, a tile ahead. Keys go from there to the first product (both of whose operands permute the
 // dims alike: lane group G has dims G Dh / 4 ..), values through LDS in fp16, from where the transposing reads take
-// them.
+// them. Bound by reading the cache where there are enough waves: 512 tokens over 1000 keys each, 32 over 8 heads of 128,
+// 121 us (4.9 TB/s, a copy's rate; over a 16-bit cache 370). About 250 VALU instructions a tile of 32 keys, half of them the
+// turning into fp16, are half of the SIMDs' cycles; a tile's chain (products, maximum, exponentials, products) is hidden
+// by four waves a SIMD, for which the registers are stated (three: 126 us, two: 147).
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void nvfp4_attn_keys_kernel(Nvfp4Attn na) {
+__global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_keys_kernel(Nvfp4Attn na) {
   constexpr int R = 16, KEYS = 32, QK_STEPS = DH / 32, DB = DH / 16, KT = WAVES * KEYS;
   constexpr int CW = DH / 32, ROWB = 2 * DH, CPR = DH / 8;  // a lane's words of codes
   const PackedAttn& a = na.p;
@@ -136,13 +153,11 @@ __global__ __launch_bounds__(WAVES * 64) void nvfp4_attn_keys_kernel(Nvfp4Attn n
     }
   };
 
-  int voff[DB][2];
-#pragma unroll
-  for (int db = 0; db < DB; ++db) {
-    const int dcol = 16 * db + 4 * (l16 & 3), key = 4 * G + (l16 >> 2);
-    voff[db][0] = tile_slot<DH>(key, dcol >> 3) + ((dcol >> 2) & 1) * 8;
-    voff[db][1] = tile_slot<DH>(key + 16, dcol >> 3) + ((dcol >> 2) & 1) * 8;
-  }
+  // This lane's bytes in the wave's tile (16 keys further on: 16 rows): where it writes, and where it reads 4 dims of a key.
+  const int put = nv_slot<DH>(l16, G * CW);
+  const int get = nv_slot<DH>(4 * G + (l16 >> 2), (l16 & 3) >> 1) + (l16 & 1) * 8;
+  // Chunk c of the same row: for aligned steps, the swizzle is an exclusive or.
+  auto step_of = [](int base, int c) { return base ^ (c << 4); };
 
   f32x4_t o[DB];
   float m_i = -INFINITY, l_i = 0.0f;
@@ -160,7 +175,7 @@ __global__ __launch_bounds__(WAVES * 64) void nvfp4_attn_keys_kernel(Nvfp4Attn n
         s[i] = AttnFp16::mfma16(xhat8(x.k[i][ks], scale_pair(x.ks[i], ks / 2)), qf[ks], s[i]);
 #pragma unroll
       for (int ks = 0; ks < QK_STEPS; ++ks)
-        *reinterpret_cast<h8_t*>(park16 + tile_slot<DH>(l16 + 16 * i, G * CW + ks)) =
+        *reinterpret_cast<h8_t*>(park16 + step_of(put, ks) + 16 * i * ROWB) =
             xhat8(x.v[i][ks], scale_pair(x.vs[i], ks / 2));
     }
     if (key0 + KEYS > lim_tile) {
@@ -188,20 +203,26 @@ __global__ __launch_bounds__(WAVES * 64) void nvfp4_attn_keys_kernel(Nvfp4Attn n
     }
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
-      const i16x8_t vt = join8(read_tr(park16 + voff[db][0]), read_tr(park16 + voff[db][1]));
+      const unsigned char* p = park16 + step_of(get, 2 * db);
+      const i16x8_t vt = join8(read_tr(p), read_tr(p + 16 * ROWB));
       o[db] = AttnFp16::mfma16(__builtin_bit_cast(h8_t, vt), pf, o[db]);
     }
   };
 
-  Tile x, y;
-  if (cnt > 0) load(x, 0);
+  constexpr int AHEAD = 1;  // tiles (two or three more in flight: 2 to 10 % slower, their registers cost more than they hide)
+  Tile x[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (i < cnt) load(x[i], i);
 #pragma unroll 1
-  for (int t = 0; t < cnt; t += 2) {
-    if (t + 1 < cnt) load(y, t + 1);
-    process(x, t);
-    if (t + 1 >= cnt) break;
-    if (t + 2 < cnt) load(x, t + 2);
-    process(y, t + 1);
+  for (int t0 = 0; t0 < cnt; t0 += AHEAD + 1) {
+#pragma unroll
+    for (int i = 0; i <= AHEAD; ++i) {
+      const int t = t0 + i;
+      if (t >= cnt) break;
+      if (t + AHEAD < cnt) load(x[(i + AHEAD) % (AHEAD + 1)], t + AHEAD);
+      process(x[i], t);
+    }
   }
   if (bad && lim > 0) l_i = NAN;  // (its scores may all be -inf: 0 otherwise)
 
@@ -330,7 +351,7 @@ __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na
   };
   int slot[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) slot[j] = tile_slot<DH>(pkey, 4 * pc + j) + (second ? TILEB : 0);
+  for (int j = 0; j < 4; ++j) slot[j] = nv_slot<DH>(pkey, 4 * pc + j) + (second ? TILEB : 0);
   auto expand = [&](const Pieces& x, unsigned char* st) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
@@ -349,14 +370,14 @@ __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na
     for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
   int koff[QK_STEPS], voff[OB][2];
 #pragma unroll
-  for (int ks = 0; ks < QK_STEPS; ++ks) koff[ks] = tile_slot<DH>(l32, ks * 2 + g);
+  for (int ks = 0; ks < QK_STEPS; ++ks) koff[ks] = nv_slot<DH>(l32, ks * 2 + g);
   {
     const int sl = lane & 15, hh = (lane >> 4) & 1, key = 4 * g + (sl >> 2);
 #pragma unroll
     for (int db = 0; db < OB; ++db) {
       const int dcol = 32 * db + 16 * hh + 4 * (sl & 3);  // first of the 4 dims this lane addresses
-      voff[db][0] = TILEB + tile_slot<DH>(key, dcol >> 3) + ((dcol >> 2) & 1) * 8;
-      voff[db][1] = TILEB + tile_slot<DH>(key + 8, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+      voff[db][0] = TILEB + nv_slot<DH>(key, dcol >> 3) + ((dcol >> 2) & 1) * 8;
+      voff[db][1] = TILEB + nv_slot<DH>(key + 8, dcol >> 3) + ((dcol >> 2) & 1) * 8;
     }
   }
   f32x16_t s[2];  // s[kb][v]: key 32 kb + 8 (v / 4) + 4 g + v % 4, row l32
@@ -490,11 +511,15 @@ __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na
 
 using namespace oudjat;
 
-static constexpr int kNvfp4Cus = 256, kNvfp4KeysWaves = 4;
+static constexpr int kNvfp4Cus = 256;
 
-// How a call is dealt, as packed_attention.hip's packed_shape.
+// How a call is dealt, as packed_attention.hip's packed_shape. Measured on one card, graphs of calls, us:
+// waves of the keys kernel: eight while there are at most two tiles for each CU and nothing is split (32 tokens over up to
+//   2000 keys, 32 over 8 heads of 128: 17.7 by eight, 21.3 by four; 64: 20.7, 22.6; 128: 38.9, 31.1).
+// target: four parts for each CU, whose waves are all that hides a tile's chain of steps (32 tokens over up to 16 k keys,
+//   32 over 8 heads of 128: 59 with one for each CU, 50 with two, 41 with four; 1 token 14.5, 15.5, 15.7). Rows kernel: one.
 struct Nvfp4Shape {
-  int R, target, min_tiles;
+  int R, waves, target, min_tiles;
   bool search;
   int64_t items;
 };
@@ -505,9 +530,10 @@ static Nvfp4Shape nvfp4_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, i
   s.R = mean <= 32 ? 16 : Dh == 128 && mean > 192 ? 256 : 128;
   s.min_tiles = s.R == 16 ? 2 : 6;
   const int64_t tiles = std::max(rows * G / s.R, seqs);  // about as many as there are
-  const int keys = s.R == 16 ? 32 * kNvfp4KeysWaves : kKeyTile;  // of a key tile
   const int64_t fill = s.R == 16 ? 4 * kNvfp4Cus : kNvfp4Cus;
-  if (tiles * Hk < fill && key_cap > 2048) s.target = (int)cdiv(kNvfp4Cus, Hk);
+  if (tiles * Hk < fill && key_cap > 2048) s.target = (int)cdiv(fill, Hk);
+  s.waves = !s.target && tiles * Hk <= 2 * kNvfp4Cus ? 8 : 4;
+  const int keys = s.R == 16 ? 32 * s.waves : kKeyTile;  // of a key tile
   s.search = S > 64 && !s.target && (S > kSortedSeqs || key_cap <= 2048);
   const int64_t most = rows * G / s.R + (s.search ? S : seqs), most_parts = cdiv(cdiv(key_cap, keys), s.min_tiles);
   s.items = s.target ? std::min(most + s.target + s.target / 16 + 1, most * most_parts) : most;
@@ -547,9 +573,9 @@ static int launch_nvfp4_rows(const Nvfp4Attn& a, hipStream_t st, const char* wha
 }
 
 template <class E, class A, int DH>
-static int launch_nvfp4(const Nvfp4Attn& a, int R, hipStream_t st, const char* what) {
+static int launch_nvfp4(const Nvfp4Attn& a, int R, int waves, hipStream_t st, const char* what) {
   constexpr int kHigh = DH == 128 ? 256 : 128;  // rows of the highest tile
-  const int rc = R == 16 ? launch_nvfp4_keys<E, DH, kNvfp4KeysWaves>(a, st, what)
+  const int rc = R == 16    ? (waves == 8 ? launch_nvfp4_keys<E, DH, 8>(a, st, what) : launch_nvfp4_keys<E, DH, 4>(a, st, what))
                  : R == 128 ? launch_nvfp4_rows<E, DH, 4>(a, st, what)
                             : launch_nvfp4_rows<E, DH, kHigh / 32>(a, st, what);
   if (rc != OUDJAT_OK || !a.p.target) return rc;
@@ -609,8 +635,8 @@ extern "C" int oudjat_packed_attention_nvfp4(const uint16_t* q, int64_t q_rs, in
                     c, scale * 1.4426950408889634f};
   hipStream_t st = as_stream(stream);
   if (dtype == OUDJAT_BF16)
-    return Dh == 64 ? launch_nvfp4<ElemBf16, AttnBf16, 64>(a, s.R, st, what)
-                    : launch_nvfp4<ElemBf16, AttnBf16, 128>(a, s.R, st, what);
-  return Dh == 64 ? launch_nvfp4<ElemFp16, AttnFp16, 64>(a, s.R, st, what)
-                  : launch_nvfp4<ElemFp16, AttnFp16, 128>(a, s.R, st, what);
+    return Dh == 64 ? launch_nvfp4<ElemBf16, AttnBf16, 64>(a, s.R, s.waves, st, what)
+                    : launch_nvfp4<ElemBf16, AttnBf16, 128>(a, s.R, s.waves, st, what);
+  return Dh == 64 ? launch_nvfp4<ElemFp16, AttnFp16, 64>(a, s.R, s.waves, st, what)
+                  : launch_nvfp4<ElemFp16, AttnFp16, 128>(a, s.R, s.waves, st, what);
 }

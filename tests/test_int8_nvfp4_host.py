@@ -207,3 +207,11 @@ def test_every_kernel_of_the_library_is_one_that_a_call_takes():
     assert {t[1:] for t in tiles} == {(64, 64, 2, 2, 4), (64, 128, 2, 4, 3), (128, 128, 2, 2, 2), (192, 256, 2, 4, 2),
                                       (256, 256, 2, 4, 2)}
     assert {t[0] for t in tiles} == {_lib.EPI_BIAS, _lib.EPI_BIAS_LS, _lib.EPI_BIAS_LS_RESID, _lib.EPI_BIAS_SILU_MUL}
+
+    def attention(kernel):
+        found = re.findall(kernel + rb"INS_8Elem(Bf16|Fp16)E((?:Li\d+E)+)E", blob)
+        return {(e.decode(), *map(int, re.findall(rb"\d+", n))) for e, n in found}
+
+    both = [(e,) for e in ("Bf16", "Fp16")]
+    assert attention(rb"nvfp4_attn_keys_kernel") == {(*e, d, w) for e in both for d in (64, 128) for w in (4, 8)}
+    assert attention(rb"nvfp4_attn_rows_kernel") == {(*e, d, w) for e in both for d, w in ((64, 4), (128, 4), (128, 8))}
