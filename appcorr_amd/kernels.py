@@ -1584,17 +1584,17 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale NaN and codes 0, so that its products are NaN. The activations of linear_int8, or its weight [N, K] (a scale for
     each output channel). K a multiple of 16, rows contiguous and 16-byte aligned."""
     dev = _gpu_of(x)
-    kind = _DTYPES.get(x.dtype)
-    _require(kind is not None and x.dim() >= 1, "quantize_int8: [.., K] bf16 or fp16")
-    K = x.shape[-1]
+    kind, shape = _DTYPES.get(x.dtype), x.shape
+    _require(kind is not None and len(shape) >= 1, "quantize_int8: [.., K] bf16 or fp16")
+    K = shape[-1]
     _require(x.stride(-1) == 1 or K <= 1, "quantize_int8: rows must be contiguous")
-    codes = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    codes = x.new_empty(shape, dtype=torch.int8)
+    scale = x.new_empty(shape[:-1], dtype=torch.float32)
     rows = scale.numel()
     if rows:
-        x2 = x.reshape(rows, K)
-        _launch_on("quantize_int8", dev, x, "oudjat_quantize_int8", x2.data_ptr(), rows, K, *_strides(x2, 1), kind,
-                   codes.data_ptr(), K, scale.data_ptr(), _lib.stream_of(x))
+        x2 = x if len(shape) == 2 else x.reshape(rows, K)
+        _launch_on("quantize_int8", dev, x, "oudjat_quantize_int8", x2.data_ptr(), rows, K, 0 if rows == 1 else x2.stride(0),
+                   kind, codes.data_ptr(), K, scale.data_ptr(), _lib.stream_of(x))
     return codes, scale
 
 
@@ -1607,33 +1607,37 @@ def linear_int8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_sca
     EPI_BIAS_LS_RESID (resid + y * gamma), EPI_BIAS_SILU_MUL (silu(y) * resid). bias, gamma [N] and resid [.., N] of that
     type; `out` may be resid but not overlap itself. K a multiple of 64 below 131072, N of 8."""
     dev = _gpu_of(x8, x_scale, w8, w_scale, bias, gamma, resid, out)
-    kind = _DTYPES.get(dtype)
+    kind, xs, ws = _DTYPES.get(dtype), x8.shape, w8.shape
     _require(kind is not None, "linear_int8: dtype must be bf16 or fp16")
-    _require(x8.dtype == w8.dtype == torch.int8 and x8.dim() >= 1 and w8.dim() == 2 and w8.shape[1] == x8.shape[-1],
+    _require(x8.dtype == w8.dtype == torch.int8 and len(ws) == 2 and len(xs) >= 1 and xs[-1] == ws[1],
              "linear_int8: int8 codes x8 [.., K] and w8 [N, K]")
-    N, Kd = w8.shape
-    _require(x_scale.shape == x8.shape[:-1] and w_scale.shape == (N,) and x_scale.dtype == w_scale.dtype == torch.float32,
+    N, Kd = ws
+    shape = (*xs[:-1], N)
+    _require(x_scale.shape == xs[:-1] and w_scale.shape == (N,) and x_scale.dtype == w_scale.dtype == torch.float32,
              "linear_int8: fp32 scales x_scale [..] and w_scale [N]")
-    M = x_scale.numel()
-    x2 = x8.reshape(M, Kd)
-    _require((x2.stride(1) == 1 and w8.stride(1) == 1) or Kd <= 1, "linear_int8: rows must be contiguous")
-    for t, name in ((bias, "bias"), (gamma, "gamma")):
-        _require(t is None or (t.shape == (N,) and t.dtype == dtype), f"linear_int8: {name} must be [N] of the output's type")
-    shape = (*x8.shape[:-1], N)
-    for t, name in ((resid, "resid"), (out, "out")):
-        _require(t is None or (t.shape == shape and t.dtype == dtype and (t.stride(-1) == 1 or N <= 1)),
-                 f"linear_int8: {name} must be [.., N] of the output's type with contiguous rows")
     if out is None:
-        out = torch.empty(shape, device=x8.device, dtype=dtype)
-    o2 = out.view(M, N)
-    r2 = None if resid is None else resid.reshape(M, N)
+        out = x8.new_empty(shape, dtype=dtype)
+    else:
+        _require(out.shape == shape and out.dtype == dtype and (out.stride(-1) == 1 or N <= 1),
+                 "linear_int8: out must be [.., N] of the output's type with contiguous rows")
+    _require(bias is None or (bias.shape == (N,) and bias.dtype == dtype), "linear_int8: bias must be [N] of the output's type")
+    _require(gamma is None or (gamma.shape == (N,) and gamma.dtype == dtype),
+             "linear_int8: gamma must be [N] of the output's type")
+    _require(resid is None or (resid.shape == shape and resid.dtype == dtype and (resid.stride(-1) == 1 or N <= 1)),
+             "linear_int8: resid must be [.., N] of the output's type with contiguous rows")
+    M = x_scale.numel()
+    x2, o2, r2 = x8, out, resid
+    if len(xs) != 2:
+        x2, o2, r2 = x8.reshape(M, Kd), out.view(M, N), None if resid is None else resid.reshape(M, N)
+    _require((x2.stride(1) == 1 and w8.stride(1) == 1) or Kd <= 1, "linear_int8: rows must be contiguous")
     sx, sw = x_scale.contiguous(), w_scale.contiguous()
     b = None if bias is None else bias.contiguous()
     g = None if gamma is None else gamma.contiguous()
-    _launch_on(site, dev, x8, "oudjat_linear_int8", x2.data_ptr(), M, Kd, *_strides(x2, 1), sx.data_ptr(), w8.data_ptr(), N,
-               *_strides(w8, 1), sw.data_ptr(), 0 if b is None else b.data_ptr(), int(epilogue),
+    _launch_on(site, dev, x8, "oudjat_linear_int8", x2.data_ptr(), M, Kd, 0 if M == 1 else x2.stride(0), sx.data_ptr(),
+               w8.data_ptr(), N, 0 if N == 1 else w8.stride(0), sw.data_ptr(), 0 if b is None else b.data_ptr(), int(epilogue),
                0 if g is None else g.data_ptr(), 0 if r2 is None else r2.data_ptr(),
-               0 if r2 is None else _strides(r2, 1)[0], o2.data_ptr(), *_strides(o2, 1), kind, _lib.stream_of(x8))
+               0 if r2 is None or M == 1 else r2.stride(0), o2.data_ptr(), 0 if M == 1 else o2.stride(0), kind,
+               _lib.stream_of(x8))
     return out
 
 
@@ -1666,17 +1670,21 @@ def kv_nvfp4_cache(batches: int, cache_len: int, kv_heads: int, head_dim: int, d
     return KvNvfp4(codes.permute(0, 3, 1, 2, 4), scales.view(torch.float8_e4m3fn).permute(0, 3, 1, 2, 4), tensor_scale)
 
 
-def _kv_nvfp4_args(cache: KvNvfp4, Hk: int, Dh: int, what: str) -> tuple:
+_SCALE_TYPES = (torch.float8_e4m3fn, torch.uint8)
+_CACHE_SHAPES = "an NVFP4 cache has codes uint8 [B, N, 2, Hk, Dh / 2] and scales e4m3 [B, N, 2, Hk, Dh / 16]"
+
+
+def _kv_nvfp4_args(cache: KvNvfp4, Hk: int, Dh: int) -> tuple:
     """(addresses and strides as the C entries take them) of a cache of Hk heads of Dh."""
     codes, scales, ts = cache.codes, cache.scales, cache.tensor_scale
-    cs, ss = codes.shape, scales.shape
-    _require(len(cs) == 5 and cs == (cs[0], cs[1], 2, Hk, Dh // 2) and ss == (cs[0], cs[1], 2, Hk, Dh // 16)
-             and codes.dtype == torch.uint8 and scales.dtype in (torch.float8_e4m3fn, torch.uint8)
-             and codes.stride(4) == 1 and scales.stride(4) == 1,
-             f"{what}: the cache must be codes uint8 [B, N, 2, Hk, Dh / 2] and scales e4m3 [B, N, 2, Hk, Dh / 16]")
+    cs, ss, cst, sst = codes.shape, scales.shape, codes.stride(), scales.stride()
+    _require(len(cs) == 5 and cs[2:] == (2, Hk, Dh // 2) and ss == (cs[0], cs[1], 2, Hk, Dh // 16)
+             and codes.dtype == torch.uint8 and scales.dtype in _SCALE_TYPES and cst[4] == 1 and sst[4] == 1, _CACHE_SHAPES)
     _require(ts.shape == (2, Hk) and ts.dtype == torch.float32 and ts.is_contiguous(),
-             f"{what}: tensor_scale must be contiguous fp32 [2, Hk]")
-    return (codes.data_ptr(), *_strides(codes, 4), scales.data_ptr(), *_strides(scales, 4), ts.data_ptr())
+             "tensor_scale must be contiguous fp32 [2, Hk]")
+    if 1 in cs:
+        cst, sst = _strides(codes, 4), _strides(scales, 4)
+    return (codes.data_ptr(), cst[0], cst[1], cst[2], cst[3], scales.data_ptr(), sst[0], sst[1], sst[2], sst[3], ts.data_ptr())
 
 
 def kv_nvfp4_write(k: torch.Tensor, v: torch.Tensor, batch_idx: torch.Tensor, token_idx: torch.Tensor,
@@ -1694,7 +1702,7 @@ def kv_nvfp4_write(k: torch.Tensor, v: torch.Tensor, batch_idx: torch.Tensor, to
     M, Hk, Dh = shape
     bi, ti = _index(batch_idx, "batch_idx"), _index(token_idx, "token_idx")
     _require(bi.shape == (M,) and ti.shape == (M,), "kv_nvfp4_write: one slot per row")
-    c = _kv_nvfp4_args(cache, Hk, Dh, "kv_nvfp4_write")
+    c = _kv_nvfp4_args(cache, Hk, Dh)
     _launch_on("kv_nvfp4_write", dev, k, "oudjat_kv_nvfp4_write", k.data_ptr(), *_strides(k, 2), v.data_ptr(),
                *_strides(v, 2), M, Hk, Dh, kind, bi.data_ptr(), ti.data_ptr(), *c, *cache.codes.shape[:2],
                _lib.stream_of(k))
@@ -1711,9 +1719,9 @@ def kv_nvfp4_read(cache: KvNvfp4, batch_idx: torch.Tensor, token_idx: torch.Tens
     bi, ti = _index(batch_idx, "batch_idx"), _index(token_idx, "token_idx")
     M = bi.shape[0]
     _require(ti.shape == (M,), "kv_nvfp4_read: batch_idx and token_idx of one length")
-    c = _kv_nvfp4_args(cache, Hk, 2 * half, "kv_nvfp4_read")
-    k = torch.empty((M, Hk, 2 * half), device=bi.device, dtype=dtype)
-    v = torch.empty((M, Hk, 2 * half), device=bi.device, dtype=dtype)
+    c = _kv_nvfp4_args(cache, Hk, 2 * half)
+    k = cache.codes.new_empty((M, Hk, 2 * half), dtype=dtype)
+    v = cache.codes.new_empty((M, Hk, 2 * half), dtype=dtype)
     _launch_on("kv_nvfp4_read", dev, bi, "oudjat_kv_nvfp4_read", *c, B, N, Hk, 2 * half, bi.data_ptr(), ti.data_ptr(), M,
                kind, k.data_ptr(), v.data_ptr(), _lib.stream_of(bi))
     return k, v
@@ -1738,10 +1746,10 @@ def packed_attention_nvfp4(q: torch.Tensor, cache: KvNvfp4, cu_q: torch.Tensor, 
              "packed_attention_nvfp4: q [M, Hq, Dh] bf16 or fp16 with contiguous heads, and a cache")
     M, Hq, Dh = qs
     B, cap, _, Hk, _ = cache.codes.shape
-    c = _kv_nvfp4_args(cache, Hk, Dh, "packed_attention_nvfp4")
+    c = _kv_nvfp4_args(cache, Hk, Dh)
     if out is None:
         dev = _gpu_of(q, cache.codes, cache.scales, cache.tensor_scale, cu_q, k_lens)
-        out = torch.empty((M, Hq * Dh), device=q.device, dtype=dtype)
+        out = q.new_empty((M, Hq * Dh))
     else:
         dev = _gpu_of(q, cache.codes, cache.scales, cache.tensor_scale, cu_q, k_lens, out)
         _require(out.shape == (M, Hq * Dh) and out.dtype == dtype and out.stride(1) == 1,
