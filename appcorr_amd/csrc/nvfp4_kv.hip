@@ -14,89 +14,146 @@
 
 namespace oudjat {
 
-static constexpr int kKvThreads = 256;
+static constexpr int kKvThreads = 256, kReadItems = 2;
 
-// Write. An item is half a block, 8 dims (16 bytes in, 4 out): the wave reads and writes consecutive pieces of a row, the
-// two lanes of a block exchange their maxima, and one lane in eight stores four scales. A workgroup takes `per_wg`
-// rows.
+// Reciprocal of a normal b whose reciprocal is normal too: one Newton step on the hardware's, which is within an ulp, gives
+// the correctly rounded one (a significand of all ones aside).
+__device__ __forceinline__ float rcp_rn(float b) {
+  const float y = __builtin_amdgcn_rcpf(b);
+  return __builtin_fmaf(__builtin_fmaf(-b, y, 1.0f), y, y);
+}
+// a / b correctly rounded, y = RN(1 / b), where nothing leaves the normal range: a - q0 b is exact.
+__device__ __forceinline__ float quotient(float a, float b, float y) {
+  const float q0 = a * y;
+  return __builtin_fmaf(__builtin_fmaf(-q0, b, a), y, q0);
+}
+
+// A block's scale byte and codes. The usual block is finite, its values and the tensor scale are of ordinary size, and the
+// scale is neither cut off nor rounded to 0; any other takes IEEE divisions and the limits that the format needs.
+template <class E>
+__device__ __forceinline__ uint2 quantize_block(const uint4& lo, const uint4& hi, float ts, uint32_t& s8) {
+  float f[16];
+  E::to8(lo, f);
+  E::to8(hi, f + 8);
+  float am = 0.0f, z = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    am = fmaxf(am, fabsf(f[e]));
+    z = __builtin_fmaf(f[e], 0.0f, z);  // NaN if any value is not finite
+  }
+  const float scaled = quotient(quotient(am, kE2m1Max, 1.0f / kE2m1Max), ts, rcp_rn(ts));
+  if (__builtin_expect(z == 0.0f && am > 1e-18f && ts > 1e-18f && ts < 1e18f && scaled > 0.001f && scaled <= kE4m3Max, 1)) {
+    s8 = e4m3_encode_pos(scaled);
+    const float unit = ts * e4m3_decode(s8), y = rcp_rn(unit);
+    return make_uint2(nvfp4_codes8(f, unit, y), nvfp4_codes8(f + 8, unit, y));
+  }
+  am = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    f[e] = f[e] == f[e] ? f[e] : 0.0f;
+    am = fmaxf(am, fabsf(f[e]));
+  }
+  float unit;
+  nvfp4_block_scale(am, ts, s8, unit);
+  if (!s8) return make_uint2(0, 0);
+  // (values past 8 units saturate all the same, and their quotients stay finite)
+  const float most = 8.0f * unit, y = 1.0f / unit;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) f[e] = fminf(fmaxf(f[e], -most), most);
+  return make_uint2(nvfp4_codes8(f, unit, y), nvfp4_codes8(f + 8, unit, y));
+}
+
+// Write. An item is a block, 16 dims of a head: the wave reads and writes consecutive pieces of a row, and one lane in four
+// stores four scales. A workgroup takes `per_wg` rows.
 template <class E>
 __global__ __launch_bounds__(kKvThreads) void kv_nvfp4_write_kernel(
     const uint16_t* __restrict__ k, int64_t k_rs, int64_t k_hs, const uint16_t* __restrict__ v, int64_t v_rs,
-    int64_t v_hs, int64_t rows, int dims8, Divisor by_row, Divisor by_head, const int64_t* __restrict__ batch_idx,
+    int64_t v_hs, int64_t rows, int blocks, Divisor by_row, Divisor by_head, const int64_t* __restrict__ batch_idx,
     const int64_t* __restrict__ token_idx, KvNvfp4 c, int per_wg) {
   const int64_t row0 = (int64_t)blockIdx.x * per_wg;
-  const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * dims8;
+  const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * blocks;
   for (int i = threadIdx.x; i < n * per_row; i += kKvThreads) {
     const int r = by_row(i), j = i - r * per_row;
-    const int kh = by_head(j), d8 = j - kh * dims8;  // key heads, then value heads; 8 dims
+    const int kh = by_head(j), d16 = j - kh * blocks;  // key heads, then value heads; 16 dims
     const bool val = kh >= c.Hk;
     const int h = val ? kh - c.Hk : kh;
     const int64_t row = row0 + r;
-    float f[8];
-    E::to8(load16((val ? v + row * v_rs + h * v_hs : k + row * k_rs + h * k_hs) + 8 * d8), f);
+    const uint16_t* src = (val ? v + row * v_rs + h * v_hs : k + row * k_rs + h * k_hs) + 16 * d16;
+    const uint4 lo = load16(src), hi = load16(src + 8);
     const int64_t b = batch_idx[row], t = token_idx[row];
-    const float ts = c.ts[kh];
-    float am = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f[e] = f[e] == f[e] ? f[e] : 0.0f;
-      am = fmaxf(am, fabsf(f[e]));
-    }
-    am = fmaxf(am, __shfl_xor(am, 1, 64));
     uint32_t s8;
-    float unit;
-    nvfp4_block_scale(am, ts, s8, unit);
-    // (values past 8 units saturate all the same, and their quotients stay finite)
-    const float most = 8.0f * unit;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fminf(fmaxf(f[e], -most), most);
-    const uint32_t word = s8 ? nvfp4_codes8(f, unit, 1.0f / unit) : 0u;
-    // Four blocks' scales into one word: lanes 8 apart hold those of the next four.
-    uint32_t four = s8 << (8 * ((d8 >> 1) & 3));
+    const uint2 codes = quantize_block<E>(lo, hi, c.ts[kh], s8);
+    uint32_t four = s8 << (8 * (d16 & 3));  // four blocks' scales into one word
+    four |= __shfl_xor(four, 1, 64);
     four |= __shfl_xor(four, 2, 64);
-    four |= __shfl_xor(four, 4, 64);
     if (b < 0 || b >= c.B || t < 0 || t >= c.N) continue;
-    *reinterpret_cast<uint32_t*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 4 * d8) = word;
-    if ((d8 & 7) == 0)
-      *reinterpret_cast<uint32_t*>(c.scales + b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d8 / 2) = four;
+    *reinterpret_cast<uint2*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 8 * d16) = codes;
+    if ((d16 & 3) == 0)
+      *reinterpret_cast<uint32_t*>(c.scales + b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d16) = four;
   }
 }
 
-// Read. An item is 8 dims: 4 bytes of codes and a scale byte in, 16 bytes out.
-template <class E>
-__global__ __launch_bounds__(kKvThreads) void kv_nvfp4_read_kernel(KvNvfp4 c, int dims8, Divisor by_row, Divisor by_head,
+// Read. An item is a block: 8 bytes of codes and a scale byte in, 32 bytes out; a thread has the loads of U in flight.
+template <class E, int U>
+__global__ __launch_bounds__(kKvThreads) void kv_nvfp4_read_kernel(KvNvfp4 c, int blocks, Divisor by_row, Divisor by_head,
                                                                    const int64_t* __restrict__ batch_idx,
                                                                    const int64_t* __restrict__ token_idx, int64_t rows,
                                                                    uint16_t* __restrict__ k_out,
                                                                    uint16_t* __restrict__ v_out, int per_wg) {
   const int64_t row0 = (int64_t)blockIdx.x * per_wg;
-  const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * dims8;
-  for (int i = threadIdx.x; i < n * per_row; i += kKvThreads) {
-    const int r = by_row(i), j = i - r * per_row;
-    const int kh = by_head(j), d8 = j - kh * dims8;
-    const bool val = kh >= c.Hk;
-    const int h = val ? kh - c.Hk : kh;
-    const int64_t row = row0 + r, b = batch_idx[row], t = token_idx[row];
-    float f[8] = {};
-    if (b >= 0 && b < c.B && t >= 0 && t < c.N) {
-      const uint32_t w =
-          *reinterpret_cast<const uint32_t*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 4 * d8);
-      const uint32_t s8 = c.scales[b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d8 / 2];
-      const float s = e4m3_decode(s8 & 0x7f), ts = c.ts[kh];
-      const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
-      const auto v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
-      const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2);
-      const auto v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
-      const float e2[8] = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+  const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * blocks;
+  for (int i0 = threadIdx.x; i0 < n * per_row; i0 += U * kKvThreads) {
+    uint2 w[U];
+    uint32_t s8[U];
+    uint16_t* dst[U];
+    float ts[U];
+    bool there[U], slot[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = (e2[e] * s) * ts;  // (the first product is exact)
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kKvThreads;
+      there[u] = i < n * per_row;
+      const int r = by_row(there[u] ? i : i0), j = (there[u] ? i : i0) - r * per_row;
+      const int kh = by_head(j), d16 = j - kh * blocks;
+      const bool val = kh >= c.Hk;
+      const int h = val ? kh - c.Hk : kh;
+      const int64_t row = row0 + r, b = batch_idx[row], t = token_idx[row];
+      slot[u] = b >= 0 && b < c.B && t >= 0 && t < c.N;
+      w[u] = make_uint2(0, 0);
+      s8[u] = 0;
+      if (slot[u]) {
+        w[u] = *reinterpret_cast<const uint2*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 8 * d16);
+        s8[u] = c.scales[b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d16];
+      }
+      ts[u] = c.ts[kh];
+      dst[u] = (val ? v_out : k_out) + (row * c.Hk + h) * (16 * blocks) + 16 * d16;
     }
-    store16((val ? v_out : k_out) + (row * c.Hk + h) * (8 * dims8) + 8 * d8, E::from8(f));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!there[u]) continue;
+      const float s = e4m3_decode(s8[u] & 0x7f);
+      float f[16];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t x = half ? w[u].y : w[u].x;
+        const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 0);
+        const auto v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 1);
+        const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 2);
+        const auto v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 3);
+        const float e2[8] = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[8 * half + e] = (e2[e] * s) * ts[u];  // (the first product is exact)
+      }
+      if (!slot[u])
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = 0.0f;
+      store16(dst[u], E::from8(f));
+      store16(dst[u] + 8, E::from8(f + 8));
+    }
   }
 }
 
-// Rows of a workgroup: about 1024 items, four a thread.
-static int kv_rows_per_wg(int64_t per_row) { return (int)std::max<int64_t>(1, 1024 / per_row); }
+// Rows of a workgroup: about `each` items a thread.
+static int kv_rows_per_wg(int64_t per_row, int each) { return (int)std::max<int64_t>(1, each * kKvThreads / per_row); }
 
 int check_kv_nvfp4(const KvNvfp4& c, int64_t Dh, const char* what) {
   OUDJAT_REQUIRE(c.bs >= 0 && c.ns >= 0 && c.cs >= 0 && c.hs >= 0 && c.sbs >= 0 && c.sns >= 0 && c.scs >= 0 && c.shs >= 0,
@@ -137,13 +194,13 @@ extern "C" int oudjat_kv_nvfp4_write(const uint16_t* k, int64_t k_rs, int64_t k_
   OUDJAT_REQUIRE(entries_apart({{B, c_bs}, {N, c_ns}, {2, c_cs}, {Hk, c_hs}}, Dh / 2) &&
                      entries_apart({{B, s_bs}, {N, s_ns}, {2, s_cs}, {Hk, s_hs}}, Dh / 16),
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: the rows of the cache must not overlap", what);
-  const int64_t per_row = 2 * Hk * Dh / 8;
-  const int per = kv_rows_per_wg(per_row);
+  const int64_t per_row = 2 * Hk * Dh / 16;
+  const int per = kv_rows_per_wg(per_row, 2);
   OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   if (empty) return OUDJAT_OK;
   auto go = [&](auto e) {
     kv_nvfp4_write_kernel<decltype(e)><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
-        k, k_rs, k_hs, v, v_rs, v_hs, rows, (int)(Dh / 8), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 8)),
+        k, k_rs, k_hs, v, v_rs, v_hs, rows, (int)(Dh / 16), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 16)),
         batch_idx, token_idx, c, per);
   };
   if (dtype == OUDJAT_BF16) go(ElemBf16{});
@@ -172,12 +229,12 @@ extern "C" int oudjat_kv_nvfp4_read(const uint8_t* codes, int64_t c_bs, int64_t 
   if (rc != OUDJAT_OK) return rc;
   OUDJAT_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16) && aligned(batch_idx, 8) && aligned(token_idx, 8),
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned outputs required", what);
-  const int64_t per_row = 2 * Hk * Dh / 8;
-  const int per = kv_rows_per_wg(per_row);
+  const int64_t per_row = 2 * Hk * Dh / 16;
+  const int per = kv_rows_per_wg(per_row, kReadItems);
   OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   auto go = [&](auto e) {
-    kv_nvfp4_read_kernel<decltype(e)><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
-        c, (int)(Dh / 8), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 8)), batch_idx, token_idx, rows, k_out,
+    kv_nvfp4_read_kernel<decltype(e), kReadItems><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
+        c, (int)(Dh / 16), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 16)), batch_idx, token_idx, rows, k_out,
         v_out, per);
   };
   if (dtype == OUDJAT_BF16) go(ElemBf16{});
