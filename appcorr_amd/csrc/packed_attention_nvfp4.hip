@@ -283,7 +283,11 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_key
 // K . Q^T and O^T += V^T . P^T on v_mfma_f32_32x32x16 as in packed_attention.hip: a row is one lane pair (l, l ^ 32), whose
 // registers hold its scores. A thread turns pieces of 32 dims (16 bytes of codes, two scales) into fp16 once for the
 // workgroup; a piece is loaded two tiles ahead and written one tile ahead, between the first product and the softmax of
-// the tile before. 16 lanes write the same dims of 16 keys, which covers all banks.
+// the tile before. 16 lanes write the same dims of 16 keys, which covers all banks. Bound by the softmax's VALU work (its
+// exponentials alone are half of it) and the matrix cores, as over a 16-bit cache: one prompt of 8192 tokens, 32 over 8
+// heads of 128, 542 us (1015 TF/s); of 4101, 16 heads of 64, 71 us, where 528 workgroups of different lengths leave CUs
+// idle at the end (every other round of them backwards: 8 % faster to 10 % slower by the lengths). A block's
+// fragments all read before its products: the same at 64 dims, 4 % slower at 128.
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int W>
 __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na) {
@@ -516,8 +520,11 @@ static constexpr int kNvfp4Cus = 256;
 // How a call is dealt, as packed_attention.hip's packed_shape. Measured on one card, graphs of calls, us:
 // waves of the keys kernel: eight while there are at most two tiles for each CU and nothing is split (32 tokens over up to
 //   2000 keys, 32 over 8 heads of 128: 17.7 by eight, 21.3 by four; 64: 20.7, 22.6; 128: 38.9, 31.1).
-// target: four parts for each CU, whose waves are all that hides a tile's chain of steps (32 tokens over up to 16 k keys,
-//   32 over 8 heads of 128: 59 with one for each CU, 50 with two, 41 with four; 1 token 14.5, 15.5, 15.7). Rows kernel: one.
+// target: keys are split while there are fewer than four tiles for each CU. Parts for each CU, keys kernel: four, whose waves
+//   are all that hides a tile's chain of steps (32 tokens over up to 16 k keys, 32 over 8 heads of 128: 59 with one, 50 with
+//   two, 41 with four; 1 token 14.5, 15.5, 15.7). Tiles of 256 rows, one workgroup on a CU: one (512 rows over 8 k keys, 32 over
+//   8 heads: 85, with two 102); of 128 rows: two (8 x 512 rows over up to 8 k keys, 16 heads of 64: 82 with one, 70 with two,
+//   129 unsplit; as many keys for all: 101 split, 99 not). 8 x 256 rows over up to 8 k keys, 32 over 8 heads: 106, 243 unsplit.
 struct Nvfp4Shape {
   int R, waves, target, min_tiles;
   bool search;
@@ -530,8 +537,8 @@ static Nvfp4Shape nvfp4_shape(int64_t rows, int64_t S, int64_t Hq, int64_t Hk, i
   s.R = mean <= 32 ? 16 : Dh == 128 && mean > 192 ? 256 : 128;
   s.min_tiles = s.R == 16 ? 2 : 6;
   const int64_t tiles = std::max(rows * G / s.R, seqs);  // about as many as there are
-  const int64_t fill = s.R == 16 ? 4 * kNvfp4Cus : kNvfp4Cus;
-  if (tiles * Hk < fill && key_cap > 2048) s.target = (int)cdiv(fill, Hk);
+  const int64_t parts = s.R == 16 ? 4 : s.R == 128 ? 2 : 1;  // for each CU
+  if (tiles * Hk < 4 * kNvfp4Cus && key_cap > 2048) s.target = (int)cdiv(parts * kNvfp4Cus, Hk);
   s.waves = !s.target && tiles * Hk <= 2 * kNvfp4Cus ? 8 : 4;
   const int keys = s.R == 16 ? 32 * s.waves : kKeyTile;  // of a key tile
   s.search = S > 64 && !s.target && (S > kSortedSeqs || key_cap <= 2048);
