@@ -66,6 +66,8 @@ struct QuantFp16 : ElemFp16 {
   static __device__ __forceinline__ float value(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
 };
 
+static constexpr int kWaveRow = 1024;  // the longest row of one wave
+
 template <class E, int LANES, int CH, bool LONG>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(const uint16_t* __restrict__ x, int64_t rows, int K,
                                                             int64_t x_rs, int8_t* __restrict__ codes, int64_t c_rs,
@@ -441,7 +443,8 @@ extern "C" int oudjat_quantize_int8(const uint16_t* x, int64_t rows, int64_t K, 
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned rows required", what);
   OUDJAT_REQUIRE(entries_apart({{rows, c_rs}}, K), OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: the rows of codes must not overlap",
                  what);
-  OUDJAT_REQUIRE(rows < (1 << 26) && K < (1 << 30), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
+  // (a launch holds less than 2^32 threads)
+  OUDJAT_REQUIRE(cdiv(rows, K <= kWaveRow ? 4 : 1) < (1 << 24) && K < (1 << 30), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   auto go = [&](auto e, auto lanes, auto ch, auto lng) {
     constexpr int L = decltype(lanes)::value;
     quantize_int8_kernel<decltype(e), L, decltype(ch)::value, decltype(lng)::value>
@@ -449,7 +452,7 @@ extern "C" int oudjat_quantize_int8(const uint16_t* x, int64_t rows, int64_t K, 
   };
   using std::integral_constant;
   auto by_len = [&](auto e) {
-    if (K <= 1024) go(e, integral_constant<int, 64>{}, integral_constant<int, 2>{}, std::false_type{});
+    if (K <= kWaveRow) go(e, integral_constant<int, 64>{}, integral_constant<int, 2>{}, std::false_type{});
     else if (K <= 4096) go(e, integral_constant<int, 256>{}, integral_constant<int, 2>{}, std::false_type{});
     else if (K <= 8192) go(e, integral_constant<int, 256>{}, integral_constant<int, 4>{}, std::false_type{});
     else go(e, integral_constant<int, 256>{}, integral_constant<int, 4>{}, std::true_type{});
@@ -459,16 +462,22 @@ extern "C" int oudjat_quantize_int8(const uint16_t* x, int64_t rows, int64_t K, 
   return check_launch(what);
 }
 
+// A launch holds less than 2^32 threads.
+static bool launch_holds(const Int8Gemm& g, int threads) {
+  return (int64_t)g.tiles_m * g.tiles_n * threads < (int64_t)1 << 32;
+}
+
 template <class E, int EPI, int BM, int BN, int WGM, int WGN, int NST>
 static int launch_tile(Int8Gemm g, hipStream_t st, const char* what) {
   static std::atomic<uint64_t> done{0};
+  g.tiles_m = (int)cdiv(g.M, BM);
+  g.tiles_n = (int)cdiv(g.N, BN);
+  if (!launch_holds(g, WGM * WGN * 64)) return set_error(OUDJAT_ERR_TOO_LARGE, "%s: too many tiles", what);
   constexpr int RB = BM / WGM % 32 ? 16 : 32;  // rows of a wave that the epilogue stages
   constexpr int lds = std::max(NST * (BM + BN) * 128, WGM * WGN * RB * (BN / WGN + 4) * 4);
   const auto fn = int8_tile_kernel<E, EPI, BM, BN, WGM, WGN, NST>;
   const int rc = allow_lds((const void*)fn, lds, done, what);
   if (rc != OUDJAT_OK) return rc;
-  g.tiles_m = (int)cdiv(g.M, BM);
-  g.tiles_n = (int)cdiv(g.N, BN);
   fn<<<(unsigned)g.tiles_m * g.tiles_n, WGM * WGN * 64, lds, st>>>(g);
   return check_launch(what);
 }
@@ -477,6 +486,7 @@ template <class E, int EPI>
 static int launch_direct(Int8Gemm g, hipStream_t st, const char* what) {
   g.tiles_m = (int)cdiv(g.M, 16);
   g.tiles_n = (int)cdiv(g.N, 16);
+  if (!launch_holds(g, kDirectWaves * 64)) return set_error(OUDJAT_ERR_TOO_LARGE, "%s: too many tiles", what);
   int8_direct_kernel<E, EPI><<<(unsigned)g.tiles_m * g.tiles_n, kDirectWaves * 64, 0, st>>>(g);
   return check_launch(what);
 }

@@ -67,6 +67,16 @@ def test_linear_refuses(status, kw):
     refused(status, "oudjat_linear_int8", *linear_args(**kw))
 
 
+@pytest.mark.parametrize("rows,K", [(1 << 24, 1040), (1 << 25, 8192), ((1 << 26) - 3, 64)])
+def test_quantize_refuses_more_workgroups_than_a_launch_holds(rows, K):
+    refused("OUDJAT_ERR_TOO_LARGE", "oudjat_quantize_int8", *quant_args(rows=rows, K=K, x_rs=K, c_rs=K))
+
+
+@pytest.mark.parametrize("M,N,K", [(1 << 27, 16, 64), ((1 << 30) - 1, 64, 64), ((1 << 30) - 1, 8, 128)])
+def test_linear_refuses_more_workgroups_than_a_launch_holds(M, N, K):
+    refused("OUDJAT_ERR_TOO_LARGE", "oudjat_linear_int8", *linear_args(M=M, N=N, K=K, lda=K, ldw=K, ldc=N))
+
+
 def cache_args(Dh=64, Hk=2, N=8, **kw):
     """A head-major cache's addresses and strides."""
     a = dict(codes=ctypes.c_void_p(1 << 20), c_bs=2 * Hk * N * Dh // 2, c_ns=Dh // 2, c_cs=Hk * N * Dh // 2,
