@@ -171,7 +171,7 @@ SIGNATURES: dict[str, list] = {
     "oudjat_packed_attention_workspace_elems": [_i64, _i64, _i64, _i64, _i64, _i64],
     "oudjat_quantize_int8": [_p, _i64, _i64, _i64, _i32, _p, _i64, _p, _p],
     "oudjat_linear_int8": [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i32, _p],
-    "oudjat_linear_int8_tile": [_i64, _i64, _i64, _p, _p],
+    "oudjat_linear_int8_tile": [_i64, _i64, _i64, _p, _p, _p],
     "oudjat_kv_nvfp4_write": [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _i64, _i64, _i64,
                               _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p],
     "oudjat_kv_nvfp4_read": [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _p,

@@ -497,7 +497,8 @@ static int launch_direct(Int8Gemm g, hipStream_t st, const char* what) {
 // Where the others lie, us by 16 x 16 directly / 64 x 64 / 64 x 128 / 128 x 128 / 192 x 256 / 256 x 256:
 //   1 x 4096 x 4096: 5.9 / 9.4 / 12 / 21 / 28 / 30;  32 x 8192 x 4096: 17 / 9.8 / 13 / 22 / 28 / 30;
 //   512 x 4096 x 4096: 114 / 16 / 14 / 25 / 40 / 47;  1656 x 4096 x 8192: 727 / 90 / 78 / 60 / 76 / 87;
-//   1656 x 12288 x 4096: 1090 / 134 / 110 / 97 / 91 / 101;  16404 x 4096 x 8192: - / 833 / 671 / 547 / 504 / 499.
+//   1656 x 12288 x 4096: 1090 / 134 / 110 / 97 / 91 / 101;  16404 x 4096 x 8192: - / 833 / 671 / 547 / 504 / 499 (452 in
+//   two launches, below).
 struct Int8Tile {
   int bm, bn;
   float start, per_k, per_tile;
@@ -506,21 +507,52 @@ static const Int8Tile kInt8Tiles[] = {
     {16, 16, 2.29f, 0.088f, 0.2f},   {64, 64, 2.27f, 0.189f, 0.91f}, {64, 128, 1.97f, 0.292f, 1.39f},
     {128, 128, 2.5f, 0.479f, 2.39f}, {192, 256, 1.0f, 1.18f, 6.87f}, {256, 256, 1.0f, 1.346f, 9.13f},
 };
-static int choose_int8(int64_t M, int64_t N, int64_t K) {
+static constexpr int kInt8Kinds = sizeof(kInt8Tiles) / sizeof(kInt8Tiles[0]);
+static constexpr int kInt8Large = 4;  // from here on a CU holds one tile at a time
+static float int8_time(const Int8Tile& t, int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
+  return t.start + (float)cdiv(tiles, 256) * ((float)K / 128.0f * t.per_k + t.per_tile);
+}
+static int choose_int8(int64_t M, int64_t N, int64_t K, float& least) {
   int best = 0;
-  float least = 0.0f;
-  for (int i = 0; i < (int)(sizeof(kInt8Tiles) / sizeof(kInt8Tiles[0])); ++i) {
-    const Int8Tile& t = kInt8Tiles[i];
-    const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
-    const float us = t.start + (float)cdiv(tiles, 256) * ((float)K / 128.0f * t.per_k + t.per_tile);
-    if (i == 0 || us < least) best = i, least = us;
+  least = int8_time(kInt8Tiles[0], M, N, K);
+  for (int i = 1; i < kInt8Kinds; ++i) {
+    const float us = int8_time(kInt8Tiles[i], M, N, K);
+    if (us < least) best = i, least = us;
   }
   return best;
 }
 
+// Rows of a plan: all by one kernel, or those that fill whole rounds of large tiles and then the rest by smaller ones in a
+// second launch. The rest reads the weight once more; a split is taken where the model says that it spares a
+// twentieth or more, and only for tiles that a CU holds one at a time, whose rounds are real ones (128 x 128 for 1024 of
+// 1300 rows, 4096 x 4096: 39 us, in one launch 33). us in one launch and in two: 4116 x 4096 x 4096: 84, 68;
+// 16404 x 1024 x 1024: 34, 28; 4600 x 4096 x 8192: 159, 139; 16404 x 4096 x 8192: 493, 452; 33000 x 4096 x 1024: 201, 197;
+// 16404 x 8192 x 4096: 506, 499; not taken, by the twentieth: 5000 x 8192 x 8192: 288, 282; 1656 x 12288 x 4096: 88, 89.
+struct Int8Plan {
+  int tile, rest;
+  int64_t first;  // rows of the first launch
+};
+static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K) {
+  float least, rest_us;
+  Int8Plan p{choose_int8(M, N, K, least), 0, M};
+  const float again = (float)N * (float)K / 5e6f;  // the weight at 5 TB/s
+  least *= 0.95f;
+  for (int i = kInt8Large; i < kInt8Kinds; ++i) {
+    const Int8Tile& t = kInt8Tiles[i];
+    const int64_t across = cdiv(N, t.bn), rounds = cdiv(cdiv(M, t.bm) * across, 256) - 1;
+    const int64_t first = rounds * 256 / across * t.bm;
+    if (first <= 0 || first >= M) continue;
+    const int rest = choose_int8(M - first, N, K, rest_us);
+    const float us = int8_time(t, first, N, K) + again + rest_us;
+    if (us < least) least = us, p = Int8Plan{i, rest, first};
+  }
+  return p;
+}
+
 template <class E, int EPI>
-static int launch_int8(const Int8Gemm& g, hipStream_t st, const char* what) {
-  switch (choose_int8(g.M, g.N, g.K)) {
+static int launch_one(int tile, const Int8Gemm& g, hipStream_t st, const char* what) {
+  switch (tile) {
     case 0: return launch_direct<E, EPI>(g, st, what);
     case 1: return launch_tile<E, EPI, 64, 64, 2, 2, 4>(g, st, what);
     case 2: return launch_tile<E, EPI, 64, 128, 2, 4, 3>(g, st, what);
@@ -529,13 +561,28 @@ static int launch_int8(const Int8Gemm& g, hipStream_t st, const char* what) {
     default: return launch_tile<E, EPI, 256, 256, 2, 4, 2>(g, st, what);
   }
 }
+template <class E, int EPI>
+static int launch_int8(Int8Gemm g, hipStream_t st, const char* what) {
+  const Int8Plan p = plan_int8(g.M, g.N, g.K);
+  const int rest = g.M - (int)p.first;
+  g.M = (int)p.first;
+  const int rc = launch_one<E, EPI>(p.tile, g, st, what);
+  if (rc != OUDJAT_OK || !rest) return rc;
+  g.a += p.first * g.lda;
+  g.sa += p.first;
+  if (g.resid) g.resid += p.first * g.ldr;
+  g.c += p.first * g.ldc;
+  g.M = rest;
+  return launch_one<E, EPI>(p.rest, g, st, what);
+}
 
-extern "C" int oudjat_linear_int8_tile(int64_t M, int64_t N, int64_t K, int* rows, int* columns) {
+extern "C" int oudjat_linear_int8_tile(int64_t M, int64_t N, int64_t K, int* rows, int* columns, int64_t* first) {
   const char* what = "linear_int8_tile";
-  OUDJAT_REQUIRE(M > 0 && N > 0 && K > 0 && rows && columns, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad argument", what);
-  const Int8Tile& t = kInt8Tiles[choose_int8(M, N, K)];
-  *rows = t.bm;
-  *columns = t.bn;
+  OUDJAT_REQUIRE(M > 0 && N > 0 && K > 0 && rows && columns && first, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad argument", what);
+  const Int8Plan p = plan_int8(M, N, K);
+  *rows = kInt8Tiles[p.tile].bm;
+  *columns = kInt8Tiles[p.tile].bn;
+  *first = p.first;
   return OUDJAT_OK;
 }
 

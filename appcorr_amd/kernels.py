@@ -1641,11 +1641,12 @@ def linear_int8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_sca
     return out
 
 
-def linear_int8_tile(M: int, N: int, K: int) -> tuple[int, int]:
-    """(rows, columns) of the output tile that linear_int8 takes for an M x N x K product."""
-    rows, columns = ctypes.c_int(0), ctypes.c_int(0)
-    call("oudjat_linear_int8_tile", M, N, K, ctypes.addressof(rows), ctypes.addressof(columns))
-    return rows.value, columns.value
+def linear_int8_tile(M: int, N: int, K: int) -> tuple[int, int, int]:
+    """(rows, columns) of the output tile that linear_int8 takes for an M x N x K product, and how many of the M rows are done so:
+    the rest, if any, take a second launch with smaller tiles, which spares a last round of few large ones."""
+    rows, columns, first = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int64(0)
+    call("oudjat_linear_int8_tile", M, N, K, ctypes.addressof(rows), ctypes.addressof(columns), ctypes.addressof(first))
+    return rows.value, columns.value, first.value
 
 
 @dataclass

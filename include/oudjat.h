@@ -836,8 +836,9 @@ int oudjat_linear_int8(const int8_t* A, int64_t M, int64_t K, int64_t lda, const
                        oudjat_stream_t stream);
 
 /* Rows and columns of the output tile that oudjat_linear_int8 takes for an M x N x K product (16 x 16: the kernel without LDS
- * tiles, for few rows). */
-int oudjat_linear_int8_tile(int64_t M, int64_t N, int64_t K, int* rows, int* columns);
+ * tiles, for few rows), and how many rows are done so: the rest, M - *first, if any, take a second launch with smaller
+ * tiles, which spares a last round of few large ones. */
+int oudjat_linear_int8_tile(int64_t M, int64_t N, int64_t K, int* rows, int* columns, int64_t* first);
 
 /* An NVFP4 K/V cache: codes [B, N, 2, Hk, Dh / 2] (two values a byte, the even one in the low nibble; strides c_bs, c_ns,
  * c_cs, c_hs) and scales [B, N, 2, Hk, Dh / 16] (e4m3, one for 16 dims; s_bs .. s_hs), strides in bytes, and tensor_scale

@@ -136,6 +136,8 @@ SHAPES = [(1, 8, 64), (1, 4096, 4096), (2, 384, 384), (15, 200, 128), (16, 1024,
 # (test_int8_nvfp4_host.py says so); the widths of this package's blocks.
 SHAPES += [(3531, 2184, 64), (2305, 5000, 192), (4117, 3896, 832), (2289, 4680, 192), (922, 11272, 320), (3000, 4104, 64),
            (3000, 4104, 192), (5243, 5448, 704), (1656, 8200, 576), (300, 1032, 2112)]
+# The last rows in a second launch.
+SHAPES += [(4116, 4096, 576), (12289, 2048, 448), (12309, 2056, 320)]
 
 
 @pytest.mark.parametrize("epi", ["bias", "ls", "ls_resid", "silu"])
@@ -183,6 +185,23 @@ def test_linear_strided_operands(dev):
     three = K.linear_int8(x8.view(7, 10, Kd), sx.view(7, 10), w8, sw, bias)
     assert three.shape == (7, 10, N)
     check(three.view(M, N), *product64(x8, sx, w8, sw, bias, None, None, "bias"))
+
+
+def test_strided_operands_in_two_launches(dev):
+    """As above where the rows are dealt to two launches."""
+    M, N, Kd = 4103, 4096, 256
+    assert K.linear_int8_tile(M, N, Kd)[2] == 4096
+    x8, sx, w8, sw, bias, gamma, resid = operands(dev, M, N, Kd, HF, "ls_resid", 5)
+    ref, size = product64(x8, sx, w8, sw, bias, gamma, resid, "ls_resid")
+    xb = torch.zeros(M, 2, Kd, device=dev, dtype=torch.int8)
+    ob = torch.full((M + 1, N + 8), 5.0, device=dev, dtype=HF)
+    xb[:, 1], ob[:M, :N] = x8, resid
+    K.linear_int8(xb[:, 1], sx, w8, sw, bias, epilogue=EPI["ls_resid"], gamma=gamma, resid=ob[:M, :N], out=ob[:M, :N], dtype=HF)
+    check(ob[:M, :N], ref, size)
+    assert (ob[M] == 5.0).all() and (ob[:, N:] == 5.0).all()
+    got = K.linear_int8(x8[:1].expand(M, Kd), sx, w8, sw, epilogue=EPI["ls_resid"], gamma=gamma, resid=resid[:1].expand(M, N),
+                        dtype=HF)
+    check(got, *product64(x8[:1].expand(M, Kd), sx, w8, sw, None, gamma, resid[:1].expand(M, N), "ls_resid"))
 
 
 def test_rows_that_are_not_finite_give_nan(dev):

@@ -205,9 +205,13 @@ def test_a_cache_lays_a_heads_tokens_side_by_side():
 def test_gpu_tests_reach_every_tile_of_the_product():
     from tests.test_gpu_int8 import SHAPES
 
-    tiles = Counter(K.linear_int8_tile(*s) for s in SHAPES)
+    plans = [(s, K.linear_int8_tile(*s)) for s in SHAPES]
+    tiles = Counter(p[:2] for _, p in plans)
     assert set(tiles) == {(16, 16), (64, 64), (64, 128), (128, 128), (192, 256), (256, 256)}
     assert min(tiles.values()) >= 2
+    split = [(s, p) for s, p in plans if p[2] != s[0]]  # rows in two launches, from either of the large tiles
+    assert {p[0] for _, p in split} == {192, 256}
+    assert all(0 < p[2] < s[0] and p[2] % p[0] == 0 for s, p in split)
 
 
 def test_every_kernel_of_the_library_is_one_that_a_call_takes():
