@@ -8,13 +8,16 @@
 // holds is finite. Element 2i lies in the low nibble of byte i. The scale bytes are read without their sign bit, and
 // 0x7f (never written) as 480, so that memory that nobody has written cannot give a NaN either.
 #include <algorithm>
+#include <type_traits>
 
 #include "elem.hpp"
 #include "nvfp4_kv.hpp"
 
 namespace oudjat {
 
-static constexpr int kKvThreads = 256, kReadItems = 2;
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+static constexpr int kKvThreads = 256;
 
 // Reciprocal of a normal b whose reciprocal is normal too: one Newton step on the hardware's, which is within an ulp, gives
 // the correctly rounded one (a significand of all ones aside).
@@ -26,6 +29,13 @@ __device__ __forceinline__ float rcp_rn(float b) {
 __device__ __forceinline__ float quotient(float a, float b, float y) {
   const float q0 = a * y;
   return __builtin_fmaf(__builtin_fmaf(-q0, b, a), y, q0);
+}
+
+// Workgroups of one XCD (b, b + 8, ..) take consecutive rows, whose slots mostly lie side by side: a line of codes holds two
+// tokens of a head, one of scales 16, and it is in one L2.
+__device__ __forceinline__ int64_t xcd_group() {
+  const int n = gridDim.x, b = blockIdx.x, xcd = b & 7, q = n >> 3, rest = n & 7;
+  return xcd * q + min(xcd, rest) + (b >> 3);
 }
 
 // A block's scale byte and codes. The usual block is finite, its values and the tensor scale are of ordinary size, and the
@@ -63,17 +73,27 @@ __device__ __forceinline__ uint2 quantize_block(const uint4& lo, const uint4& hi
   return make_uint2(nvfp4_codes8(f, unit, y), nvfp4_codes8(f + 8, unit, y));
 }
 
+// UNI: a row is whole waves of items, so that what belongs to the row alone (its slot, its addresses) is the scalar unit's
+// (reads of 16404 rows of 32 heads of 128: 195 -> 189 us as they were then, of 4116 of 16 of 64 13.3 -> 12.6).
+template <bool UNI>
+__device__ __forceinline__ int row_of(int r) {
+  return UNI ? __builtin_amdgcn_readfirstlane(r) : r;
+}
+
 // Write. An item is a block, 16 dims of a head: the wave reads and writes consecutive pieces of a row, and one lane in four
-// stores four scales. A workgroup takes `per_wg` rows.
-template <class E>
+// stores four scales. A workgroup takes `per_wg` rows. Bound by HBM and by the pieces' ends: a token of a head is 64 or 32
+// bytes of codes and 8 or 4 of scales. 16404 rows of 32 heads of 128, 344 MB, us: in slot order 73 (4.7 TB/s; without the
+// order by XCD 77), shuffled 87; 4116 of 16 of 64: 7.9 and 8.7 (8.4 and 9.0 with two rounds of items a workgroup). Half of the
+// SIMDs' cycles are the quantisation's VALU instructions (IEEE divisions for every block and value: 114).
+template <class E, bool UNI>
 __global__ __launch_bounds__(kKvThreads) void kv_nvfp4_write_kernel(
     const uint16_t* __restrict__ k, int64_t k_rs, int64_t k_hs, const uint16_t* __restrict__ v, int64_t v_rs,
     int64_t v_hs, int64_t rows, int blocks, Divisor by_row, Divisor by_head, const int64_t* __restrict__ batch_idx,
     const int64_t* __restrict__ token_idx, KvNvfp4 c, int per_wg) {
-  const int64_t row0 = (int64_t)blockIdx.x * per_wg;
+  const int64_t row0 = xcd_group() * per_wg;
   const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * blocks;
   for (int i = threadIdx.x; i < n * per_row; i += kKvThreads) {
-    const int r = by_row(i), j = i - r * per_row;
+    const int r = row_of<UNI>(by_row(i)), j = i - r * per_row;
     const int kh = by_head(j), d16 = j - kh * blocks;  // key heads, then value heads; 16 dims
     const bool val = kh >= c.Hk;
     const int h = val ? kh - c.Hk : kh;
@@ -93,67 +113,68 @@ __global__ __launch_bounds__(kKvThreads) void kv_nvfp4_write_kernel(
   }
 }
 
-// Read. An item is a block: 8 bytes of codes and a scale byte in, 32 bytes out; a thread has the loads of U in flight.
-template <class E, int U>
+// The value of the lane next to this one (l ^ 1).
+__device__ __forceinline__ uint32_t swap_lanes(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true);
+}
+
+// Read. An item is a block: 8 bytes of codes and a scale byte in, 32 bytes out. Two lanes exchange halves of their blocks, so
+// that a wave's store is one piece of memory, and the stores bypass the caches, which then keep the lines of the cache
+// that neighbouring tokens share. 16404 rows of 32 heads of 128 written and as many others, 690 MB in all, us: in slot order
+// 120 (5.7 TB/s), shuffled 168; through the caches 181 and 193; pieces of 16 bytes of two lanes' blocks past the caches 271,
+// 263; two blocks a thread 125, 214.
+template <class E, bool UNI>
 __global__ __launch_bounds__(kKvThreads) void kv_nvfp4_read_kernel(KvNvfp4 c, int blocks, Divisor by_row, Divisor by_head,
                                                                    const int64_t* __restrict__ batch_idx,
                                                                    const int64_t* __restrict__ token_idx, int64_t rows,
                                                                    uint16_t* __restrict__ k_out,
                                                                    uint16_t* __restrict__ v_out, int per_wg) {
-  const int64_t row0 = (int64_t)blockIdx.x * per_wg;
+  const int64_t row0 = xcd_group() * per_wg;
   const int n = (int)min((int64_t)per_wg, rows - row0), per_row = 2 * c.Hk * blocks;
-  for (int i0 = threadIdx.x; i0 < n * per_row; i0 += U * kKvThreads) {
-    uint2 w[U];
-    uint32_t s8[U];
-    uint16_t* dst[U];
-    float ts[U];
-    bool there[U], slot[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kKvThreads;
-      there[u] = i < n * per_row;
-      const int r = by_row(there[u] ? i : i0), j = (there[u] ? i : i0) - r * per_row;
-      const int kh = by_head(j), d16 = j - kh * blocks;
-      const bool val = kh >= c.Hk;
-      const int h = val ? kh - c.Hk : kh;
-      const int64_t row = row0 + r, b = batch_idx[row], t = token_idx[row];
-      slot[u] = b >= 0 && b < c.B && t >= 0 && t < c.N;
-      w[u] = make_uint2(0, 0);
-      s8[u] = 0;
-      if (slot[u]) {
-        w[u] = *reinterpret_cast<const uint2*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 8 * d16);
-        s8[u] = c.scales[b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d16];
-      }
-      ts[u] = c.ts[kh];
-      dst[u] = (val ? v_out : k_out) + (row * c.Hk + h) * (16 * blocks) + 16 * d16;
+  const bool odd = threadIdx.x & 1;
+  for (int i = threadIdx.x; i < n * per_row; i += kKvThreads) {
+    const int r = row_of<UNI>(by_row(i)), j = i - r * per_row;
+    const int kh = by_head(j), d16 = j - kh * blocks;
+    const bool val = kh >= c.Hk;
+    const int h = val ? kh - c.Hk : kh;
+    const int64_t row = row0 + r, b = batch_idx[row], t = token_idx[row];
+    uint2 w = make_uint2(0, 0);  // a slot outside the cache: zeros, whatever the tensor scale is
+    uint32_t s8 = 0;
+    float ts = 0.0f;
+    if (b >= 0 && b < c.B && t >= 0 && t < c.N) {
+      w = *reinterpret_cast<const uint2*>(c.codes + b * c.bs + t * c.ns + (val ? c.cs : 0) + h * c.hs + 8 * d16);
+      s8 = c.scales[b * c.sbs + t * c.sns + (val ? c.scs : 0) + h * c.shs + d16];
+      ts = c.ts[kh];
     }
+    const float s = e4m3_decode(s8 & 0x7f);
+    float f[16];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!there[u]) continue;
-      const float s = e4m3_decode(s8[u] & 0x7f);
-      float f[16];
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t x = half ? w.y : w.x;
+      const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 0);
+      const auto v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 1);
+      const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 2);
+      const auto v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 3);
+      const float e2[8] = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t x = half ? w[u].y : w[u].x;
-        const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 0);
-        const auto v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 1);
-        const auto v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 2);
-        const auto v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, 1.0f, 3);
-        const float e2[8] = {v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[8 * half + e] = (e2[e] * s) * ts[u];  // (the first product is exact)
-      }
-      if (!slot[u])
-#pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = 0.0f;
-      store16(dst[u], E::from8(f));
-      store16(dst[u] + 8, E::from8(f + 8));
+      for (int e = 0; e < 8; ++e) f[8 * half + e] = (e2[e] * s) * ts;  // (the first product is exact)
     }
+    const u32x4_t lo = __builtin_bit_cast(u32x4_t, E::from8(f)), hi = __builtin_bit_cast(u32x4_t, E::from8(f + 8));
+    u32x4_t first, second;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t got = swap_lanes(odd ? lo[e] : hi[e]);  // (a row has an even number of blocks: both lanes are here)
+      first[e] = odd ? got : lo[e];
+      second[e] = odd ? hi[e] : got;
+    }
+    uint16_t* dst = (val ? v_out : k_out) + (row * c.Hk + h) * (16 * blocks) + 16 * (d16 & ~1) + (odd ? 8 : 0);
+    __builtin_nontemporal_store(first, reinterpret_cast<u32x4_t*>(dst));
+    __builtin_nontemporal_store(second, reinterpret_cast<u32x4_t*>(dst + 16));
   }
 }
 
-// Rows of a workgroup: about `each` items a thread.
-static int kv_rows_per_wg(int64_t per_row, int each) { return (int)std::max<int64_t>(1, each * kKvThreads / per_row); }
+// Rows of a workgroup: as many whole ones as its threads, one at the least.
+static int kv_rows_per_wg(int64_t per_row) { return (int)std::max<int64_t>(1, kKvThreads / per_row); }
 
 int check_kv_nvfp4(const KvNvfp4& c, int64_t Dh, const char* what) {
   OUDJAT_REQUIRE(c.bs >= 0 && c.ns >= 0 && c.cs >= 0 && c.hs >= 0 && c.sbs >= 0 && c.sns >= 0 && c.scs >= 0 && c.shs >= 0,
@@ -195,16 +216,17 @@ extern "C" int oudjat_kv_nvfp4_write(const uint16_t* k, int64_t k_rs, int64_t k_
                      entries_apart({{B, s_bs}, {N, s_ns}, {2, s_cs}, {Hk, s_hs}}, Dh / 16),
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: the rows of the cache must not overlap", what);
   const int64_t per_row = 2 * Hk * Dh / 16;
-  const int per = kv_rows_per_wg(per_row, 2);
+  const int per = kv_rows_per_wg(per_row);
   OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   if (empty) return OUDJAT_OK;
-  auto go = [&](auto e) {
-    kv_nvfp4_write_kernel<decltype(e)><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
+  auto go = [&](auto e, auto uni) {
+    kv_nvfp4_write_kernel<decltype(e), decltype(uni)::value><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
         k, k_rs, k_hs, v, v_rs, v_hs, rows, (int)(Dh / 16), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 16)),
         batch_idx, token_idx, c, per);
   };
-  if (dtype == OUDJAT_BF16) go(ElemBf16{});
-  else go(ElemFp16{});
+  auto by_row = [&](auto e) { per_row % 64 ? go(e, std::false_type{}) : go(e, std::true_type{}); };
+  if (dtype == OUDJAT_BF16) by_row(ElemBf16{});
+  else by_row(ElemFp16{});
   return check_launch(what);
 }
 
@@ -230,14 +252,15 @@ extern "C" int oudjat_kv_nvfp4_read(const uint8_t* codes, int64_t c_bs, int64_t 
   OUDJAT_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16) && aligned(batch_idx, 8) && aligned(token_idx, 8),
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned outputs required", what);
   const int64_t per_row = 2 * Hk * Dh / 16;
-  const int per = kv_rows_per_wg(per_row, kReadItems);
+  const int per = kv_rows_per_wg(per_row);
   OUDJAT_REQUIRE(cdiv(rows, per) < (1 << 24), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
-  auto go = [&](auto e) {
-    kv_nvfp4_read_kernel<decltype(e), kReadItems><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
+  auto go = [&](auto e, auto uni) {
+    kv_nvfp4_read_kernel<decltype(e), decltype(uni)::value><<<(unsigned)cdiv(rows, per), kKvThreads, 0, as_stream(stream)>>>(
         c, (int)(Dh / 16), Divisor((uint32_t)per_row), Divisor((uint32_t)(Dh / 16)), batch_idx, token_idx, rows, k_out,
         v_out, per);
   };
-  if (dtype == OUDJAT_BF16) go(ElemBf16{});
-  else go(ElemFp16{});
+  auto by_row = [&](auto e) { per_row % 64 ? go(e, std::false_type{}) : go(e, std::true_type{}); };
+  if (dtype == OUDJAT_BF16) by_row(ElemBf16{});
+  else by_row(ElemFp16{});
   return check_launch(what);
 }

@@ -229,3 +229,6 @@ def test_every_kernel_of_the_library_is_one_that_a_call_takes():
     both = [(e,) for e in ("Bf16", "Fp16")]
     assert attention(rb"nvfp4_attn_keys_kernel") == {(*e, d, w) for e in both for d in (64, 128) for w in (4, 8)}
     assert attention(rb"nvfp4_attn_rows_kernel") == {(*e, d, w) for e in both for d, w in ((64, 4), (128, 4), (128, 8))}
+    rows = {(e.decode(), m.decode(), int(u)) for m, e, u in
+            re.findall(rb"kv_nvfp4_(write|read)_kernelINS_8Elem(Bf16|Fp16)ELb([01])EE", blob)}
+    assert rows == {(e, m, u) for (e,) in both for m in ("write", "read") for u in (0, 1)}
