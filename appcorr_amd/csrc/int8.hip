@@ -21,6 +21,8 @@ typedef int i32x4v_t __attribute__((ext_vector_type(4)));
 // Quotients are the IEEE ones: with y = RN(1 / s), q0 = RN(x y), r = x - q0 s (exact by an FMA), RN(q0 + r y) is the
 // correctly rounded quotient; where s is so small that y overflows or r underflows, x and s are scaled by 2^100 first.
 // Adding 1.5 2^23 leaves the nearest whole number (ties to even) in the low byte.
+// Bound by HBM: 16404 rows of 8192 in 62 to 73 us (5.5 TB/s and more, VALU 68 % busy), 1656 of 4096 in 7.2; few rows by a launch
+// and a round of loads (2.2 to 3.4).
 // ------------------------------------------------------------------------------------------------
 struct QuantRow {
   float s, t, y, up;  // scale; the scale and its inverse as they are used, the factor between

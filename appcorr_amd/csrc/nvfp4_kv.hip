@@ -83,8 +83,8 @@ __device__ __forceinline__ int row_of(int r) {
 // Write. An item is a block, 16 dims of a head: the wave reads and writes consecutive pieces of a row, and one lane in four
 // stores four scales. A workgroup takes `per_wg` rows. Bound by HBM and by the pieces' ends: a token of a head is 64 or 32
 // bytes of codes and 8 or 4 of scales. 16404 rows of 32 heads of 128, 344 MB, us: in slot order 73 (4.7 TB/s; without the
-// order by XCD 77), shuffled 87; 4116 of 16 of 64: 7.9 and 8.7 (8.4 and 9.0 with two rounds of items a workgroup). Half of the
-// SIMDs' cycles are the quantisation's VALU instructions (IEEE divisions for every block and value: 114).
+// order by XCD 77), shuffled 87; 4116 of 16 of 64: 7.9 and 8.7 (8.4 and 9.0 with two rounds of items a workgroup). The
+// quantisation's VALU instructions take 80 % of the SIMDs' cycles (with IEEE divisions for every block and value: 114 us).
 template <class E, bool UNI>
 __global__ __launch_bounds__(kKvThreads) void kv_nvfp4_write_kernel(
     const uint16_t* __restrict__ k, int64_t k_rs, int64_t k_hs, const uint16_t* __restrict__ v, int64_t v_rs,
