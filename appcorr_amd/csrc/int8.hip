@@ -224,6 +224,17 @@ __global__ __launch_bounds__(kDirectWaves * 64) void int8_direct_kernel(Int8Gemm
   if (m0 + l16 < g.M && n0 + 4 * G < g.N) int8_store4<E, EPI>(g, m0 + l16, n0 + 4 * G, acc);
 }
 
+// Eight outputs of a tile. Large tiles store past the caches, which then keep the operands that other tiles read: with the
+// quantiser that reads the output next, 16404 x 8192 x 4096: 563 -> 546 us (the product alone 493 -> 456), 4176 x 4096 x 1024: 42 ->
+// 40, 16404 x 4096 x 4096 and 1656 x 8192 x 4096: the same. Small tiles make outputs that are still in the caches when they are
+// read (40 x 4096 x 4096: 12.9, past them 13.2).
+template <bool PAST>
+__device__ __forceinline__ void store_row(uint16_t* p, const uint4& v) {
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  if constexpr (PAST) __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, v), reinterpret_cast<u32x4_t*>(p));
+  else store16(p, v);
+}
+
 // Tile kernel: BM x BN outputs, WGM x WGN waves of WM x WN each, K in tiles of 128 bytes through NST stages of LDS that
 // buffer loads fill (descriptors of the tile's rows that exist: others load as zeros). LDS row r keeps its 16-byte chunk
 // c in slot c ^ (r / 2) % 8, so that 16 rows at one chunk cover all banks. v_mfma_i32_16x16x64_i8 with the weight as its
@@ -422,7 +433,7 @@ __global__ __launch_bounds__(WGM * WGN * 64) void int8_tile_kernel(Int8Gemm g) {
         for (int e = 0; e < 8; ++e)
           v[e] = EPI == OUDJAT_EPI_BIAS_LS_RESID ? v[e] + t[e] : silu(v[e]) * t[e];
       }
-      if (m < g.M && n < g.N) store16(g.c + (int64_t)m * g.ldc + n, E::from8(v));
+      if (m < g.M && n < g.N) store_row<(BM >= 128)>(g.c + (int64_t)m * g.ldc + n, E::from8(v));
     }
   }
 }
