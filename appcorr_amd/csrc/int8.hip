@@ -136,9 +136,11 @@ __device__ __forceinline__ float silu(float y) {
   return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.44269504f));
 }
 
-// Four outputs of one row, columns n .. n + 3.
+// Four outputs of one row, columns n .. n + 3, with the roundings of the tile kernel, where y gamma goes through LDS before the
+// residual is added: no contraction of the two, so that a row's bits do not depend on the kernel.
 template <class E, int EPI>
 __device__ __forceinline__ void int8_store4(const Int8Gemm& g, int m, int n, const i32x4v_t& acc) {
+#pragma clang fp contract(off)
   typedef uint16_t u16x4_t __attribute__((ext_vector_type(4)));
   auto four = [&](const uint16_t* p, float* f) {
     const u16x4_t v = *reinterpret_cast<const u16x4_t*>(p);

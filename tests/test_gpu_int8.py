@@ -154,6 +154,21 @@ def test_linear(dev, M, N, Kd, dtype, epi):
         assert torch.equal(out, got)
 
 
+@pytest.mark.parametrize("epi", ["bias", "ls", "ls_resid", "silu"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_a_rows_result_does_not_depend_on_the_other_rows(dev, dtype, epi):
+    """Rows of a product in two launches, and the same rows by themselves through other kernels: the same bits."""
+    M, N, Kd = 4116, 4096, 576
+    x8, sx, w8, sw, bias, gamma, resid = operands(dev, M, N, Kd, dtype, epi, 11)
+    whole = K.linear_int8(x8, sx, w8, sw, bias, epilogue=EPI[epi], gamma=gamma, resid=resid, dtype=dtype)
+    cuts = [(7, 8), (40, 60), (100, 200), (300, 800), (900, 2000), (2000, 4000), (4090, 4116)]
+    assert len({K.linear_int8_tile(b - a, N, Kd)[:2] for a, b in cuts} | {K.linear_int8_tile(M, N, Kd)[:2]}) >= 5
+    for a, b in cuts:
+        part = K.linear_int8(x8[a:b], sx[a:b], w8, sw, bias, epilogue=EPI[epi], gamma=gamma,
+                             resid=None if resid is None else resid[a:b], dtype=dtype)
+        assert torch.equal(part, whole[a:b]), (a, b)
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_linear_is_exact_at_the_largest_sums(dev, M):
     """Codes of -128 everywhere, K just below 2^17: the sums come within 2^20 of 2^31."""
