@@ -7,8 +7,8 @@
 // multiplies by 2^8). Both products run in fp16 for either type of the queries: a query row is scaled by a power of two
 // that brings its largest value to 2^14 .. 2^15 (bf16 values keep all their bits down to 2^-28 of it), that power and
 // the key head's h go into the row's factor of the scores, the value head's h into the output. Probabilities are kept
-// 2^7 larger than their reference says, at most 2^15 with the 2^8 that the reference may lag, so that weights down to
-// 2^-21 of the largest are normal numbers of fp16 (rounded by at most 2^-11 of their value).
+// 2^7 larger than their reference says, at most 2^15 with the 2^8 that the reference may lag (kFarScore: whatever the
+// scores' size), so that weights down to 2^-21 of the largest are normal numbers of fp16 (rounded by at most 2^-11 of their value).
 #include "elem.hpp"
 #include "nvfp4_kv.hpp"
 
@@ -24,6 +24,23 @@ typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 
 static constexpr float kProbShift = 7.0f;
+
+// The weight of score s is 2^(c s + shift), c the row's factor. With a reference of ordinary size one FMA takes it off,
+// shift = 7 - c ref, rounded no more than the score itself would be in fp32. From 2^20 on the reference is taken off the
+// scores first, exactly where they lie close, so that c (s - ref) is at most the 8 that it may lag: further out the rounding
+// of the shift is whole exponents (16 at 2^28: infinite weights, or none at all). A trained model has no such row. The keys
+// kernel looks at the reference in every tile; the rows kernel, where that costs 1 to 2 % at 64 dims, decides by the row's factor
+// alone (scaled queries are below 2^15 and x^ is at most 6 * 480: Dh = 128, query values of 100 against keys of 450 at the usual
+// scale are still near) and sends such rows through its masked tiles.
+static constexpr float kFarScore = 1048576.0f;
+template <int DH>
+__device__ __forceinline__ bool far_scores(float c) {
+  return c > kFarScore / (DH * 32768.0f * 2880.0f);
+}
+// A reference as the exponent that the other waves' and parts' meet, kept finite (-inf, no key, too: its sum is 0).
+__device__ __forceinline__ float ref_exponent(float m, float c) { return fminf(fmaxf(m * c, -3.40282347e38f), 3.40282347e38f); }
+// A row's factor of its scores. Not 0 and not infinite, so that a hidden key's -inf stays what it is and a difference of 0 is 0.
+__device__ __forceinline__ float score_factor(float c) { return fminf(fmaxf(c, 1.17549435e-38f), 3.40282347e38f); }
 
 // Byte of 16-byte chunk `chunk` of key row `row` in a tile. Dh = 128: the chunks of row r lie at chunk ^ swz(r), swz a
 // permutation of 0 .. 15 that puts four consecutive rows into four quarters of a row and the next four into the other
@@ -121,8 +138,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_key
   const float down = load_query<E, QK_STEPS>(
       a.q + (int64_t)(w.q0 + tok) * a.q_rs + (int64_t)(h * a.G + head) * a.q_hs + G * (DH / 4), 8, qf, bad,
       [](float x) { return xor32_max(xor16_max(x)); }, [](float x) { return xor32_sum(xor16_sum(x)); });
-  // The scores' factor; not 0, so that a hidden key's -inf stays what it is.
-  const float c = fmaxf(na.scale_log2 * na.c.ts[h] * down, 1.17549435e-38f);
+  const float c = score_factor(na.scale_log2 * na.c.ts[h] * down);
 
   struct Tile {
     uint32_t k[2][CW], v[2][CW], ks[2], vs[2];
@@ -187,13 +203,21 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_key
     }
     float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
     mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mx = xor32_max(xor16_max(mx)) * c;
-    const float m_new = softmax_ref_max(m_i, mx, 1.0f);
-    const float mc = ref_shift(m_new, 1.0f);
-    const float alpha = __builtin_amdgcn_exp2f(m_i - mc);
+    mx = xor32_max(xor16_max(mx));
+    const float m_new = softmax_ref_max(m_i, mx, c);
+    const float ref = ref_shift(m_new, 1.0f);
+    const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * c);
+    float shift = kProbShift - ref * c;
+    const bool far = fabsf(ref * c) > kFarScore;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(far) != 0, 0)) {
+      const float off = far ? ref : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] -= off;
+      shift = far ? kProbShift : shift;
+    }
     float p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], c, kProbShift - mc));
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], c, shift));
     const h8_t pf = round8<AttnFp16>(p);
     l_i = l_i * alpha + xor32_sum(xor16_sum(AttnFp16::sum8(pf, 0.0f)));
     m_i = m_new;
@@ -233,7 +257,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_key
   {
     float* p = park + wave * WROWS;
     if (G == 0) {
-      p[l16] = m_i;
+      p[l16] = ref_exponent(m_i, c);
       p[R + l16] = l_i;
     }
 #pragma unroll
@@ -319,14 +343,16 @@ __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na
   const int per = w.parts == 1 ? all_tiles : (all_tiles + w.parts - 1) / w.parts;
   const int tb = w.part * per;                       // first key tile of this part; tiles are numbered from it below
   const int ntiles = max(0, min(per, all_tiles - tb));
-  const int nfull = lim_tile / kKeyTile - tb;
 
   h8_t qf[QK_STEPS];  // lane: row l32, dims 16 ks + 8 g ..
   bool bad;
   const float down = load_query<E, QK_STEPS>(
       a.q + (int64_t)(w.q0 + tok) * a.q_rs + (int64_t)(h * a.G + head) * a.q_hs + 8 * g, 16, qf, bad,
       [](float x) { return xor32_max(x); }, [](float x) { return xor32_sum(x); });
-  const float c = fmaxf(na.scale_log2 * na.c.ts[h] * down, 1.17549435e-38f);
+  const float c = score_factor(na.scale_log2 * na.c.ts[h] * down);
+  const bool far = far_scores<DH>(c), any_far = __builtin_amdgcn_ballot_w64(far) != 0;
+  // Tiles that need neither a mask nor a reference taken off first (a wave's own: every tile has one barrier).
+  const int nfull = any_far ? 0 : lim_tile / kKeyTile - tb;
 
   // This thread's pieces: with one a thread the waves' first half takes keys, the second values.
   const int pw = PIECES == 1 ? wave % (W / 2) : wave, pkey = pw * PPW + (lane & 15) + 16 * (lane / (16 * (DH / 32)));
@@ -413,11 +439,18 @@ __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na
 #pragma unroll
       for (int v = 1; v < 8; ++v) mq[q4] = fmaxf(mq[q4], s[q4 >> 1][8 * (q4 & 1) + v]);
     }
-    const float mx = xor32_max(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]))) * c;
-    const float m_new = softmax_ref_max(m_i, mx, 1.0f);
-    const float mc = ref_shift(m_new, 1.0f);
-    const float alpha = __builtin_amdgcn_exp2f(m_i - mc);
-    const float shift = kProbShift - mc;
+    const float mx = xor32_max(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
+    const float m_new = softmax_ref_max(m_i, mx, c);
+    const float ref = ref_shift(m_new, 1.0f);
+    const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * c);
+    float shift = kProbShift - ref * c;
+    if (decltype(masked)::value && any_far) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kb][v] -= far ? ref : 0.0f;
+      if (far) shift = kProbShift;
+    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -487,7 +520,7 @@ __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na
     float* ws = a.ws + ((int64_t)item * a.Hk + h) * part_floats(R, DH);
     const int r = row - r0;
     if (g == 0) {
-      ws[r] = m_i;
+      ws[r] = ref_exponent(m_i, c);
       ws[R + r] = l_i;
     }
     float* wo = ws + 2 * R + (int64_t)r * DH + 4 * g;

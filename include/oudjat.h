@@ -865,8 +865,8 @@ int oudjat_kv_nvfp4_read(const uint8_t* codes, int64_t c_bs, int64_t c_ns, int64
                          uint16_t* v_out, oudjat_stream_t stream);
 
 /* oudjat_packed_attention over an NVFP4 cache (sequence s in batch s, key_cap tokens each, keys[s] of them), with the
- * cached values as k and v. The probabilities are rounded to fp16 whatever the type of q and out. A query row with a NaN
- * or an infinity gives NaN where it sees a key. c_ns, s_ns < 2^24. Workspace of
+ * cached values as k and v. The probabilities are rounded to fp16 whatever the type of q and out, and the scores of a finite
+ * query row may be of any size. A query row with a NaN or an infinity gives NaN where it sees a key. c_ns, s_ns < 2^24. Workspace of
  * oudjat_packed_attention_nvfp4_workspace_elems fp32 elements as there. */
 int oudjat_packed_attention_nvfp4(const uint16_t* q, int64_t q_rs, int64_t q_hs, int64_t rows, int64_t Hq, int64_t Dh,
                                   const uint8_t* codes, int64_t c_bs, int64_t c_ns, int64_t c_cs, int64_t c_hs,
