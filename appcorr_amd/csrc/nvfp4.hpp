@@ -64,7 +64,7 @@ __device__ __forceinline__ void nvfp4_block_scale(float amax, float ts, uint32_t
 }
 
 // e2m1 codes of x_e / tot (IEEE quotient, e = 0..7) as one 32-bit word, element e in nibble e.
-// Quotient: Markstein's correction step. With y = RN(1 / tot) (one IEEE division per block),
+// Quotient: Markstein's correction step. With y = RN(1 / tot) (one IEEE division per block, or what equals it),
 // q0 = RN(x y) is within one ulp of x / tot, the remainder r = x - q0 tot is exact under an FMA,
 // and RN(q0 + r y) is the correctly rounded quotient (Markstein's theorem for round-to-nearest;
 // checked bitwise against IEEE division on 2.7e8 random pairs on gfx950, all-ones significands
