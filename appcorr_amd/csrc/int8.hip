@@ -477,17 +477,11 @@ extern "C" int oudjat_quantize_int8(const uint16_t* x, int64_t rows, int64_t K, 
   return check_launch(what);
 }
 
-// A launch holds less than 2^32 threads.
-static bool launch_holds(const Int8Gemm& g, int threads) {
-  return (int64_t)g.tiles_m * g.tiles_n * threads < (int64_t)1 << 32;
-}
-
 template <class E, int EPI, int BM, int BN, int WGM, int WGN, int NST>
 static int launch_tile(Int8Gemm g, hipStream_t st, const char* what) {
   static std::atomic<uint64_t> done{0};
   g.tiles_m = (int)cdiv(g.M, BM);
   g.tiles_n = (int)cdiv(g.N, BN);
-  if (!launch_holds(g, WGM * WGN * 64)) return set_error(OUDJAT_ERR_TOO_LARGE, "%s: too many tiles", what);
   constexpr int RB = BM / WGM % 32 ? 16 : 32;  // rows of a wave that the epilogue stages
   constexpr int lds = std::max(NST * (BM + BN) * 128, WGM * WGN * RB * (BN / WGN + 4) * 4);
   const auto fn = int8_tile_kernel<E, EPI, BM, BN, WGM, WGN, NST>;
@@ -501,7 +495,6 @@ template <class E, int EPI>
 static int launch_direct(Int8Gemm g, hipStream_t st, const char* what) {
   g.tiles_m = (int)cdiv(g.M, 16);
   g.tiles_n = (int)cdiv(g.N, 16);
-  if (!launch_holds(g, kDirectWaves * 64)) return set_error(OUDJAT_ERR_TOO_LARGE, "%s: too many tiles", what);
   int8_direct_kernel<E, EPI><<<(unsigned)g.tiles_m * g.tiles_n, kDirectWaves * 64, 0, st>>>(g);
   return check_launch(what);
 }
@@ -515,17 +508,21 @@ static int launch_direct(Int8Gemm g, hipStream_t st, const char* what) {
 //   1656 x 12288 x 4096: 1090 / 134 / 110 / 97 / 91 / 101;  16404 x 4096 x 8192: - / 833 / 671 / 547 / 504 / 499 (452 in
 //   two launches, below).
 struct Int8Tile {
-  int bm, bn;
+  int bm, bn, threads;
   float start, per_k, per_tile;
 };
 static const Int8Tile kInt8Tiles[] = {
-    {16, 16, 2.29f, 0.088f, 0.2f},   {64, 64, 2.27f, 0.189f, 0.91f}, {64, 128, 1.97f, 0.292f, 1.39f},
-    {128, 128, 2.5f, 0.479f, 2.39f}, {192, 256, 1.0f, 1.18f, 6.87f}, {256, 256, 1.0f, 1.346f, 9.13f},
+    {16, 16, kDirectWaves * 64, 2.29f, 0.088f, 0.2f}, {64, 64, 256, 2.27f, 0.189f, 0.91f},
+    {64, 128, 512, 1.97f, 0.292f, 1.39f},             {128, 128, 256, 2.5f, 0.479f, 2.39f},
+    {192, 256, 512, 1.0f, 1.18f, 6.87f},              {256, 256, 512, 1.0f, 1.346f, 9.13f},
 };
 static constexpr int kInt8Kinds = sizeof(kInt8Tiles) / sizeof(kInt8Tiles[0]);
 static constexpr int kInt8Large = 4;  // from here on a CU holds one tile at a time
+// (a launch holds less than 2^32 threads: a kernel that needs more is never the one)
+static constexpr float kInt8Never = 3.40282347e38f;
 static float int8_time(const Int8Tile& t, int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
+  if (tiles * t.threads >= (int64_t)1 << 32) return kInt8Never;
   return t.start + (float)cdiv(tiles, 256) * ((float)K / 128.0f * t.per_k + t.per_tile);
 }
 static int choose_int8(int64_t M, int64_t N, int64_t K, float& least) {
@@ -544,13 +541,17 @@ static int choose_int8(int64_t M, int64_t N, int64_t K, float& least) {
 // 1300 rows, 4096 x 4096: 39 us, in one launch 33). us in one launch and in two: 4116 x 4096 x 4096: 84, 68;
 // 16404 x 1024 x 1024: 34, 28; 4600 x 4096 x 8192: 159, 139; 16404 x 4096 x 8192: 493, 452; 33000 x 4096 x 1024: 201, 197;
 // 16404 x 8192 x 4096: 506, 499; not taken, by the twentieth: 5000 x 8192 x 8192: 288, 282; 1656 x 12288 x 4096: 88, 89.
+static bool int8_size(int64_t M, int64_t N) {
+  return M < (1 << 30) && N < (1 << 30) && cdiv(M, 16) * cdiv(N, 16) < (int64_t)1 << 31;
+}
 struct Int8Plan {
   int tile, rest;
   int64_t first;  // rows of the first launch
 };
-static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K) {
+static bool plan_int8(int64_t M, int64_t N, int64_t K, Int8Plan& p) {  // false: no kernel's launch holds the call
   float least, rest_us;
-  Int8Plan p{choose_int8(M, N, K, least), 0, M};
+  p = Int8Plan{choose_int8(M, N, K, least), 0, M};
+  if (least == kInt8Never) return false;
   const float again = (float)N * (float)K / 5e6f;  // the weight at 5 TB/s
   least *= 0.95f;
   for (int i = kInt8Large; i < kInt8Kinds; ++i) {
@@ -562,7 +563,7 @@ static Int8Plan plan_int8(int64_t M, int64_t N, int64_t K) {
     const float us = int8_time(t, first, N, K) + again + rest_us;
     if (us < least) least = us, p = Int8Plan{i, rest, first};
   }
-  return p;
+  return true;
 }
 
 template <class E, int EPI>
@@ -578,7 +579,8 @@ static int launch_one(int tile, const Int8Gemm& g, hipStream_t st, const char* w
 }
 template <class E, int EPI>
 static int launch_int8(Int8Gemm g, hipStream_t st, const char* what) {
-  const Int8Plan p = plan_int8(g.M, g.N, g.K);
+  Int8Plan p;
+  if (!plan_int8(g.M, g.N, g.K, p)) return set_error(OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   const int rest = g.M - (int)p.first;
   g.M = (int)p.first;
   const int rc = launch_one<E, EPI>(p.tile, g, st, what);
@@ -594,7 +596,8 @@ static int launch_int8(Int8Gemm g, hipStream_t st, const char* what) {
 extern "C" int oudjat_linear_int8_tile(int64_t M, int64_t N, int64_t K, int* rows, int* columns, int64_t* first) {
   const char* what = "linear_int8_tile";
   OUDJAT_REQUIRE(M > 0 && N > 0 && K > 0 && rows && columns && first, OUDJAT_ERR_INVALID_ARGUMENT, "%s: bad argument", what);
-  const Int8Plan p = plan_int8(M, N, K);
+  Int8Plan p;
+  OUDJAT_REQUIRE(int8_size(M, N) && plan_int8(M, N, K, p), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   *rows = kInt8Tiles[p.tile].bm;
   *columns = kInt8Tiles[p.tile].bn;
   *first = p.first;
@@ -628,9 +631,7 @@ extern "C" int oudjat_linear_int8(const int8_t* A, int64_t M, int64_t K, int64_t
                  OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: 16-byte aligned operands and rows required", what);
   OUDJAT_REQUIRE(entries_apart({{M, ldc}}, N), OUDJAT_ERR_UNSUPPORTED_LAYOUT, "%s: the rows of the output must not overlap",
                  what);
-  OUDJAT_REQUIRE(M < (1 << 30) && N < (1 << 30) && lda < (1 << 22) && ldw < (1 << 22) &&
-                     cdiv(M, 16) * cdiv(N, 16) < ((int64_t)1 << 31),
-                 OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
+  OUDJAT_REQUIRE(int8_size(M, N) && lda < (1 << 22) && ldw < (1 << 22), OUDJAT_ERR_TOO_LARGE, "%s: too large", what);
   const Int8Gemm g{A, lda, a_scale, W, ldw, w_scale, bias, gamma, resid, ldr, C, ldc, (int)M, (int)N, (int)K, 0, 0};
   hipStream_t st = as_stream(stream);
   auto by_epi = [&](auto e) {

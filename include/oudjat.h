@@ -822,14 +822,16 @@ int64_t oudjat_packed_attention_workspace_elems(int64_t rows, int64_t S, int64_t
 /* Rows of x [rows, K] (row stride x_rs) in 8 bits: scale[r] = max |x[r]| / 127 (fp32), codes[r, i] = x[r, i] / scale[r] to the
  * nearest whole number, ties to even (IEEE quotient; 0 where the scale is 0). A row with a NaN or an infinity gets the
  * scale NaN and codes 0. The same for a weight [N, K]: a scale for each output channel. K % 16 == 0; 16-byte aligned
- * rows, those of codes (stride c_rs) apart from one another and from x. */
+ * rows, those of codes (stride c_rs) apart from one another and from x. Fewer than 2^26 rows (2^24 with K > 1024): a launch
+ * holds no more. */
 int oudjat_quantize_int8(const uint16_t* x, int64_t rows, int64_t K, int64_t x_rs, int dtype, int8_t* codes, int64_t c_rs,
                          float* scale, oudjat_stream_t stream);
 
 /* C[m, n] = epilogue((sum_k A[m, k] W[n, k]) (a_scale[m] w_scale[n]) + bias[n]) of int8 codes A [M, K], W [N, K], the sum
  * exact in int32. Epilogues OUDJAT_EPI_BIAS, _LS (times gamma[n]), _LS_RESID (resid[m, n] + that) and _SILU_MUL (y / (1 +
  * e^-y) resid[m, n]), in fp32 with one rounding at the end. bias (may be NULL), gamma, resid and C of type `dtype`. K % 64
- * == 0, K < 2^17, N % 8 == 0; 16-byte aligned operands and rows (a_scale: 4). The rows of C apart; C may be resid. */
+ * == 0, K < 2^17, N % 8 == 0; 16-byte aligned operands and rows (a_scale: 4). The rows of C apart; C may be resid. M and N below
+ * 2^30, fewer than 2^31 blocks of 16 x 16 outputs, lda and ldw below 2^22. */
 int oudjat_linear_int8(const int8_t* A, int64_t M, int64_t K, int64_t lda, const float* a_scale, const int8_t* W,
                        int64_t N, int64_t ldw, const float* w_scale, const uint16_t* bias, int epi,
                        const uint16_t* gamma, const uint16_t* resid, int64_t ldr, uint16_t* C, int64_t ldc, int dtype,
