@@ -252,10 +252,9 @@ __device__ __forceinline__ void store_row(uint16_t* p, const uint4& v) {
 template <class E, int EPI, int BM, int BN, int WGM, int WGN, int NST>
 __global__ __launch_bounds__(WGM * WGN * 64) void int8_tile_kernel(Int8Gemm g) {
   constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
-  constexpr int STAGE = (BM + BN) * 128, L = (BM + BN + 8 * NW - 1) / (8 * NW);
-  constexpr int LEAST = (BM + BN) / (8 * NW);  // loads of a tile that every wave has
-  static_assert(BM % 16 == 0 && BN % 16 == 0 && WM % 16 == 0 && WN % 16 == 0, "whole blocks");
-  static_assert(NST >= 2 && (NST - 1) * L < 64, "vmcnt range");
+  constexpr int STAGE = (BM + BN) * 128, L = (BM + BN) / (8 * NW);  // a wave's loads of a tile
+  static_assert(WM % 16 == 0 && WN % 16 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole blocks and loads");
+  static_assert(NST >= 2 && NST <= 4 && (NST - 1) * L < 64, "wait_tiles, vmcnt range");
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 63, l16 = lane & 15, G = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -277,13 +276,8 @@ __global__ __launch_bounds__(WGM * WGN * 64) void int8_tile_kernel(Int8Gemm g) {
   auto load = [&](int kt, int i) __attribute__((always_inline)) {  // load i of L: rows of A, then of W
     unsigned char* st = smem + (kt % NST) * STAGE + (i * NW + wave) * 1024;
     const uint32_t k0 = (uint32_t)kt * 128u;
-    const uint32_t oa = va + (uint32_t)(i * 8 * NW) * (uint32_t)g.lda + k0;
-    if ((i + 1) * 8 * NW > BM + BN && i * 8 * NW + 8 * wave >= BM + BN) return;
-    const uint32_t ow = vw + (uint32_t)(i * 8 * NW - BM) * (uint32_t)g.ldw + k0;
-    if ((i + 1) * 8 * NW <= BM) buffer_load_lds16(ra, st, oa);
-    else if (i * 8 * NW >= BM) buffer_load_lds16(rw, st, ow);
-    else if (i * 8 * NW + 8 * wave < BM) buffer_load_lds16(ra, st, oa);
-    else buffer_load_lds16(rw, st, ow);
+    if (i * 8 * NW < BM) buffer_load_lds16(ra, st, va + (uint32_t)(i * 8 * NW) * (uint32_t)g.lda + k0);
+    else buffer_load_lds16(rw, st, vw + (uint32_t)(i * 8 * NW - BM) * (uint32_t)g.ldw + k0);
   };
 
   struct Frags {
@@ -329,13 +323,12 @@ __global__ __launch_bounds__(WGM * WGN * 64) void int8_tile_kernel(Int8Gemm g) {
   using Yes = std::true_type;
   using No = std::false_type;
   const int KT = (g.K + 127) / 128;
-  auto wait_tiles = [&](int n) __attribute__((always_inline)) {  // the loads of n tiles may stay in flight
+  auto wait_tiles = [&](int n) __attribute__((always_inline)) {  // the loads of n tiles, NST - 2 at most, may stay in flight
     if constexpr (NST > 3) {
-      if (n >= 3) return wait_vmcnt<(NST > 4 ? 3 : 2) * LEAST>();
+      if (n >= 2) return wait_vmcnt<2 * L>();
     }
     if constexpr (NST > 2) {
-      if (n == 2) return wait_vmcnt<(NST > 3 ? 2 : 1) * LEAST>();
-      if (n == 1) return wait_vmcnt<LEAST>();
+      if (n >= 1) return wait_vmcnt<L>();
     }
     wait_vmcnt<0>();
   };
