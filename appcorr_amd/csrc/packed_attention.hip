@@ -206,9 +206,9 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
       for (int v = 1; v < 8; ++v) mq[q4] = fmaxf(mq[q4], s[q4 >> 1][8 * (q4 & 1) + v]);
     }
     const float mx = xor32_max(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
-    const float m_new = softmax_ref_max(m_i, mx, a.scale_log2);
-    const float mc = ref_shift(m_new, a.scale_log2);
-    const float alpha = __builtin_amdgcn_exp2f(fmaf(m_i, a.scale_log2, -mc));
+    const float m_new = softmax_ref_max(m_i, mx, a.scale_log2), ref = finite_ref(m_new);
+    const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * a.scale_log2);
+    const float mc = ref * a.scale_log2;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -466,9 +466,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
     float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
     mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mx = xor32_max(xor16_max(mx));
-    const float m_new = softmax_ref_max(m_i, mx, a.scale_log2);
-    const float mc = ref_shift(m_new, a.scale_log2);
-    const float alpha = __builtin_amdgcn_exp2f(fmaf(m_i, a.scale_log2, -mc));
+    const float m_new = softmax_ref_max(m_i, mx, a.scale_log2), ref = finite_ref(m_new);
+    const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * a.scale_log2);
+    const float mc = ref * a.scale_log2;
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], a.scale_log2, -mc));
@@ -566,10 +566,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
     mp[i] = park[i * WROWS + r];
     m = fmaxf(m, mp[i]);
   }
-  const float mc = ref_shift(m, a.scale_log2);
+  const float ref = finite_ref(m);
 #pragma unroll
   for (int i = 0; i < WAVES; ++i) {
-    const float f = __builtin_amdgcn_exp2f(fmaf(mp[i], a.scale_log2, -mc));
+    const float f = __builtin_amdgcn_exp2f((mp[i] - ref) * a.scale_log2);
     l = fmaf(park[i * WROWS + R + r], f, l);
     const float* src = park + i * WROWS + 2 * R + r * OROW + 8 * c;
 #pragma unroll

@@ -205,7 +205,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_key
     mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mx = xor32_max(xor16_max(mx));
     const float m_new = softmax_ref_max(m_i, mx, c);
-    const float ref = ref_shift(m_new, 1.0f);
+    const float ref = finite_ref(m_new);
     const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * c);
     float shift = kProbShift - ref * c;
     const bool far = fabsf(ref * c) > kFarScore;
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_key
     mp[i] = park[i * WROWS + r];
     m = fmaxf(m, mp[i]);
   }
-  const float mc = ref_shift(m, 1.0f);
+  const float mc = finite_ref(m);
 #pragma unroll
   for (int i = 0; i < WAVES; ++i) {
     const float f = __builtin_amdgcn_exp2f(mp[i] - mc);
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na
     }
     const float mx = xor32_max(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
     const float m_new = softmax_ref_max(m_i, mx, c);
-    const float ref = ref_shift(m_new, 1.0f);
+    const float ref = finite_ref(m_new);
     const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * c);
     float shift = kProbShift - ref * c;
     if (decltype(masked)::value && any_far) {

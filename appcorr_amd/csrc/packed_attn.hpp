@@ -291,8 +291,10 @@ __device__ __forceinline__ i16x4_t read_tr(const unsigned char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)p);
 }
 
-// exp2 arguments are finite or -inf: a reference of -inf (no key seen yet) is replaced by 0.
-__device__ __forceinline__ float ref_shift(float m, float scale_log2) { return m == -INFINITY ? 0.0f : m * scale_log2; }
+// exp2 arguments are finite or -inf: a reference of -inf (no key seen yet) is replaced by 0. References are compared by their
+// difference, before the factor: 2^(c (m - m)) is 1, where m c with its product rounded would be off by up to half an ulp of
+// it, once in every tile.
+__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // Merge of the key parts of the items whose tile was split (workgroups of the others leave at once). With
 // m = max_p m_p and f_p = 2^(c (m_p - m)): out = sum_p f_p o_p / sum_p f_p l_p; a part without a visible key has l_p = 0
@@ -335,8 +337,8 @@ __global__ __launch_bounds__(256) void packed_attn_merge_kernel(PackedAttn a) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (lp[u] != 0.0f) top = fmaxf(top, mp[u]);
-      const float tc = ref_shift(top, a.scale_log2);
-      const float keep = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
+      const float ref = finite_ref(top);
+      const float keep = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2);
       m = top;
       l *= keep;
 #pragma unroll
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(256) void packed_attn_merge_kernel(PackedAttn a) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (lp[u] != 0.0f) {
-          const float f = __builtin_amdgcn_exp2f(fmaf(mp[u], a.scale_log2, -tc));
+          const float f = __builtin_amdgcn_exp2f((mp[u] - ref) * a.scale_log2);
           l = fmaf(lp[u], f, l);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = fmaf(y[u][e >> 2][e & 3], f, x[e]);
@@ -353,9 +355,9 @@ __global__ __launch_bounds__(256) void packed_attn_merge_kernel(PackedAttn a) {
     if constexpr (PL > 1) {
 #pragma unroll
       for (int s = CPR; s < 64; s <<= 1) {
-        const float m2 = __shfl_xor(m, s, 64), top = fmaxf(m, m2), tc = ref_shift(top, a.scale_log2);
-        const float f = __builtin_amdgcn_exp2f(fmaf(m, a.scale_log2, -tc));
-        const float f2 = __builtin_amdgcn_exp2f(fmaf(m2, a.scale_log2, -tc));
+        const float m2 = __shfl_xor(m, s, 64), top = fmaxf(m, m2), ref = finite_ref(top);
+        const float f = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2);
+        const float f2 = __builtin_amdgcn_exp2f((m2 - ref) * a.scale_log2);
         m = top;
         l = l * f + __shfl_xor(l, s, 64) * f2;
 #pragma unroll
