@@ -45,6 +45,11 @@ __device__ __forceinline__ void split_nonfinite(i16x8_t& v, i16x8_t& plus, i16x8
     minus[e] = bad && (nan || (b & 0x8000)) ? (short)E::kOne : 0;
   }
 }
+// Whether a row has to be done again with its reference taken off the scores: one further out than kFarScore, or (from an
+// earlier one that was) a sum that is not finite.
+__device__ __forceinline__ bool far_row(float m, float l, float scale_log2) {
+  return (m > -INFINITY && fabsf(m * scale_log2) > kFarScore) || !(l < INFINITY);
+}
 template <class V>
 __device__ __forceinline__ V add_nonfinite(V o, V plus, V minus, int n) {
 #pragma unroll
@@ -72,7 +77,7 @@ __device__ __forceinline__ V add_nonfinite(V o, V plus, V minus, int n) {
 // 0 * inf = NaN in the second product. Only where a row came out non-finite is the item done again on a slow path
 // that takes such values out of the product and adds them to the rows that see them. So are, without a mask too, value
 // rows that lie closer than a row (one value for all keys, a cache of one token): the descriptor of a sequence's last
-// tile shows visible values again behind the last key.
+// tile shows visible values again behind the last key. And so are items with a row whose scores are far (kFarScore).
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int W>
 __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn a) {
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
       for (int ks = 1; ks < QK_STEPS; ++ks) sc.s[kb] = E::mfma32(kf[ks], qf[ks], sc.s[kb]);
     }
   };
-  // MODE 0: no key of the tile is hidden from any row; 1: some may be; 2: and values may be non-finite.
+  // MODE 0: no key of the tile is hidden from any row; 1: some may be; 2: and values may be non-finite, or scores far.
   auto finish = [&](Scores& sc, const unsigned char* st, int t, auto mode) __attribute__((always_inline)) {
     constexpr int MODE = decltype(mode)::value;
     f32x16_t (&s)[2] = sc.s;
@@ -208,7 +213,15 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
     const float mx = xor32_max(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
     const float m_new = softmax_ref_max(m_i, mx, a.scale_log2), ref = finite_ref(m_new);
     const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * a.scale_log2);
-    const float mc = ref * a.scale_log2;
+    float mc = ref * a.scale_log2;
+    if constexpr (MODE == 2) {
+      const bool far = fabsf(mc) > kFarScore;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kb][v] -= far ? ref : 0.0f;
+      mc = far ? 0.0f : mc;
+    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -294,31 +307,31 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
     block_barrier();
     if (active) pipeline(std::true_type{});
     else pipeline(std::false_type{});
+    float z = far_row(m_i, l_i, a.scale_log2) ? 1.0f : 0.0f;
     if ((a.causal || a.values_overlap) && (tb + ntiles) * kKeyTile > lim_tile) {  // keys were hidden
-      float z = 0.0f;
 #pragma unroll
       for (int d = 0; d < OB; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) z = fmaf(o[d][v], 0.0f, z);
-      if (__syncthreads_or(mine && z != 0.0f)) {
-        rewind();
-        m_i = -INFINITY;
-        l_i = 0.0f;
+    }
+    if (__syncthreads_or(mine && z != 0.0f)) {
+      rewind();
+      m_i = -INFINITY;
+      l_i = 0.0f;
 #pragma unroll
-        for (int d = 0; d < OB; ++d)
+      for (int d = 0; d < OB; ++d)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+        for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
 #pragma unroll 1
-        for (int t = 0; t < ntiles; ++t) {
-          __syncthreads();
-          issue(0);
-          wait_vmcnt<0>();
-          __syncthreads();
-          if ((tb + t) * kKeyTile < kend_wave) {
-            Scores sc;
-            scores(sc, smem);
-            finish(sc, smem, t, I2{});
-          }
+      for (int t = 0; t < ntiles; ++t) {
+        __syncthreads();
+        issue(0);
+        wait_vmcnt<0>();
+        __syncthreads();
+        if ((tb + t) * kKeyTile < kend_wave) {
+          Scores sc;
+          scores(sc, smem);
+          finish(sc, smem, t, I2{});
         }
       }
     }
@@ -455,7 +468,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
     }
   };
   v8 pf;
-  auto softmax = [&](int key0) __attribute__((always_inline)) {
+  auto softmax = [&](int key0, auto safe) __attribute__((always_inline)) {
     if (key0 + KEYS > lim_tile) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -468,7 +481,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
     mx = xor32_max(xor16_max(mx));
     const float m_new = softmax_ref_max(m_i, mx, a.scale_log2), ref = finite_ref(m_new);
     const float alpha = __builtin_amdgcn_exp2f((m_i - ref) * a.scale_log2);
-    const float mc = ref * a.scale_log2;
+    float mc = ref * a.scale_log2;
+    if constexpr (decltype(safe)::value) {
+      const bool far = fabsf(mc) > kFarScore;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] -= far ? ref : 0.0f;
+      mc = far ? 0.0f : mc;
+    }
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], a.scale_log2, -mc));
@@ -513,7 +532,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
       reads_done();
       issue(kring, kbase, a.k_rs, t + NS);
     }
-    softmax(key_of(t));
+    softmax(key_of(t), std::false_type{});
     wait_loads(ahead + (t + NS < cnt ? 1 : 0));
     values(vring + (t % NS) * TILEB, std::false_type{});
     if (t + NS < cnt) {
@@ -523,24 +542,24 @@ __global__ __launch_bounds__(WAVES * 64, 2) void packed_attn_keys_kernel(PackedA
   }
   // Keys were hidden: see the rows kernel. The last tile of 32 loads keys past kend, which hide even where
   // all rows of the tile see the same keys (16 query heads of one key head: one token).
+  float z = far_row(m_i, l_i, a.scale_log2) ? 1.0f : 0.0f;
   if ((a.causal || a.values_overlap) && kfirst + n32 * KEYS > lim_tile) {
-    float z = 0.0f;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int v = 0; v < 4; ++v) z = fmaf(o[d][v], 0.0f, z);
-    if (__builtin_amdgcn_ballot_w64(mine && z != 0.0f)) {
-      reset();
+  }
+  if (__builtin_amdgcn_ballot_w64(mine && z != 0.0f)) {
+    reset();
 #pragma unroll 1
-      for (int t = 0; t < cnt; ++t) {
-        reads_done();
-        issue(kring, kbase, a.k_rs, t);
-        issue(vring, vbase, a.v_rs, t);
-        wait_loads(0);
-        scores(kring + (t % NS) * TILEB);
-        softmax(key_of(t));
-        values(vring + (t % NS) * TILEB, std::true_type{});
-      }
+    for (int t = 0; t < cnt; ++t) {
+      reads_done();
+      issue(kring, kbase, a.k_rs, t);
+      issue(vring, vbase, a.v_rs, t);
+      wait_loads(0);
+      scores(kring + (t % NS) * TILEB);
+      softmax(key_of(t), std::true_type{});
+      values(vring + (t % NS) * TILEB, std::true_type{});
     }
   }
 

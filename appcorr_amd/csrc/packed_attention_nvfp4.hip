@@ -32,7 +32,6 @@ static constexpr float kProbShift = 7.0f;
 // kernel looks at the reference in every tile; the rows kernel, where that costs 1 to 2 % at 64 dims, decides by the row's factor
 // alone (scaled queries are below 2^15 and x^ is at most 6 * 480: Dh = 128, query values of 100 against keys of 450 at the usual
 // scale are still near) and sends such rows through its masked tiles.
-static constexpr float kFarScore = 1048576.0f;
 template <int DH>
 __device__ __forceinline__ bool far_scores(float c) {
   return c > kFarScore / (DH * 32768.0f * 2880.0f);

@@ -296,6 +296,10 @@ __device__ __forceinline__ i16x4_t read_tr(const unsigned char* p) {
 // it, once in every tile.
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// A score further out than this (log2) is compared with its reference by difference too: the rounding of the reference's
+// product is whole exponents there (16 at 2^28), which gives infinite weights, or none at all.
+static constexpr float kFarScore = 1048576.0f;
+
 // Merge of the key parts of the items whose tile was split (workgroups of the others leave at once). With
 // m = max_p m_p and f_p = 2^(c (m_p - m)): out = sum_p f_p o_p / sum_p f_p l_p; a part without a visible key has l_p = 0
 // and is left out. DH / 8 lanes hold a row's dims; the other lanes of a wave take further parts of it (PL at a time,
