@@ -21,7 +21,7 @@ typedef int i32x4v_t __attribute__((ext_vector_type(4)));
 // Quotients are the IEEE ones: with y = RN(1 / s), q0 = RN(x y), r = x - q0 s (exact by an FMA), RN(q0 + r y) is the
 // correctly rounded quotient (Markstein); where s is so small that y overflows or r underflows, x and s are scaled by 2^100 first.
 // Adding 1.5 2^23 leaves the nearest whole number (ties to even) in the low byte.
-// Bound by HBM: 16404 rows of 8192 in 62 to 73 us (5.5 TB/s and more, VALU 68 % busy), 1656 of 4096 in 7.2; few rows by a launch
+// Bound by HBM: 16404 rows of 8192 in 60 to 73 us (5.5 TB/s and more, VALU 74 % busy), 1656 of 4096 in 7.2; few rows by a launch
 // and a round of loads (2.2 to 3.4).
 // ------------------------------------------------------------------------------------------------
 struct QuantRow {
@@ -227,10 +227,13 @@ __global__ __launch_bounds__(kDirectWaves * 64) void int8_direct_kernel(Int8Gemm
   if (m0 + l16 < g.M && n0 + 4 * G < g.N) int8_store4<E, EPI>(g, m0 + l16, n0 + 4 * G, acc);
 }
 
-// Eight outputs of a tile. Large tiles store past the caches, which then keep the operands that other tiles read: with the
-// quantiser that reads the output next, 16404 x 8192 x 4096: 563 -> 546 us (the product alone 493 -> 456), 4176 x 4096 x 1024: 42 ->
-// 40, 16404 x 4096 x 4096 and 1656 x 8192 x 4096: the same. Small tiles make outputs that are still in the caches when they are
-// read (40 x 4096 x 4096: 12.9, past them 13.2).
+// Eight outputs of a tile. Large tiles store past the caches, which then keep the operands that other tiles read. Us of the
+// product alone, through the caches -> past them, one card, both in turn: 16404 x 8192 x 4096 470 -> 460 (with a residual 533 ->
+// 514), 16404 x 4096 x 8192 437 -> 428 (474 -> 468), 16404 x 4096 x 4096 241 -> 237 (269 -> 249), 4176 x 4096 x 1024 29.6 -> 26.9,
+// 1656 x 12288 x 4096 86.6 -> 85.2; in place of the residual, whose lines the caches hold: the same. What reads the output next
+// gives some of it back: with a quantiser behind it, 570 -> 550 (with a residual 619 -> 634), 479 -> 481 (514 -> 510), 269 -> 272
+// (306 -> 312), 39.8 -> 38.7, 99 -> 100. Small tiles make outputs that are still in the caches when they are read (40 x 4096 x 4096
+// with the quantiser: 12.9, past them 13.2).
 template <bool PAST>
 __device__ __forceinline__ void store_row(uint16_t* p, const uint4& v) {
   typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -246,9 +249,10 @@ __device__ __forceinline__ void store_row(uint16_t* p, const uint4& v) {
 // barrier in the middle of the tile says that all waves have read it, so that the loads of the K tile NST further on may
 // go to its stage, and that the next tile has landed.
 // 256 x 256: eight waves of 128 x 64, two on a SIMD (four of 128 x 128 with twice the accumulators need both register files,
-// and moves between them: 571 us against 433 at 8192^3). 8192^3: 433 us, 2540 TOP/s at 1.9 GHz, matrix cores busy 65 %
-// (the library's product 1897 TOP/s there, 2335 at 16384^3). Small tiles are bound by their fragments' way through
-// LDS and by the two rounds of its latency in each K tile, which deeper stages do not shorten.
+// and moves between them: 571 us against 433 at 8192^3). 8192^3: 417 to 466 us by the card, 2635 TOP/s at best, matrix cores
+// busy 65 % (the library's product 1824 TOP/s on the card of the 417, 2347 at 16384^3).
+// Small tiles are bound by their fragments' way through LDS and by the two rounds of its latency in each K tile, which
+// deeper stages do not shorten.
 template <class E, int EPI, int BM, int BN, int WGM, int WGN, int NST>
 __global__ __launch_bounds__(WGM * WGN * 64) void int8_tile_kernel(Int8Gemm g) {
   constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
@@ -500,7 +504,7 @@ static int launch_direct(Int8Gemm g, hipStream_t st, const char* what) {
 //   1 x 4096 x 4096: 5.9 / 9.4 / 12 / 21 / 28 / 30;  32 x 8192 x 4096: 17 / 9.8 / 13 / 22 / 28 / 30;
 //   512 x 4096 x 4096: 114 / 16 / 14 / 25 / 40 / 47;  1656 x 4096 x 8192: 727 / 90 / 78 / 60 / 76 / 87;
 //   1656 x 12288 x 4096: 1090 / 134 / 110 / 97 / 91 / 101;  16404 x 4096 x 8192: - / 833 / 671 / 547 / 504 / 499 (452 in
-//   two launches, below).
+//   two launches, below). These and the figures of splits below were taken when all tiles stored through the caches.
 struct Int8Tile {
   int bm, bn, threads;
   float start, per_k, per_tile;

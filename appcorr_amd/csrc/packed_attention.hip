@@ -24,8 +24,8 @@
 //
 // Two kernels. packed_attn_rows: R = 32 W rows, a wave owns 32, all waves of the workgroup share K/V tiles of 64 keys.
 // packed_attn_keys, for few rows: R = 16, the waves share the rows and take 32 keys each in turn. Measured:
-// prompts of up to 16384 tokens, 32 over 8 heads of 128, 3.32 to 3.52 ms by the card (977 to 1040 TF/s; a 16384^3 product
-// of the library 1360); 32 tokens over caches of up to 16385 keys 155 us (5.0 TB/s); 24 crops of up to 1029 tokens, 16
+// prompts of up to 16384 tokens, 32 over 8 heads of 128, 3.13 to 3.18 ms (1082 to 1101 TF/s; a 16384^3 product of the
+// library 1649 on that card); 32 tokens over caches of up to 16385 keys 155 us (5.0 TB/s); 24 crops of up to 1029 tokens, 16
 // heads of 64, 43 us on a GPU that is busy, 47 on one that was idle. The steps' figures below were taken one against the
 // other on one card.
 #include "packed_attn.hpp"
@@ -371,7 +371,8 @@ __global__ __launch_bounds__(W * 64, 2) void packed_attn_rows_kernel(PackedAttn 
 // Keys kernel, for sequences of few packed rows (single tokens): 16 rows per workgroup, whose waves take 32 keys each
 // in turn through rings of their own in LDS (two tiles of K and two of V, each refilled as soon as it is read), so that
 // no barrier holds a wave and the loads of a CU (up to 96 KB) are never drained; the waves' results meet in LDS at the
-// end. Bound by reading K and V once: 512 tokens over 1000 keys each, 32 over 8 heads of 128, 370 us, 5.7 TB/s.
+// end. Bound by reading K and V once: 512 tokens over 1000 keys each, 32 over 8 heads of 128, 370 to 383 us
+// by the card, 5.7 to 5.5 TB/s.
 // S^T per 16-key block on v_mfma_f32_16x16x32 (lane l, G = l / 16: keys 4 G + v of row l % 16), O^T per 16 dims
 // (keys 4 G + {0..3} and 16 + 4 G + {0..3} per lane, V^T by the transposing LDS read).
 // ------------------------------------------------------------------------------------------------

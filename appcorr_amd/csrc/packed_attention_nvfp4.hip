@@ -100,9 +100,10 @@ __device__ __forceinline__ float load_query(const uint16_t* p, int step, h8_t* q
 // scales into registers, a tile ahead. Keys go from there to the first product (both of whose operands permute the
 // dims alike: lane group G has dims G Dh / 4 ..), values through LDS in fp16, from where the transposing reads take
 // them. Bound by reading the cache where there are enough waves: 512 tokens over 1000 keys each, 32 over 8 heads of 128,
-// 121 us (4.9 TB/s, a copy's rate; over a 16-bit cache 370). About 250 VALU instructions a tile of 32 keys, half of them the
-// turning into fp16, are half of the SIMDs' cycles; a tile's chain (products, maximum, exponentials, products) is hidden
-// by four waves a SIMD, for which the registers are stated (three: 126 us, two: 147).
+// 121 to 125 us by the card (4.9 TB/s, a copy's rate; over a 16-bit cache 370 to 383).
+// About 250 VALU instructions a tile of 32 keys, half of them the turning into fp16, are half of the SIMDs' cycles; a tile's
+// chain (products, maximum, exponentials, products) is hidden by four waves a SIMD, for which the registers are stated
+// (three: 126 us, two: 147).
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_keys_kernel(Nvfp4Attn na) {
@@ -306,11 +307,12 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 4 : 2) void nvfp4_attn_key
 // K . Q^T and O^T += V^T . P^T on v_mfma_f32_32x32x16 as in packed_attention.hip: a row is one lane pair (l, l ^ 32), whose
 // registers hold its scores. A thread turns pieces of 32 dims (16 bytes of codes, two scales) into fp16 once for the
 // workgroup; a piece is loaded two tiles ahead and written one tile ahead, between the first product and the softmax of
-// the tile before. 16 lanes write the same dims of 16 keys, which covers all banks. Bound by the softmax's VALU work (its
-// exponentials alone are half of it) and the matrix cores, as over a 16-bit cache: one prompt of 8192 tokens, 32 over 8
-// heads of 128, 542 us (1015 TF/s); of 4101, 16 heads of 64, 71 us, where 528 workgroups of different lengths leave CUs
-// idle at the end (every other round of them backwards: 8 % faster to 10 % slower by the lengths). A block's
-// fragments all read before its products: the same at 64 dims, 4 % slower at 128.
+// the tile before. 16 lanes write the same dims of 16 keys, which covers all banks. Neither the VALU nor the matrix cores are
+// busy all the time, since a wave's softmax and products wait for one another and two waves a SIMD cover a part of it: 49 and 42 %
+// of the SIMD cycles in one prompt of 8192 tokens, 32 over 8 heads of 128, 541 to 564 us by the card (1017 to 975 TF/s); 50 and
+// 22 % in four prompts of up to 4101, 16 heads of 64; one of 4101 73 us, where 528 workgroups of different lengths leave CUs idle
+// at the end (every other round of them backwards: 8 % faster to 10 % slower by the lengths). A block's fragments all read
+// before its products: the same at 64 dims, 4 % slower at 128.
 // ------------------------------------------------------------------------------------------------
 template <class E, int DH, int W>
 __global__ __launch_bounds__(W * 64, 2) void nvfp4_attn_rows_kernel(Nvfp4Attn na) {
